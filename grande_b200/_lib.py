@@ -64,10 +64,50 @@ class LayaSeqC(C.Structure):
     ]
 
 
+class PagedCacheC(C.Structure):
+    # omg_paged_cache
+    _fields_ = [
+        ("rows", C.c_void_p), ("n_pages", C.c_int64), ("page_rows", C.c_int32),
+        ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("dtype", C.c_int32),
+    ]
+
+
+class PagedBatchC(C.Structure):
+    # omg_paged_batch
+    _fields_ = [
+        ("q_start", C.c_void_p), ("lens", C.c_void_p), ("pages", C.c_void_p),
+        ("group_start", C.c_void_p), ("prefix_lens", C.c_void_p), ("prefix_pages", C.c_void_p),
+        ("n_seqs", C.c_int32), ("n_groups", C.c_int32), ("max_pages", C.c_int32),
+        ("max_prefix_pages", C.c_int32),
+    ]
+
+
+class AppendArgsC(C.Structure):
+    # omg_append_args
+    _fields_ = [
+        ("qkv", C.c_void_p), ("qkv_stride", C.c_int64), ("qkv_dtype", C.c_int32),
+        ("tokens", C.c_int32), ("heads", C.c_int32), ("has_kv", C.c_int32),
+        ("q_out", C.c_void_p), ("q_stride", C.c_int64), ("q_norm", C.c_void_p),
+        ("k_norm", C.c_void_p), ("v_norm", C.c_int32), ("norm_offset", C.c_float),
+        ("eps", C.c_float), ("q_scale", C.c_float), ("inv_freq", C.c_void_p),
+        ("n_freq", C.c_int32),
+    ]
+
+
+class AttentionArgsC(C.Structure):
+    # omg_attention_args
+    _fields_ = [
+        ("q", C.c_void_p), ("q_stride", C.c_int64), ("out", C.c_void_p), ("out_stride", C.c_int64),
+        ("tokens", C.c_int32), ("heads", C.c_int32), ("window", C.c_int32), ("scale", C.c_float),
+    ]
+
+
 vp = C.c_void_p
 pp = C.POINTER(C.c_void_p)
 cs = C.c_char_p
 sz = C.c_size_t
+CacheP = C.POINTER(PagedCacheC)
+BatchP = C.POINTER(PagedBatchC)
 GroupP = C.POINTER(GroupC)
 BranchP = C.POINTER(Branch)
 
@@ -161,6 +201,10 @@ PROTOTYPES: dict[str, tuple] = {
     "omg_laya_record_event": (C.c_int, [vp, C.c_int]),
     "omg_laya_elapsed_ms": (C.c_int, [vp, C.c_int, C.c_int, f32p]),
     "omg_laya_destroy": (None, [vp]),
+    "omg_paged_attention_workspace": (sz, [C.c_int, CacheP, BatchP, C.c_int, C.c_int]),
+    "omg_paged_attention": (C.c_int, [C.c_int, CacheP, BatchP, C.POINTER(AttentionArgsC), vp, sz,
+                                      vp]),
+    "omg_paged_append": (C.c_int, [C.c_int, CacheP, BatchP, C.POINTER(AppendArgsC), vp]),
 }
 
 

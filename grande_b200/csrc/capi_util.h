@@ -58,3 +58,21 @@ int guarded(F&& f) {
 }  // namespace omg
 
 #define CUDA_TRY(expr) ::omg::cuda_check((expr), #expr, __FILE__, __LINE__)
+
+namespace omg {
+
+// Makes `device` current for the scope of a call and puts the caller's
+// current device back on every exit path.
+struct DeviceScope {
+  int prev = -1;
+  explicit DeviceScope(int device) {
+    CUDA_TRY(cudaGetDevice(&prev));
+    if (prev != device) CUDA_TRY(cudaSetDevice(device));
+  }
+  ~DeviceScope() {
+    int cur = -1;
+    if (prev >= 0 && cudaGetDevice(&cur) == cudaSuccess && cur != prev) cudaSetDevice(prev);
+  }
+};
+
+}  // namespace omg

@@ -69,20 +69,6 @@ __global__ void sum_slabs(const float* __restrict__ part, int splits, size_t sla
   }
 }
 
-// Makes `device` current for the scope of a call and puts the caller's
-// current device back on every exit path.
-struct DeviceScope {
-  int prev = -1;
-  explicit DeviceScope(int device) {
-    CUDA_TRY(cudaGetDevice(&prev));
-    if (prev != device) CUDA_TRY(cudaSetDevice(device));
-  }
-  ~DeviceScope() {
-    int cur = -1;
-    if (prev >= 0 && cudaGetDevice(&cur) == cudaSuccess && cur != prev) cudaSetDevice(prev);
-  }
-};
-
 }  // namespace
 }  // namespace omg
 

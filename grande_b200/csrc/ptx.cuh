@@ -193,6 +193,21 @@ __device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t adesc, uint64
       : "memory");
 }
 
+// umma_f16 that leaves the TMEM lanes set in `off` (lane i: bit i % 32 of
+// word i / 32) as they are.
+__device__ __forceinline__ void umma_f16_lanes(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc,
+                                               uint32_t idesc, uint32_t accumulate,
+                                               const uint32_t (&off)[4]) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(
+          tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(off[0]), "r"(off[1]), "r"(off[2]),
+      "r"(off[3])
+      : "memory");
+}
+
 // Arrive on `bar` once every MMA this thread issued so far has completed.
 __device__ __forceinline__ void umma_commit(uint64_t* bar) {
   asm volatile(
@@ -293,6 +308,11 @@ __host__ __device__ constexpr uint32_t idesc_f16_f32(int M, int N) {
          | (0u << 7) | (0u << 10)                    // A, B format f16
          | (static_cast<uint32_t>(N >> 3) << 17)     // N / 8
          | (static_cast<uint32_t>(M >> 4) << 24);    // M / 16
+}
+
+// Both operands bf16 instead.
+__host__ __device__ constexpr uint32_t idesc_bf16(uint32_t idesc) {
+  return idesc | (1u << 7) | (1u << 10);
 }
 
 // The same with B MN-major (B stored [K][N], N contiguous).

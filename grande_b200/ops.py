@@ -1,0 +1,259 @@
+"""Operators on device memory: a K/V cache in pages, attention over it, and
+sampling, for programs that keep many states and branches in HBM at once and
+let branches answer in tokens (the engine keeps one prefix resident and reads
+whole rows back, crates/omg-wgpu/src/engine.rs:1942-2150).
+
+Tensors are torch tensors on one GPU. A call launches on that device's
+current torch stream and returns without waiting; lengths, page tables and
+per-row settings are read on the device when the kernels run, so a captured
+graph follows them. What the host can see is checked before the launch and
+refused with :class:`OmgError`; :meth:`PagedBatch.validate` reads the tables
+back and checks those too.
+
+A step of a batch of branches::
+
+    q = paged_append(qkv, cache, batch, heads=8, q_norm=qn, k_norm=kn,
+                     inv_freq=rope_frequencies(1e6, 256), q_scale=scale)
+    out = paged_attention(q, cache, batch, window=512)
+    ...
+    tokens, probs = sample(logits, uniforms, top_k=64, top_p=0.95)
+"""
+from __future__ import annotations
+
+import ctypes as C
+from dataclasses import dataclass, field
+from typing import Optional
+
+import numpy as np
+import torch
+
+from . import _lib
+from ._lib import OmgError, check, lib
+
+_TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+
+
+def _fail(msg: str):
+    raise OmgError(msg)
+
+
+def _table(t, name: str, shape: tuple, device):
+    if t.dtype != torch.int32 or t.device != device or not t.is_contiguous():
+        _fail(f"PagedBatch: {name} must be a contiguous int32 tensor on {device}")
+    if t.dim() != len(shape) or any(s is not None and s != n for s, n in zip(shape, t.shape)):
+        want = ", ".join("*" if s is None else str(s) for s in shape)
+        _fail(f"PagedBatch: {name} is {list(t.shape)}, expected [{want}]")
+
+
+@dataclass(frozen=True)
+class PagedBatch:
+    """The sequences of a call and where their tokens live (int32 tensors).
+
+    Sequence s has query rows ``q_start[s]:q_start[s + 1]`` and ``lens[s]``
+    own tokens, the query rows' own included and last, in the pages
+    ``pages[s]`` (own token i on page ``i // page``, row ``i % page``). Group g
+    is the sequences ``group_start[g]:group_start[g + 1]`` and the
+    ``prefix_lens[g]`` tokens before them in ``prefix_pages[g]``; without the
+    three group tensors there are no prefixes. Query rows past the last
+    sequence are padding and stay as they were. The tables are read when the
+    kernels run: write a step's lengths into the tensors in place."""
+    q_start: torch.Tensor
+    lens: torch.Tensor
+    pages: torch.Tensor
+    group_start: Optional[torch.Tensor] = None
+    prefix_lens: Optional[torch.Tensor] = None
+    prefix_pages: Optional[torch.Tensor] = None
+    _c: object = field(init=False, repr=False, compare=False, default=None)
+
+    def __post_init__(self):
+        dev = self.q_start.device
+        n = self.lens.numel()
+        _table(self.lens, "lens", (None,), dev)
+        _table(self.q_start, "q_start", (n + 1,), dev)
+        _table(self.pages, "pages", (n, None), dev)
+        groups = (self.group_start, self.prefix_lens, self.prefix_pages)
+        g = pp = 0
+        if any(t is not None for t in groups):
+            if any(t is None for t in groups):
+                _fail("PagedBatch: group_start, prefix_lens and prefix_pages go together")
+            g = self.prefix_lens.numel()
+            _table(self.prefix_lens, "prefix_lens", (None,), dev)
+            _table(self.group_start, "group_start", (g + 1,), dev)
+            _table(self.prefix_pages, "prefix_pages", (g, None), dev)
+            pp = self.prefix_pages.shape[1]
+        ptr = [t.data_ptr() if t is not None and t.numel() else None
+               for t in (self.q_start, self.lens, self.pages) + groups]
+        object.__setattr__(self, "_c", _lib.PagedBatchC(*ptr, n, g, self.pages.shape[1], pp))
+
+    def validate(self, cache: torch.Tensor, tokens: int):
+        """Read the tables back (this waits for the device) and raise on the
+        first thing a call over ``cache`` with ``tokens`` query rows could not
+        honour: rows out of order, lengths below the query rows' or beyond the
+        tables, pages outside the pool, a page appended to twice."""
+        n_pages, page = cache.shape[0], cache.shape[1]
+        q, lens, pages = (t.cpu().numpy().astype(np.int64)
+                          for t in (self.q_start, self.lens, self.pages))
+        new = np.diff(q)
+        if q[0] < 0 or (new < 0).any() or q[-1] > tokens:
+            _fail(f"PagedBatch: q_start must ascend within 0..{tokens}")
+        self._lengths("sequence", lens, pages, page, n_pages)
+        for s in np.flatnonzero(lens < new):
+            _fail(f"PagedBatch: sequence {s} has {lens[s]} tokens, {new[s]} of them new")
+        writes = [pages[s, i] for s in np.flatnonzero(new > 0)
+                  for i in range((lens[s] - new[s]) // page, -(-lens[s] // page))]
+        if len(set(writes)) != len(writes):
+            _fail("PagedBatch: two sequences append to one page")
+        if self.group_start is not None:
+            gs, plens, ppages = (t.cpu().numpy().astype(np.int64) for t in
+                                 (self.group_start, self.prefix_lens, self.prefix_pages))
+            if gs[0] != 0 or (np.diff(gs) < 0).any() or gs[-1] != lens.size:
+                _fail(f"PagedBatch: group_start must ascend from 0 to {lens.size}")
+            self._lengths("prefix", plens, ppages, page, n_pages)
+
+    @staticmethod
+    def _lengths(what, lens, pages, page, n_pages):
+        for s, n in enumerate(lens):
+            used = -(-n // page)
+            if n < 0 or used > pages.shape[1]:
+                _fail(f"PagedBatch: {what} {s} has {n} tokens in {pages.shape[1]} pages of {page}")
+            bad = (pages[s, :used] < 0) | (pages[s, :used] >= n_pages)
+            if bad.any():
+                _fail(f"PagedBatch: {what} {s} uses page {pages[s, :used][bad][0]} of {n_pages}")
+
+
+def rope_frequencies(theta: float, head_dim: int, rope_dims: Optional[int] = None,
+                     scale: float = 1.0, device=None) -> torch.Tensor:
+    """theta^(-2 d / head_dim) / scale for the ``rope_dims // 2`` rotated pairs
+    (all of the head by default), in 64 bits: radians per position. ``scale``
+    stretches the positions (long contexts)."""
+    rope_dims = head_dim if rope_dims is None else rope_dims
+    if rope_dims < 0 or rope_dims > head_dim or rope_dims % 2:
+        _fail(f"rope_dims {rope_dims} for head_dim {head_dim}")
+    if not theta > 0 or not scale > 0:
+        _fail(f"rope theta {theta}, scale {scale}")
+    d = torch.arange(rope_dims // 2, dtype=torch.float64)
+    return (float(theta) ** (-2.0 * d / head_dim) / scale).to(device or "cuda")
+
+
+def _cache(op: str, cache: torch.Tensor, batch: PagedBatch) -> "_lib.PagedCacheC":
+    if cache.dim() != 5 or cache.shape[2] != 2 or not cache.is_contiguous():
+        _fail(f"{op}: the cache must be a contiguous [pages, page, 2, kv_heads, head_dim] tensor")
+    if cache.dtype not in (torch.float16, torch.bfloat16):
+        _fail(f"{op}: cache dtype {cache.dtype} (float16 or bfloat16)")
+    if cache.device.type != "cuda":
+        _fail(f"{op}: the cache must be on a GPU")
+    if batch.q_start.device != cache.device:
+        _fail(f"{op}: the batch is on {batch.q_start.device}, the cache on {cache.device}")
+    return _lib.PagedCacheC(cache.data_ptr(), cache.shape[0], cache.shape[1], cache.shape[3],
+                            cache.shape[4], _TYPES[cache.dtype])
+
+
+def _vector(op: str, t, name: str, n: int, dtype, device):
+    if t is None:
+        return None
+    if t.dtype != dtype or t.device != device or t.dim() != 1 or t.numel() != n or (
+            n > 1 and t.stride(0) != 1):
+        _fail(f"{op}: {name} must be {n} contiguous {dtype} values on {device}")
+    return t.data_ptr()
+
+
+def _out(op: str, out, shape, like: torch.Tensor):
+    if out is None:
+        return torch.empty(shape, dtype=like.dtype, device=like.device)
+    if tuple(out.shape) != tuple(shape) or out.dtype != like.dtype or out.device != like.device:
+        _fail(f"{op}: out must be {list(shape)} {like.dtype} on {like.device}")
+    return out
+
+
+def _rows(op: str, t: torch.Tensor, name: str):
+    """Row stride of [tokens, heads, head_dim] rows whose heads are packed."""
+    if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
+        _fail(f"{op}: the heads of {name} must be contiguous")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+
+
+def _stream(device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def paged_append(qkv: torch.Tensor, cache: torch.Tensor, batch: PagedBatch, *, heads: int,
+                 q_norm: Optional[torch.Tensor] = None, k_norm: Optional[torch.Tensor] = None,
+                 norm_offset: float = 0.0, eps: float = 1e-6, v_norm: bool = False,
+                 inv_freq: Optional[torch.Tensor] = None, q_scale: float = 1.0,
+                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Norm, rotate and store one projection's rows (qk_prep.wgsl, per head).
+
+    ``qkv`` [tokens, (heads + 2 kv_heads) * head_dim] holds each token's q, k
+    and v heads, or its q heads alone (a layer that reads another layer's
+    K/V), in f32 or the cache's type. q and k heads are RMS-normalised with
+    weights ``norm_offset + q_norm`` / ``k_norm`` (None: not), v heads without
+    weights when ``v_norm``; the pairs (d, d + head_dim / 2) of q and k are
+    rotated by position * inv_freq[d] (f64, :func:`rope_frequencies`). k and v
+    go to their cache rows, q times ``q_scale`` is returned
+    [tokens, heads, head_dim]."""
+    op = "paged_append"
+    c = _cache(op, cache, batch)
+    kvh, hd = c.kv_heads, c.head_dim
+    dev = cache.device
+    if qkv.device != dev or qkv.dtype not in (torch.float32, cache.dtype):
+        _fail(f"{op}: qkv must be float32 or {cache.dtype} on {dev}")
+    width = heads * hd
+    if qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.shape[1] not in (width, width + 2 * kvh * hd):
+        _fail(f"{op}: qkv is {list(qkv.shape)}, expected [tokens, {width + 2 * kvh * hd}] (q, k, v "
+              f"heads) or [tokens, {width}] (q heads), rows contiguous")
+    n = qkv.shape[0]
+    out = _out(op, out, (n, heads, hd), cache)
+    args = _lib.AppendArgsC(
+        qkv.data_ptr(), qkv.stride(0) if n > 1 else qkv.shape[1], _TYPES[qkv.dtype], n, heads,
+        int(qkv.shape[1] > width), out.data_ptr(), _rows(op, out, "out"),
+        _vector(op, q_norm, "q_norm", hd, torch.float32, dev),
+        _vector(op, k_norm, "k_norm", hd, torch.float32, dev), int(v_norm), norm_offset, eps,
+        q_scale,
+        _vector(op, inv_freq, "inv_freq", 0 if inv_freq is None else inv_freq.numel(),
+                torch.float64, dev),
+        0 if inv_freq is None else inv_freq.numel())
+    check(lib().omg_paged_append(dev.index, C.byref(c), C.byref(batch._c), C.byref(args),
+                                 _stream(dev)))
+    return out
+
+
+def paged_attention(q: torch.Tensor, cache: torch.Tensor, batch: PagedBatch, *,
+                    scale: float = 1.0, window: int = 0, out: Optional[torch.Tensor] = None,
+                    workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of query rows ``q`` [tokens, heads, head_dim] over the paged
+    cache: each row sees its group's prefix and its own sequence's keys up to
+    its own position, the last ``window`` of them if that is not 0. A prefix
+    is read once for all the sequences of its group. Rows that see nothing
+    are zero. ``workspace`` (uint8, :func:`paged_attention_workspace` bytes)
+    is allocated from torch's pool when not given."""
+    op = "paged_attention"
+    c = _cache(op, cache, batch)
+    dev = cache.device
+    if q.device != dev or q.dtype != cache.dtype or q.dim() != 3 or q.shape[2] != c.head_dim:
+        _fail(f"{op}: q is {list(q.shape)} {q.dtype} on {q.device}, expected [tokens, heads, "
+              f"{c.head_dim}] {cache.dtype} on {dev}")
+    n, heads = q.shape[0], q.shape[1]
+    out = _out(op, out, (n, heads, c.head_dim), q)
+    if workspace is None:
+        workspace = torch.empty(_workspace(dev, c, batch, n, heads), dtype=torch.uint8, device=dev)
+    elif workspace.device != dev or workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+        _fail(f"{op}: the workspace must be contiguous uint8 on {dev}")
+    args = _lib.AttentionArgsC(q.data_ptr(), _rows(op, q, "q"), out.data_ptr(),
+                               _rows(op, out, "out"), n, heads, window, scale)
+    check(lib().omg_paged_attention(dev.index, C.byref(c), C.byref(batch._c), C.byref(args),
+                                    workspace.data_ptr(), workspace.numel(), _stream(dev)))
+    return out
+
+
+def _workspace(dev, c, batch, tokens, heads) -> int:
+    n = lib().omg_paged_attention_workspace(dev.index, C.byref(c), C.byref(batch._c), tokens, heads)
+    return n if n else check(-1)
+
+
+def paged_attention_workspace(cache: torch.Tensor, batch: PagedBatch, tokens: int,
+                              heads: int) -> int:
+    """Workspace bytes of a :func:`paged_attention` call with ``tokens`` query
+    rows. Calls that may overlap (two streams, two captured graphs) need a
+    workspace each."""
+    return _workspace(cache.device, _cache("paged_attention_workspace", cache, batch), batch,
+                      tokens, heads)

@@ -467,6 +467,97 @@ int omg_gemm_splitk_noalloc(int device, const void* x_f16, int m, int k, int lda
                             const void* w_f16, int n, int splits, float* out, int ldo,
                             void* stream);
 
+
+/* ---- operators on device memory --------------------------------------------
+ * No counterpart in the reference, whose engine keeps one prefix resident in
+ * a contiguous cache and reads whole logits rows back. These serve programs
+ * that keep many states and branches in HBM at once and let branches answer
+ * in tokens: a K/V cache in pages, attention over it, sampling.
+ *
+ * Every pointer is device memory of the caller on `device`, `stream` a
+ * cudaStream_t or NULL. A call launches its kernels on `stream` and returns;
+ * it allocates nothing, synchronises nothing and may be captured into a CUDA
+ * graph: lengths, tables and settings are read on the device when the
+ * kernels run. The caller's current device is left as it was. What the host
+ * can see is checked and refused with an error before anything is launched;
+ * what sits in device tables is bounded by the kernels as stated below.
+ *
+ * Cache: a pool of pages, rows [n_pages][page_rows][2 * kv_heads * head_dim]
+ * (an engine cache row: K heads, then V heads), page_rows 16, 32, 64, 128 or
+ * 256, head_dim 64, 128, 256 or 512, f16 or bf16.
+ *
+ * Batch: sequence s has query rows q_start[s] .. q_start[s + 1] (ascending,
+ * possibly none) and lens[s] own tokens, the query rows' own included and
+ * last; own token i lives in row i % page_rows of page
+ * pages[s * max_pages + i / page_rows]. Group g is the sequences
+ * group_start[g] .. group_start[g + 1] and the prefix_lens[g] tokens before
+ * them, in pages prefix_pages[g * max_prefix_pages + ..]: own token i of a
+ * sequence is at position prefix_lens[g] + i. n_groups 0 (group arrays NULL):
+ * no prefixes. Query rows from q_start[n_seqs] on are padding and their
+ * outputs are left as they were. Lengths beyond a table's columns are cut
+ * there; page ids outside the pool are never read or written. */
+enum { OMG_TYPE_F16 = 0, OMG_TYPE_BF16 = 1, OMG_TYPE_F32 = 2 };
+
+typedef struct {
+  void* rows;
+  int64_t n_pages;
+  int32_t page_rows, kv_heads, head_dim, dtype;
+} omg_paged_cache;
+
+typedef struct {
+  const int32_t *q_start, *lens, *pages;
+  const int32_t *group_start, *prefix_lens, *prefix_pages;
+  int32_t n_seqs, n_groups, max_pages, max_prefix_pages;
+} omg_paged_batch;
+
+typedef struct {
+  const void* qkv;         /* [tokens] projection rows: q heads, k heads, v heads */
+  int64_t qkv_stride;      /* elements between rows, rows 16-byte aligned */
+  int32_t qkv_dtype;       /* F32, or the cache's dtype */
+  int32_t tokens, heads;
+  int32_t has_kv;          /* 0: rows hold q heads only and the cache is not touched */
+  void* q_out;             /* [tokens] rows of heads * head_dim in the cache's dtype */
+  int64_t q_stride;
+  const float *q_norm, *k_norm; /* [head_dim] or NULL (no norm) */
+  int32_t v_norm;
+  float norm_offset, eps, q_scale;
+  const double* inv_freq;  /* [n_freq] radians per position, or NULL */
+  int32_t n_freq;          /* rotated pairs (d, d + head_dim / 2), <= head_dim / 2 */
+} omg_append_args;
+
+/* The per-head norms, rotation and scaling of a fused projection row
+ * (qk_prep.wgsl), q to q_out, k and v to the token's cache row. A token
+ * whose row is outside its table or the pool gets its q row and no cache
+ * row. Two tokens of one batch given the same cache row race. */
+int omg_paged_append(int device, const omg_paged_cache* cache, const omg_paged_batch* batch,
+                     const omg_append_args* args, void* stream);
+
+typedef struct {
+  const void* q;       /* [tokens] rows of heads * head_dim in the cache's dtype */
+  int64_t q_stride;    /* elements between rows, rows 16-byte aligned */
+  void* out;           /* the same layout */
+  int64_t out_stride;
+  int32_t tokens, heads; /* heads a multiple of kv_heads, at most 128 per KV head */
+  int32_t window;      /* keys at positions > position - window only; 0: all */
+  float scale;         /* of the scores, > 0 */
+} omg_attention_args;
+
+/* Device workspace bytes of a call with these sizes (0: an error, e.g. more
+ * sequences and row tiles than a call takes). Two calls that may overlap, or
+ * two captured graphs that may, need a workspace each. */
+size_t omg_paged_attention_workspace(int device, const omg_paged_cache* cache,
+                                     const omg_paged_batch* batch, int tokens, int heads);
+
+/* Softmax attention of every query row over its group's prefix and its own
+ * sequence's keys up to its own position (attention.wgsl's visibility, over
+ * pages): a prefix is read once for all the sequences of its group. A row
+ * that sees no key gets zeros. Keys and values a row does not see never
+ * reach it, whatever they hold; a page id outside the pool reads as zeros.
+ * A row whose kernel gave up waiting (a bounded device wait) is NaN. */
+int omg_paged_attention(int device, const omg_paged_cache* cache, const omg_paged_batch* batch,
+                        const omg_attention_args* args, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
 #ifdef __cplusplus
 }
 #endif
