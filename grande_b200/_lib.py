@@ -102,6 +102,17 @@ class AttentionArgsC(C.Structure):
     ]
 
 
+class SampleArgsC(C.Structure):
+    # omg_sample_args
+    _fields_ = [
+        ("logits", C.c_void_p), ("stride", C.c_int64), ("dtype", C.c_int32), ("rows", C.c_int32),
+        ("vocab", C.c_int32), ("u", C.c_void_p), ("temperature", C.c_void_p),
+        ("top_k", C.c_void_p), ("top_p", C.c_void_p), ("min_p", C.c_void_p),
+        ("temperature_all", C.c_float), ("top_k_all", C.c_int32), ("top_p_all", C.c_float),
+        ("min_p_all", C.c_float), ("tokens", C.c_void_p), ("probs", C.c_void_p),
+    ]
+
+
 vp = C.c_void_p
 pp = C.POINTER(C.c_void_p)
 cs = C.c_char_p
@@ -204,6 +215,7 @@ PROTOTYPES: dict[str, tuple] = {
     "omg_paged_attention_workspace": (sz, [C.c_int, CacheP, BatchP, C.c_int, C.c_int]),
     "omg_paged_attention": (C.c_int, [C.c_int, CacheP, BatchP, C.POINTER(AttentionArgsC), vp, sz,
                                       vp]),
+    "omg_sample": (C.c_int, [C.c_int, C.POINTER(SampleArgsC), vp]),
     "omg_paged_append": (C.c_int, [C.c_int, CacheP, BatchP, C.POINTER(AppendArgsC), vp]),
 }
 

@@ -7,6 +7,7 @@
 #include "capi_util.h"
 #include "omg_b200.h"
 #include "paged.cuh"
+#include "sample.cuh"
 
 using namespace omg;
 
@@ -33,6 +34,7 @@ const DeviceInfo& device_info(int device) {
     CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
     DeviceScope on(device);
     paged_attention_setup_device();
+    sample_setup_device();
     CUDA_TRY(cudaGetLastError());
     d.sms = sms;
   }
@@ -227,6 +229,46 @@ int omg_paged_attention(int device, const omg_paged_cache* cache, const omg_page
     if (!paged_attention_maps(a, p->q, p->q_stride, &tq, &tkv, err, sizeof err))
       fail("%s: %s", op, err);
     launch_paged_attention(a, tq, tkv, static_cast<cudaStream_t>(stream));
+    CUDA_TRY(cudaGetLastError());
+    return 0;
+  });
+}
+
+int omg_sample(int device, const omg_sample_args* p, void* stream) {
+  return guarded([&]() -> int {
+    const char* op = "omg_sample";
+    check_device(op, device);
+    if (!p) fail("%s: args is null", op);
+    if (p->dtype != OMG_TYPE_F32 && p->dtype != OMG_TYPE_F16 && p->dtype != OMG_TYPE_BF16)
+      fail("%s: dtype %d", op, p->dtype);
+    SampleArgs a{};
+    a.dtype = p->dtype == OMG_TYPE_F32 ? kOpF32 : p->dtype == OMG_TYPE_F16 ? kOpF16 : kOpBf16;
+    if (p->rows < 0 || p->rows > (1 << 24)) fail("%s: %d rows", op, p->rows);
+    if (p->vocab < 1 || p->vocab > sample_max_vocab(a.dtype))
+      fail("%s: vocabulary of %d (1 to %d)", op, p->vocab, sample_max_vocab(a.dtype));
+    if (p->stride < p->vocab)
+      fail("%s: stride %lld < vocabulary %d", op, static_cast<long long>(p->stride), p->vocab);
+    if (p->rows == 0) return 0;
+    check_aligned(op, "logits", p->logits, p->dtype == OMG_TYPE_F32 ? 4 : 2);
+    check_aligned(op, "u", p->u, 4);
+    check_aligned(op, "tokens", p->tokens, 4);
+    a.logits = p->logits;
+    a.stride = p->stride;
+    a.rows = p->rows;
+    a.vocab = p->vocab;
+    a.u = p->u;
+    a.temperature = p->temperature;
+    a.top_k = p->top_k;
+    a.top_p = p->top_p;
+    a.min_p = p->min_p;
+    a.temperature1 = p->temperature_all;
+    a.top_k1 = p->top_k_all;
+    a.top_p1 = p->top_p_all;
+    a.min_p1 = p->min_p_all;
+    a.tokens = p->tokens;
+    a.probs = p->probs;
+    DeviceScope on(device);
+    launch_sample(a, device_info(device).sms, static_cast<cudaStream_t>(stream));
     CUDA_TRY(cudaGetLastError());
     return 0;
   });

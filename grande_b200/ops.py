@@ -257,3 +257,51 @@ def paged_attention_workspace(cache: torch.Tensor, batch: PagedBatch, tokens: in
     workspace each."""
     return _workspace(cache.device, _cache("paged_attention_workspace", cache, batch), batch,
                       tokens, heads)
+
+
+def _setting(op: str, v, name: str, n: int, dtype, device, off):
+    """(pointer, value): a tensor of one value per row, or one for all."""
+    if v is None:
+        return None, off
+    if isinstance(v, torch.Tensor):
+        return _vector(op, v, name, n, dtype, device), off
+    return None, v
+
+
+def sample(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature=None, top_k=None,
+           top_p=None, min_p=None, tokens: Optional[torch.Tensor] = None,
+           probs: Optional[torch.Tensor] = None):
+    """A token for each row of ``logits`` [rows, vocab] (f32, f16 or bf16) and
+    its probability in what the filters left: (tokens int32, probs f32).
+
+    ``uniforms`` [rows] f32 in [0, 1) decide the draw. ``temperature``,
+    ``top_k``, ``top_p`` and ``min_p`` are a number for all rows or a tensor
+    with one per row (int32 for top_k, f32 otherwise); None is off. The top_k
+    largest stay (equal logits by index), of those the fewest that hold top_p
+    of their probability, of those the ones at least min_p times as likely as
+    the likeliest. Temperature 0 takes the largest logit. A row of nothing but
+    -infinity and NaN gets token -1 and probability 0."""
+    op = "sample"
+    if logits.device.type != "cuda":
+        _fail(f"{op}: logits must be on a GPU")
+    dev = logits.device
+    if logits.dim() != 2 or logits.dtype not in _TYPES or (
+            logits.shape[1] > 1 and logits.stride(1) != 1):
+        _fail(f"{op}: logits must be [rows, vocab] float32, float16 or bfloat16, rows contiguous")
+    n, vocab = logits.shape
+    f32, i32 = torch.float32, torch.int32
+    if tokens is None:
+        tokens = torch.empty(n, dtype=i32, device=dev)
+    if probs is None:
+        probs = torch.empty(n, dtype=f32, device=dev)
+    temp = _setting(op, temperature, "temperature", n, f32, dev, 1.0)
+    k = _setting(op, top_k, "top_k", n, i32, dev, 0)
+    p = _setting(op, top_p, "top_p", n, f32, dev, 1.0)
+    m = _setting(op, min_p, "min_p", n, f32, dev, 0.0)
+    args = _lib.SampleArgsC(
+        logits.data_ptr(), logits.stride(0) if n > 1 else vocab, _TYPES[logits.dtype], n, vocab,
+        _vector(op, uniforms, "uniforms", n, f32, dev), temp[0], k[0], p[0], m[0], temp[1], k[1],
+        p[1], m[1], _vector(op, tokens, "tokens", n, i32, dev),
+        _vector(op, probs, "probs", n, f32, dev))
+    check(lib().omg_sample(dev.index, C.byref(args), _stream(dev)))
+    return tokens, probs

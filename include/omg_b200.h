@@ -558,6 +558,35 @@ int omg_paged_attention(int device, const omg_paged_cache* cache, const omg_page
                         const omg_attention_args* args, void* workspace, size_t workspace_bytes,
                         void* stream);
 
+typedef struct {
+  const void* logits;      /* [rows] rows of vocab values, any element alignment */
+  int64_t stride;          /* elements between rows */
+  int32_t dtype;           /* OMG_TYPE_* */
+  int32_t rows, vocab;     /* vocab up to 327,680 (f32) or 524,288 (f16, bf16) */
+  const float* u;          /* [rows] uniform numbers in [0, 1) */
+  /* [rows] settings, or NULL and the one value after them for every row. */
+  const float* temperature;
+  const int32_t* top_k;
+  const float *top_p, *min_p;
+  float temperature_all;
+  int32_t top_k_all;
+  float top_p_all, min_p_all;
+  int32_t* tokens;         /* [rows] */
+  float* probs;            /* [rows] or NULL */
+} omg_sample_args;
+
+/* A token for each logits row. With w_i = exp((x_i - max) / temperature), in
+ * the order of descending x (equal ones by ascending index): the first top_k
+ * are kept (0 or less: all); of those the shortest run whose w sums to at
+ * least top_p of their sum (1 or more: all; 0 or less: the first); of those
+ * the ones with w_i >= min_p (0 or less: all). The token is the first in
+ * index order whose running sum of kept w exceeds u times their sum, its
+ * probability that of the kept distribution. A temperature of 0 or less, or
+ * NaN: the largest logit, lowest index first, with probability 1. NaN logits
+ * count as -infinity; a row of nothing else gets token -1, probability 0.
+ * Weights are counted in units of 2^-44 of the largest. */
+int omg_sample(int device, const omg_sample_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -124,3 +124,27 @@ def append(qkv, cache, b, heads, qn, kn, offset, eps, v_norm, freq, q_scale):
                 row = int(b.pages[s][i // b.page]) * b.page + i % b.page
                 flat[row, 0], flat[row, 1] = rot(k[t]), v[t]
     return out, flat.reshape(cache.shape)
+
+
+def sample(x, u, temperature, top_k, top_p, min_p):
+    """(token, probability) of one row in 64 bits."""
+    x = np.where(np.isnan(x), -np.inf, x.astype(np.float64))
+    order = np.argsort(-x, kind="stable")
+    best = x[order[0]]
+    if best == -np.inf:
+        return -1, 0.0
+    if not temperature > 0 or top_p <= 0:
+        return int(order[0]), 1.0
+    with np.errstate(invalid="ignore", over="ignore"):
+        w = np.where(x == best, 1.0, np.exp((x - best) / np.float64(temperature)))
+    w = np.nan_to_num(w)
+    if top_k > 0:
+        order = order[:top_k]
+    if top_p < 1:
+        cum = np.cumsum(w[order])
+        order = order[:np.searchsorted(cum, np.float64(top_p) * cum[-1], side="left") + 1]
+    order = order[w[order] >= min(float(min_p), 1.0)]
+    kept = np.sort(order)
+    cum = np.cumsum(w[kept])
+    at = min(int(np.searchsorted(cum, np.float64(u) * cum[-1], side="right")), len(kept) - 1)
+    return int(kept[at]), w[kept[at]] / cum[-1]

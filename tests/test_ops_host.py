@@ -191,3 +191,27 @@ def test_rope_frequencies():
     for a in [(1e6, 256, 258), (1e6, 256, 3), (0.0, 256, 64)]:
         with pytest.raises(L.OmgError):
             ops.rope_frequencies(*a, device="cpu")
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(dtype=3), "dtype 3"),
+    (dict(rows=-1), "-1 rows"),
+    (dict(vocab=0), "vocabulary of 0"),
+    (dict(vocab=327681, stride=1 << 20), "vocabulary of 327681"),
+    (dict(dtype=1, vocab=524289, stride=1 << 20), "vocabulary of 524289"),
+    (dict(stride=99), "stride 99 < vocabulary 100"),
+    (dict(logits=0), "logits is null"),
+    (dict(logits=P + 2), "logits is not 4-byte aligned"),
+    (dict(u=0), "u is null"),
+    (dict(tokens=0), "tokens is null"),
+])
+def test_samples_refused(kw, text):
+    f = dict(logits=P, stride=100, dtype=2, rows=2, vocab=100, u=P, temperature_all=1.0,
+             top_p_all=1.0, tokens=P, probs=P)
+    f.update(kw)
+    refused(L.lib().omg_sample(0, C.byref(L.SampleArgsC(**f)), None), text)
+
+
+def test_host_logits_refused():
+    with pytest.raises(L.OmgError, match="on a GPU"):
+        ops.sample(torch.zeros(1, 5), torch.zeros(1))
