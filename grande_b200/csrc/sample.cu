@@ -17,9 +17,8 @@
 // The outcome is discrete, so sums have to be good to well under a border's
 // width: a border of the running sum lies within 2^-24 of u times the total
 // for about one row in 2^24 / vocab, far too often for f32. Weights are
-// 64-bit integers in units of 2^-44 of the largest, from a 64-bit exp2 (table
-// of 64 and a polynomial), so all sums are exact and the same in any order,
-// atomics included.
+// 64-bit integers in units of 2^-44 of the largest, from a 64-bit exp2, so all
+// sums are exact and the same in any order, atomics included.
 //
 // Bound: one read of the logits at HBM rate; above it stands the 64-bit
 // exponential of every element where no top-k cuts the row first.
@@ -27,6 +26,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "ptx.cuh"
 #include "sample.cuh"
@@ -37,20 +37,26 @@ namespace {
 
 namespace cg = cooperative_groups;
 using u64 = unsigned long long;
+// The kernel is one body of lambdas; left to itself the compiler calls some
+// of them, with their captures in local memory.
+#define INLINE __attribute__((always_inline))
 
 constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 2944;      // log2 w from 0 to -46 in steps of 1/64
 constexpr int kList = 2048;      // elements the first CTA sorts
 constexpr int kScale = 44;       // weights in units of 2^-44
-constexpr int kMaxCluster = 8;
-constexpr int kSliceBytes = 160 * 1024;
+constexpr int kMaxCluster = 16;
+constexpr int kSliceBytes = 160 * 1024;     // of a row in a CTA's shared memory
+constexpr int kEach = kList / kThreads;     // list entries per thread
+constexpr int kRankSort = 512;              // lists up to this are sorted by counting
 constexpr int kSubBits = 11;     // refinement: up to 2^11 bins of the (value, index) order
 
+// The crossing bin of a search: what lies before it, what it holds, and the
+// target (counts or masses).
 struct Found {
   int ok, bin;
-  unsigned above_cnt, bin_cnt;
-  u64 above_mass, bin_mass;
+  u64 above, here, target;
 };
 
 struct Shared {
@@ -62,12 +68,15 @@ struct Shared {
       u64 comp[kList];
       u64 w[kList];
     } l;
+    float queue[kWarps][8][32];  // the draw: each lane's kept values to weigh
   };
-  double table[64];
+  double table[kBins];
   u64 red[kWarps];
   unsigned redc[kWarps];
+  float redf[kWarps];
   // Read by the other CTAs of the cluster.
   u64 best, part_mass, lo, hi;
+  float top;
   unsigned part_cnt, list_n;
   Found found;
   u64 threshold;
@@ -96,37 +105,39 @@ __device__ __forceinline__ float value_of(u64 comp) {
   return __uint_as_float(key ^ (key >> 31 ? 0x80000000u : 0xffffffffu));
 }
 
-// log2 w of a value, and w as an integer.
+// Bin and weight of a value. The bin is -64 log2 w rounded, in f32: monotone
+// in the value, which is all that the search needs of it. The weight is
+// 2^44 w rounded, from 64 bits: 2^(44 - bin / 64) from a table and
+// 2^(r / 64), r what the bin's rounding left (|r| < 0.51), a polynomial of
+// degree 4 in (ln 2 / 64)^k / k! r^k, good to 2^-44.
 struct Weigher {
-  double c, mc;  // log2(e) / T, the same times the row's largest
-  float best;
+  float best, c64;      // the row's largest; 64 log2(e) / T
+  double bestd, c64d;
   const double* table;
 
-  // -64 log2 w rounded, or -1 when w is zero; *y: log2 w.
-  __device__ __forceinline__ int bin(float x, double* y) const {
-    const double v = x == best ? 0.0 : fma(static_cast<double>(x), c, -mc);
-    if (!(v > -45.5)) return -1;
-    *y = v;
-    const double magic = 6755399441055744.0 / 64;  // 1.5 * 2^52 / 64: units of 1/64
-    const int t = __double2loint(v + magic);
-    return t > 0 ? 0 : -t;
+  static constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: units of 1
+  // The bin as kMagic - bin; a weight below 2^-45.5 lies below kLast.
+  static constexpr float kLast = kMagic - 2912.0f;
+  __device__ __forceinline__ float mark(float x) const { return fmaf(x - best, c64, kMagic); }
+  static __device__ __forceinline__ int bin_of_mark(float m) {
+    return 0x4B400000 - __float_as_int(m);
   }
-  __device__ __forceinline__ u64 weight(double y) const {
-    const double magic = 6755399441055744.0 / 64;
-    const double s = y + magic;
-    const int t = __double2loint(s);
-    const double r = y - (s - magic);  // |r| <= 1/128
-    // 2^r - 1 = r (ln 2 + r (ln 2)^2 / 2 + ...), to 2^-44 of it.
-    double p = fma(r, 9.618129107628477e-3, 5.550410866482158e-2);
-    p = fma(p, r, 2.402265069591007e-1);
-    p = fma(p, r, 6.931471805599453e-1);
-    const double b = table[t & 63];
-    const double m = fma(b * r, p, b);
-    const long long bits = __double_as_longlong(m);
-    const int e = static_cast<int>(bits >> 52) - 1023 + (t >> 6);
-    const int shift = 52 - kScale - e;
-    const u64 mant = (bits & 0xfffffffffffffll) | 0x10000000000000ll;
-    return shift > 60 ? 0 : (mant + (1ull << (shift - 1))) >> shift;
+  __device__ __forceinline__ int bin(float x) const {
+    const float m = mark(x);
+    return m >= kLast ? bin_of_mark(m) : -1;
+  }
+  __device__ __forceinline__ u64 weight(float x, unsigned bin) const {
+    // The bin as a double, through the low bits of 2^52.
+    const double db = __hiloint2double(0x43300000, bin) - 4503599627370496.0;
+    const double r = fma(static_cast<double>(x) - bestd, c64d, db);
+    constexpr double l = 1.0830424696249145e-2;  // ln 2 / 64
+    double p = fma(r, l * l * l * l / 24, l * l * l / 6);
+    p = fma(p, r, l * l / 2);
+    p = fma(p, r, l);
+    const double b = table[bin];
+    const double w = fma(b * r, p, b) + 4503599627370496.0;
+    return (static_cast<u64>(__double2hiint(w) - 0x43300000) << 32) |
+           static_cast<unsigned>(__double2loint(w));
   }
 };
 
@@ -165,8 +176,8 @@ __device__ __forceinline__ void block_scan(Shared& sh, unsigned& c, u64& m, unsi
   }
   __syncthreads();
   if (warp == 0) {
-    unsigned a = sh.redc[lane];
-    u64 b = sh.red[lane];
+    unsigned a = lane < kWarps ? sh.redc[lane] : 0;
+    u64 b = lane < kWarps ? sh.red[lane] : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const unsigned a2 = __shfl_up_sync(0xffffffffu, a, o);
@@ -176,8 +187,10 @@ __device__ __forceinline__ void block_scan(Shared& sh, unsigned& c, u64& m, unsi
         b += b2;
       }
     }
-    sh.redc[lane] = a;
-    sh.red[lane] = b;
+    if (lane < kWarps) {
+      sh.redc[lane] = a;
+      sh.red[lane] = b;
+    }
   }
   __syncthreads();
   c = ci - c + (warp ? sh.redc[warp - 1] : 0);
@@ -197,11 +210,32 @@ __device__ __forceinline__ u64 floor_part(float u, u64 m) {
   return __umul64hi(__double2ull_rz(static_cast<double>(u) * 18446744073709551616.0), m);
 }
 
-// Sort sh.l.comp[0 .. n) ascending (n a power of two).
+// Sort sh.l.comp[0 .. n) ascending; n <= kList. Short lists by counting the
+// smaller entries (all are distinct but for the padding ~0, which may land
+// anywhere behind), longer ones bitonically, padded to a power of two.
 __device__ void sort_list(Shared& sh, int n) {
-  for (int k = 2; k <= n; k <<= 1)
+  const int tid = threadIdx.x;
+  __syncthreads();
+  if (n <= kRankSort) {
+    static_assert(kRankSort <= kThreads, "an entry per thread");
+    const u64 mine = tid < n ? sh.l.comp[tid] : ~0ull;
+    int at = 0;
+    if (tid < n) {
+#pragma unroll 8
+      for (int i = 0; i < n; ++i) at += sh.l.comp[i] < mine || (sh.l.comp[i] == mine && i < tid);
+    }
+    __syncthreads();
+    if (tid < n) sh.l.comp[at] = mine;
+    __syncthreads();
+    return;
+  }
+  int pad = 2;
+  while (pad < n) pad <<= 1;
+  for (int i = n + tid; i < pad; i += kThreads) sh.l.comp[i] = ~0ull;
+  __syncthreads();
+  for (int k = 2; k <= pad; k <<= 1)
     for (int j = k >> 1; j > 0; j >>= 1) {
-      for (int i = threadIdx.x; i < n / 2; i += kThreads) {
+      for (int i = tid; i < pad / 2; i += kThreads) {
         const int a = 2 * i - (i & (j - 1)), b = a + j;
         const u64 x = sh.l.comp[a], y = sh.l.comp[b];
         if ((x > y) == ((a & k) == 0)) {
@@ -213,7 +247,7 @@ __device__ void sort_list(Shared& sh, int n) {
     }
 }
 
-template <class T>
+template <class T, bool STAGED>
 __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
   Shared& sh = *reinterpret_cast<Shared*>(smem);
@@ -222,71 +256,78 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
   const int rank = static_cast<int>(cluster.block_rank());
   const int row = blockIdx.x / C;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  auto peer = [&](int r) -> Shared& { return *cluster.map_shared_rank(&sh, r); };
+  auto peer = [&](int r) INLINE -> Shared& { return *cluster.map_shared_rank(&sh, r); };
 
-  // This CTA's slice [i0, i0 + n) of the row, kept at x[0 .. n).
+  // This CTA's slice [i0, i0 + n) of the row, in blocks of 16 aligned bytes:
+  // block j holds elements j kVec - lead and on; those outside the slice read
+  // as -infinity, which nothing keeps.
   const int per = (a.vocab + C - 1) / C;
   const int i0 = min(rank * per, a.vocab), n = min(per, a.vocab - i0);
   const T* src = static_cast<const T*>(a.logits) + row * a.stride + i0;
   constexpr int kVec = 16 / sizeof(T);
   const int lead = static_cast<int>((reinterpret_cast<uintptr_t>(src) & 15) / sizeof(T));
-  T* x = reinterpret_cast<T*>(smem + (sizeof(Shared) + 15) / 16 * 16) + lead;
-  if (tid < 64) sh.table[tid] = exp2(tid / 64.0);
+  const int blocks = (lead + n + kVec - 1) / kVec;
+  uint4* staged = reinterpret_cast<uint4*>(smem + (sizeof(Shared) + 15) / 16 * 16);
+  auto fetch_global = [&](int j) INLINE -> uint4 {
+    const int at = j * kVec - lead;
+    if (at >= 0 && at + kVec <= n) return *reinterpret_cast<const uint4*>(src + at);
+    union {
+      T e[kVec];
+      uint4 v;
+    } u;
+#pragma unroll
+    for (int q = 0; q < kVec; ++q)
+      u.e[q] = at + q >= 0 && at + q < n ? src[at + q] : static_cast<T>(-INFINITY);
+    return u.v;
+  };
+  for (int i = tid; i < kBins; i += kThreads) sh.table[i] = exp2(kScale - i / 64.0);
   if (tid == 0) {
     sh.list_n = 0;
     sh.threshold = ~0ull;
   }
-  u64 best = ~0ull;
+  // Whole blocks [b0, b1); only the first and the last can be cut.
+  const int b0 = lead ? 1 : 0, b1 = max(b0, (lead + n) / kVec);
+  const uint4* whole = reinterpret_cast<const uint4*>(src - lead);
+  float top = -INFINITY;  // fmaxf passes over NaN
+  auto top_of = [&](const uint4& v) INLINE {
+    const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+    for (int q = 0; q < kVec; ++q) top = fmaxf(top, as_float(e[q]));
+  };
   {
-    const int head = min(n, lead ? kVec - lead : 0);
-    const int body = (n - head) / kVec;
-    for (int i = tid; i < head; i += kThreads) {
-      x[i] = src[i];
-      best = min(best, order_of(as_float(x[i]), i0 + i));
-    }
-    const uint4* vs = reinterpret_cast<const uint4*>(src + head);
-    uint4* vd = reinterpret_cast<uint4*>(x + head);
-    for (int j0 = 0; j0 < body; j0 += 4 * kThreads) {
+    int j = b0 + tid;
+    for (; j + 3 * kThreads < b1; j += 4 * kThreads) {
       uint4 v[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int j = j0 + k * kThreads + tid;
-        if (j < body) v[k] = __ldcs(vs + j);
-      }
+      for (int k = 0; k < 4; ++k) v[k] = whole[j + k * kThreads];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int j = j0 + k * kThreads + tid;
-        if (j >= body) break;
-        vd[j] = v[k];
-        const T* e = reinterpret_cast<const T*>(&v[k]);
-        float m = -INFINITY;
-        int at = 0;
-#pragma unroll
-        for (int q = 0; q < kVec; ++q) {
-          const float f = as_float(e[q]);
-          if (f > m) {
-            m = f;
-            at = q;
-          }
-        }
-        best = min(best, order_of(m, i0 + head + j * kVec + at));
+        if (STAGED) staged[j + k * kThreads] = v[k];
+        top_of(v[k]);
       }
     }
-    for (int i = head + body * kVec + tid; i < n; i += kThreads) {
-      x[i] = src[i];
-      best = min(best, order_of(as_float(x[i]), i0 + i));
+    for (; j < b1; j += kThreads) {
+      const uint4 v = whole[j];
+      if (STAGED) staged[j] = v;
+      top_of(v);
+    }
+    // The cut blocks.
+    const int edge = tid == 0 && b0 ? 0 : tid == 1 && b1 < blocks ? b1 : -1;
+    if (edge >= 0) {
+      const uint4 v = fetch_global(edge);
+      if (STAGED) staged[edge] = v;
+      top_of(v);
     }
   }
-  best = warp_min64(best);
-  if (lane == 0) sh.red[warp] = best;
+  top = warp_max(top);
+  if (lane == 0) sh.redf[warp] = top;
   __syncthreads();
   if (warp == 0) {
-    best = warp_min64(sh.red[lane]);
-    if (lane == 0) sh.best = best;
+    top = warp_max(sh.redf[lane]);
+    if (lane == 0) sh.top = top;
   }
   cluster.sync();
-  best = ~0ull;
-  for (int r = 0; r < C; ++r) best = min(best, peer(r).best);
+  top = warp_max(lane < C ? peer(lane).top : -INFINITY);
 
   const float temp = a.temperature ? a.temperature[row] : a.temperature1;
   int k = a.top_k ? a.top_k[row] : a.top_k1;
@@ -296,106 +337,187 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
   const float u = fminf(fmaxf(a.u[row], 0.0f), 0.99999994f);
   if (k <= 0 || k >= a.vocab) k = INT_MAX;
   if (!(top_p < 1.0f)) top_p = 1.0f;
-  Weigher wt;
-  wt.best = value_of(best);
-  const bool dead = wt.best == -INFINITY;
+  const bool dead = top == -INFINITY;
+  const bool infinite = top == INFINITY;  // the infinite elements share the row
+  if (infinite) top = 0.0f;
+  // One sweep: f(index of the first, kVec values) for every block of
+  // [first, last), `step` threads side by side. Rounds of whole blocks go
+  // without checks, U at a time with their loads ahead; the rest is checked.
+  // Whole warps stay together: blocks that are not there are -infinity.
+  auto unpack = [&](const uint4& b, float (&v)[kVec]) INLINE {
+    const T* e = reinterpret_cast<const T*>(&b);
+#pragma unroll
+    for (int q = 0; q < kVec; ++q) v[q] = as_float(e[q]);
+    if (infinite) {
+#pragma unroll
+      for (int q = 0; q < kVec; ++q) v[q] = v[q] == INFINITY ? 0.0f : -INFINITY;
+    }
+  };
+  auto sweep_run = [&](int first, int last, int step, auto unroll, auto f) INLINE {
+    constexpr int U = decltype(unroll)::value;
+    const int me = step == 32 ? lane : tid;
+    const int lo = max(first, min(b0, last)), hi = max(lo, min(last, b1));
+    const int rounds = (hi - lo) / step / U;
+    const uint4* p = (STAGED ? staged : whole) + lo + me;
+    int i = i0 + (lo + me) * kVec - lead;
+#pragma unroll 1
+    for (int r = 0; r < rounds; ++r) {
+      uint4 b[U];
+#pragma unroll
+      for (int k = 0; k < U; ++k) b[k] = p[k * step];
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        float v[kVec];
+        unpack(b[k], v);
+        f(i, v);
+        i += step * kVec;
+      }
+      p += U * step;
+    }
+    // What is cut or left over: blocks [first, lo) and [at, last).
+    const int at = lo + rounds * U * step, count = (lo - first) + (last - at);
+#pragma unroll 1
+    for (int q0 = 0; q0 < count; q0 += step) {
+      const int q = q0 + me;
+      const int j = q < lo - first ? first + q : at + q - (lo - first);
+      float v[kVec];
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) v[e] = -INFINITY;
+      if (q < count) unpack(STAGED ? staged[j] : fetch_global(j), v);
+      f(i0 + j * kVec - lead, v);
+    }
+  };
+  auto sweep = [&](auto unroll, auto f) INLINE { sweep_run(0, blocks, kThreads, unroll, f); };
+  constexpr std::integral_constant<int, 1> one{};
+  constexpr std::integral_constant<int, 4> light{};
+  constexpr std::integral_constant<int, kVec == 4 ? 2 : 1> heavy{};
+
   if (dead || !(temp > 0.0f) || k == 1 || top_p <= 0.0f) {
     // The largest alone. (Every CTA of the cluster takes the same branches.)
-    if (rank == 0 && tid == 0) {
-      a.tokens[row] = dead ? -1 : static_cast<int>(best & 0xffffffffu);
-      if (a.probs) a.probs[row] = dead ? 0.0f : 1.0f;
+    unsigned at = UINT_MAX;
+    if (!dead)
+      sweep(light, [&](int i, const float(&v)[kVec]) INLINE {
+#pragma unroll
+        for (int q = 0; q < kVec; ++q)
+          if (v[q] == top) at = min(at, static_cast<unsigned>(i + q));
+      });
+    at = __reduce_min_sync(0xffffffffu, at);
+    if (lane == 0) sh.redc[warp] = at;
+    __syncthreads();
+    if (warp == 0) {
+      at = __reduce_min_sync(0xffffffffu, sh.redc[lane]);
+      if (lane == 0) sh.part_cnt = at;
+    }
+    cluster.sync();
+    if (rank == 0 && warp == 0) {
+      at = __reduce_min_sync(0xffffffffu, lane < C ? peer(lane).part_cnt : UINT_MAX);
+      if (lane == 0) {
+        a.tokens[row] = dead ? -1 : static_cast<int>(at);
+        if (a.probs) a.probs[row] = dead ? 0.0f : 1.0f;
+      }
     }
     cluster.sync();  // no CTA leaves while another may read its memory
     return;
   }
-  wt.c = 1.4426950408889634 / static_cast<double>(temp);
-  wt.mc = static_cast<double>(wt.best) * wt.c;
+  Weigher wt;
+  wt.best = top;
+  wt.bestd = top;
+  // Finite for the least temperatures, too: the largest itself is in bin 0.
+  wt.c64d = fmin(64 * 1.4426950408889634 / static_cast<double>(temp), 1e38);
+  wt.c64 = static_cast<float>(wt.c64d);
   wt.table = sh.table;
   const double min_w = static_cast<double>(min_p) * static_cast<double>(1ull << kScale);
+  auto bin_of = [&](float v) INLINE { return wt.bin(v); };
+  auto weight_of = [&](float v, int b) INLINE { return wt.weight(v, b); };
 
-  // Element i of the slice: its order, and its bin (-1: no weight).
-  auto comp_at = [&](int i) { return order_of(as_float(x[i]), i0 + i); };
-  auto bin_at = [&](int i, double* y) {
-    float v = as_float(x[i]);
-    return wt.bin(v, y);
-  };
-
-  // Histograms of one sweep: elements of order at most `limit` that `key`
-  // gives a bin >= 0.
-  auto clear_hist = [&]() {
-    for (int i = tid; i < kBins; i += kThreads) sh.h.cnt[i] = sh.h.lo[i] = sh.h.hi[i] = 0;
+  // Histograms of one sweep over the slice, counts or masses.
+  auto clear_hist = [&](bool mass) INLINE {
+    for (int i = tid; i < kBins; i += kThreads) {
+      if (mass)
+        sh.h.lo[i] = sh.h.hi[i] = 0;
+      else
+        sh.h.cnt[i] = 0;
+    }
     if (tid == 0) sh.found.ok = 0;
     __syncthreads();
   };
-  auto add = [&](int bin, u64 w, bool mass) {
-    atomicAdd(&sh.h.cnt[bin], 1u);
+  auto add = [&](int bin, u64 w, bool mass) INLINE {
     if (mass) {
+      // 64 bits from two 32-bit atomics: whoever wraps the low word carries.
       const unsigned lo = static_cast<unsigned>(w);
       const unsigned old = atomicAdd(&sh.h.lo[bin], lo);
       const unsigned hi = static_cast<unsigned>(w >> 32) + (old + lo < old ? 1u : 0u);
       if (hi) atomicAdd(&sh.h.hi[bin], hi);
+    } else {
+      atomicAdd(&sh.h.cnt[bin], 1u);
     }
   };
-  // The first bin at which the running count reaches `count`, or (mass) the
-  // running mass reaches `target` (0: top_p of the total).
-  auto find = [&](bool mass, unsigned count, u64 target) -> Found {
+  // The first bin at which the running sum (of counts or masses) reaches
+  // `target`; 0: top_p of the mass.
+  auto find = [&](bool mass, u64 target) INLINE -> Found {
     cluster.sync();
     const int share = kBins / C;  // C divides it
     const int each = (share + kThreads - 1) / kThreads;
-    unsigned c[3];
-    u64 m[3];
-    unsigned ct = 0;
+    constexpr int kMost = (kBins + kThreads - 1) / kThreads;
+    // This thread's bins, from every CTA: all loads in flight together (a
+    // load from a peer takes several hundred clocks).
+    u64 m[kMost];
     u64 mt = 0;
+    if (C == 1) {
 #pragma unroll
-    for (int e = 0; e < 3; ++e) {
-      c[e] = 0;
-      m[e] = 0;
-      const int b = tid * each + e;
-      if (e < each && b < share) {
-        const int g = rank * share + b;
-        for (int r = 0; r < C; ++r) {
-          Shared& p = peer(r);
-          c[e] += p.h.cnt[g];
-          if (mass) m[e] += (static_cast<u64>(p.h.hi[g]) << 32) + p.h.lo[g];
+      for (int e = 0; e < kMost; ++e) {
+        const int b = tid * each + e;
+        m[e] = e < each && b < share
+                   ? (mass ? (static_cast<u64>(sh.h.hi[b]) << 32) + sh.h.lo[b] : sh.h.cnt[b])
+                   : 0;
+        mt += m[e];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < kMost; ++e) {
+        m[e] = 0;
+        const int b = tid * each + e;
+        if (e < each && b < share) {
+          const int g = rank * share + b;
+#pragma unroll 1
+          for (int r0 = 0; r0 < C; r0 += 8) {
+            unsigned lo[8], hi[8];
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+              lo[r] = hi[r] = 0;
+              if (r0 + r < C) {
+                const Shared& p = peer(r0 + r);
+                lo[r] = mass ? p.h.lo[g] : p.h.cnt[g];
+                if (mass) hi[r] = p.h.hi[g];
+              }
+            }
+#pragma unroll
+            for (int r = 0; r < 8; ++r) m[e] += (static_cast<u64>(hi[r]) << 32) + lo[r];
+          }
         }
+        mt += m[e];
       }
-      ct += c[e];
-      mt += m[e];
     }
-    unsigned cx = ct, ctot;
+    unsigned none = 0, ntot;
     u64 mx = mt, mtot;
-    block_scan(sh, cx, mx, &ctot, &mtot);
-    if (tid == 0) {
-      sh.part_cnt = ctot;
-      sh.part_mass = mtot;
-    }
+    block_scan(sh, none, mx, &ntot, &mtot);
+    if (tid == 0) sh.part_mass = mtot;
     cluster.sync();
-    u64 all = 0;
-    for (int r = 0; r < C; ++r) {
-      const u64 pm = peer(r).part_mass;
-      const unsigned pc = peer(r).part_cnt;
-      all += pm;
-      if (r < rank) {
-        cx += pc;
-        mx += pm;
-      }
-    }
-    if (mass && target == 0) target = ceil_part(top_p, all);
+    const u64 part = lane < C ? peer(lane).part_mass : 0;
+    const u64 all = warp_sum64(part);
+    mx += warp_sum64(lane < rank ? part : 0);
+    if (target == 0) target = ceil_part(top_p, all);
 #pragma unroll
-    for (int e = 0; e < 3; ++e) {
-      const bool here = mass ? mx < target && mx + m[e] >= target
-                             : cx < count && cx + c[e] >= count;
-      if (here) {
+    for (int e = 0; e < kMost; ++e) {
+      if (mx < target && mx + m[e] >= target) {
         Found f;
         f.ok = 1;
         f.bin = rank * share + tid * each + e;
-        f.above_cnt = cx;
-        f.bin_cnt = c[e];
-        f.above_mass = mx;
-        f.bin_mass = target;  // handed on: the target of the mass
+        f.above = mx;
+        f.here = m[e];
+        f.target = target;
         for (int r = 0; r < C; ++r) peer(r).found = f;
       }
-      cx += c[e];
       mx += m[e];
     }
     cluster.sync();
@@ -403,84 +525,125 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
     __syncthreads();  // read by all before the next sweep clears it
     return f;
   };
-  // Elements of `pred` (the same total in every CTA's eyes, at most kList)
-  // into the first CTA's list; returns their number, padded list sorted there.
-  auto gather = [&](auto pred) -> int {
+  // Elements of `pred(value, index)` (at most kList in the cluster) into the
+  // first CTA's list, sorted there; returns their number there, 0 elsewhere.
+  // `maybe(mark)` is a cheap test that they all pass; most warps go on from it.
+  auto gather = [&](auto maybe, auto pred) INLINE -> int {
     Shared& first = peer(0);
-    const int rounds = (n + kThreads - 1) / kThreads;
-    for (int q = 0; q < rounds; ++q) {
-      const int i = q * kThreads + tid;
-      const bool in = i < n && pred(i);
-      const unsigned vote = __ballot_sync(0xffffffffu, in);
-      if (!vote) continue;
+    sweep(light, [&](int i, const float(&v)[kVec]) INLINE {
+      bool any = false;
+#pragma unroll
+      for (int q = 0; q < kVec; ++q) any |= maybe(wt.mark(v[q]));
+      if (!__any_sync(0xffffffffu, any)) return;
+      unsigned in = 0;
+#pragma unroll
+      for (int q = 0; q < kVec; ++q)
+        if (pred(v[q], i + q)) in |= 1u << q;
+      unsigned upto = __popc(in);
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += y;
+      }
       unsigned at = 0;
-      if (lane == 0) at = atomicAdd(&first.list_n, static_cast<unsigned>(__popc(vote)));
-      at = __shfl_sync(0xffffffffu, at, 0) + __popc(vote & ((1u << lane) - 1));
-      if (in && at < kList) first.l.comp[at] = comp_at(i);
-    }
+      if (lane == 31) at = atomicAdd(&first.list_n, upto);
+      at = __shfl_sync(0xffffffffu, at, 31) + upto - __popc(in);
+#pragma unroll
+      for (int q = 0; q < kVec; ++q)
+        if ((in >> q) & 1) {
+          if (at < kList) first.l.comp[at] = order_of(v[q], i + q);
+          ++at;
+        }
+    });
     cluster.sync();
     int count = 0;
     if (rank == 0) {
       count = min(static_cast<int>(sh.list_n), kList);
-      int pad = 2;
-      while (pad < count) pad <<= 1;
-      for (int i = count + tid; i < pad; i += kThreads) sh.l.comp[i] = ~0ull;
-      __syncthreads();
+      sort_list(sh, count);
       if (tid == 0) sh.list_n = 0;
-      sort_list(sh, pad);
     }
     return count;
   };
-  // Weight of list entry i.
-  auto list_weight = [&](u64 comp) -> u64 {
-    double y;
-    return wt.bin(value_of(comp), &y) < 0 ? 0 : wt.weight(y);
+  auto list_weight = [&](u64 comp) INLINE -> u64 {
+    const float v = value_of(comp);
+    const int b = bin_of(v);
+    return b < 0 ? 0 : weight_of(v, b);
   };
 
-  // The order of the last element kept by top-k (mass false) or top-p, among
-  // elements of order <= limit; ~0: all that have weight. With `whole` (a
-  // count of at most kList) the elements down to the crossing go to the first
-  // CTA's list instead, sorted, and their number is *listed there.
-  auto search = [&](bool mass, unsigned count, u64 limit, bool whole, int* listed) -> u64 {
-    clear_hist();
-    for (int i = tid; i < n; i += kThreads) {
-      if (limit != ~0ull && comp_at(i) > limit) continue;
-      double y;
-      const int b = bin_at(i, &y);
-      if (b >= 0) add(b, mass ? wt.weight(y) : 0, mass);
-    }
-    Found f = find(mass, count, 0);
+  // Finds the last element that top-k (mass false, `count`) or top-p keeps
+  // among those of order at most `limit`. If all the elements down to it fit
+  // the list, they are in the first CTA's list, sorted, and *listed their
+  // number there (top-k up to kList: always); otherwise *listed is -1 and its
+  // order comes back (~0: every element with weight).
+  auto search = [&](bool mass, unsigned count, u64 limit, int* listed, u64* goal) INLINE -> u64 {
+    *listed = -1;
+    clear_hist(mass);
+    auto tally = [&](int i, const float(&v)[kVec], bool limited) INLINE {
+#pragma unroll
+      for (int q0 = 0; q0 < kVec; q0 += 4) {
+        // Four weights first: their 64-bit chains overlap.
+        unsigned b[4];
+        bool on[4];
+        u64 w[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float m = wt.mark(v[q0 + q]);
+          on[q] = m >= Weigher::kLast;
+          b[q] = on[q] ? Weigher::bin_of_mark(m) : 0;
+          if (limited) on[q] = on[q] && order_of(v[q0 + q], i + q0 + q) <= limit;
+          w[q] = mass ? weight_of(v[q0 + q], b[q]) : 0;
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (on[q]) add(b[q], w[q], mass);
+      }
+    };
+    if (limit == ~0ull)
+      sweep(heavy, [&](int i, const float(&v)[kVec]) INLINE { tally(i, v, false); });
+    else
+      sweep(one, [&](int i, const float(&v)[kVec]) INLINE { tally(i, v, true); });
+    Found f = find(mass, mass ? 0 : count);
+    const u64 target = f.target;
+    *goal = target;
+    const int bin = f.bin;
+    const float bin_mark = Weigher::kMagic - static_cast<float>(bin);
     if (!f.ok) {
-      if (!whole) return limit;
-      // Fewer than `count` elements have weight: all of them.
-      *listed = gather([&](int i) {
-        double y;
-        return bin_at(i, &y) >= 0;
+      // Fewer than `count` elements have weight.
+      if (count <= kList) *listed = gather([&](float m) INLINE { return m >= Weigher::kLast; },
+                                        [&](float v, int) INLINE { return bin_of(v) >= 0; });
+      return limit;
+    }
+    u64 above = f.above;
+    // Bounds on numbers of elements: of a mass, it over its least weight.
+    const u64 least = mass ? max(1ull, static_cast<u64>(exp2(kScale - (bin + 1.0) / 64))) : 1;
+    if ((above + f.here) / least <= kList) {
+      *listed = gather([&](float m) INLINE { return m >= bin_mark; }, [&](float v, int i) INLINE {
+        const int b = bin_of(v);
+        return b >= 0 && b <= bin && (limit == ~0ull || order_of(v, i) <= limit);
       });
       return limit;
     }
-    const u64 target = f.bin_mass;
-    const int bin = f.bin;
-    unsigned above = f.above_cnt;
-    u64 above_mass = f.above_mass;
     u64 lo = 0, hi = ~0ull;  // orders still in question, within the bin
-    auto open = [&](int i) {
-      double y;
-      if (bin_at(i, &y) != bin) return false;
-      const u64 o = comp_at(i);
+    auto open = [&](float v, int i) INLINE {
+      if (wt.mark(v) != bin_mark) return false;
+      const u64 o = order_of(v, i);
       return o >= lo && o <= hi && o <= limit;
     };
+    const bool few = !mass && count <= kList;  // the list is to hold all of them
     bool first = true;
-    while ((whole ? above : 0) + f.bin_cnt > kList) {
+    while ((few ? above + f.here : f.here) / least > kList) {
       if (first) {
         // The bin's least and greatest order.
         u64 mn = ~0ull, mx = ~0ull;  // mx: the complement's least
-        for (int i = tid; i < n; i += kThreads)
-          if (open(i)) {
-            const u64 o = comp_at(i);
-            mn = min(mn, o);
-            mx = min(mx, ~o);
-          }
+        sweep(one, [&](int i, const float(&v)[kVec]) INLINE {
+#pragma unroll
+          for (int q = 0; q < kVec; ++q)
+            if (open(v[q], i + q)) {
+              const u64 o = order_of(v[q], i + q);
+              mn = min(mn, o);
+              mx = min(mx, ~o);
+            }
+        });
         mn = warp_min64(mn);
         mx = warp_min64(mx);
         __syncthreads();
@@ -491,177 +654,221 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
           atomicMin(&sh.hi, mx);
         }
         cluster.sync();
-        mn = mx = ~0ull;
-        for (int r = 0; r < C; ++r) {
-          mn = min(mn, peer(r).lo);
-          mx = min(mx, peer(r).hi);
-        }
-        lo = mn;
-        hi = ~mx;
+        lo = warp_min64(lane < C ? peer(lane).lo : ~0ull);
+        hi = ~warp_min64(lane < C ? peer(lane).hi : ~0ull);
         first = false;
       }
+      if (lo == hi) break;  // one element is left, however heavy
       const u64 span = hi - lo;
       const int bits = 64 - __clzll(static_cast<long long>(span));
       const int shift = max(0, bits - kSubBits);
-      clear_hist();
-      for (int i = tid; i < n; i += kThreads) {
-        if (!open(i)) continue;
-        double y;
-        bin_at(i, &y);
-        add(static_cast<int>((comp_at(i) - lo) >> shift), mass ? wt.weight(y) : 0, mass);
-      }
-      f = find(mass, count - above, mass ? target - above_mass : 0);
-      above += f.above_cnt;
-      above_mass += f.above_mass;
+      clear_hist(mass);
+      sweep(one, [&](int i, const float(&v)[kVec]) INLINE {
+#pragma unroll
+        for (int q = 0; q < kVec; ++q)
+          if (open(v[q], i + q))
+            add(static_cast<int>((order_of(v[q], i + q) - lo) >> shift),
+                mass ? weight_of(v[q], bin) : 0, mass);
+      });
+      f = find(mass, target - above);
+      above += f.above;
       lo += static_cast<u64>(f.bin) << shift;
       hi = min(hi, lo + (1ull << shift) - 1);
     }
-    if (whole) {
-      *listed = gather([&](int i) {
-        double y;
-        const int b = bin_at(i, &y);
-        if (b < 0 || b > bin) return false;
-        const u64 o = comp_at(i);
-        return b < bin || (o <= hi && o <= limit);
+    if (few) {
+      *listed = gather([&](float m) INLINE { return m >= bin_mark; }, [&](float v, int i) INLINE {
+        const int b = bin_of(v);
+        return b >= 0 && (b < bin || (b == bin && order_of(v, i) <= hi));
       });
-      return ~0ull;
+      return limit;
     }
-    const int got = gather(open);
+    const int got = gather([&](float m) INLINE { return m == bin_mark; }, open);
     if (rank == 0) {
-      u64 found = 0;
-      if (mass) {
-        // Two entries per thread.
-        u64 w[2];
-        unsigned none = 0, nt;
-        for (int e = 0; e < 2; ++e) {
-          const int i = 2 * tid + e;
-          w[e] = i < got ? list_weight(sh.l.comp[i]) : 0;
-        }
-        u64 at = w[0] + w[1], tot;
-        block_scan(sh, none, at, &nt, &tot);
-        at += above_mass;
-        if (tid == 0) sh.threshold = sh.l.comp[max(got - 1, 0)];
-        __syncthreads();
-        for (int e = 0; e < 2; ++e) {
-          if (at < target && at + w[e] >= target) {
-            found = sh.l.comp[2 * tid + e];
-            sh.threshold = found;
-          }
-          at += w[e];
-        }
-      } else if (tid == 0) {
-        sh.threshold = sh.l.comp[min(static_cast<int>(count - above) - 1, got - 1)];
+      u64 w[kEach];
+      u64 at = 0, tot;
+      unsigned none = 0, nt;
+      for (int e = 0; e < kEach; ++e) {
+        const int i = kEach * tid + e;
+        w[e] = i < got ? (mass ? list_weight(sh.l.comp[i]) : 1) : 0;
+        at += w[e];
+      }
+      block_scan(sh, none, at, &nt, &tot);
+      at += above;
+      for (int e = 0; e < kEach; ++e) {
+        if (at < target && at + w[e] >= target) sh.threshold = sh.l.comp[kEach * tid + e];
+        at += w[e];
       }
     }
     cluster.sync();
     const u64 th = peer(0).threshold;
     cluster.sync();
-    return min(th, limit);
+    return th;
   };
-
-  auto finish = [&](int token, u64 w, u64 total) {
+  auto finish = [&](int token, u64 w, u64 total) INLINE {
     a.tokens[row] = token;
     if (a.probs)
       a.probs[row] = static_cast<float>(static_cast<double>(w) / static_cast<double>(total));
   };
 
-  if (k <= kList) {
-    // The kept elements are few: the first CTA does the rest from its list.
-    int listed = 0;
-    search(false, k, ~0ull, true, &listed);
-    if (rank == 0) {
-      const int kept = min(listed, k);
-      u64 w[2];
-      unsigned none = 0, ntot;
-      for (int e = 0; e < 2; ++e) {
-        const int i = 2 * tid + e;
-        w[e] = i < kept ? list_weight(sh.l.comp[i]) : 0;
-      }
-      u64 at = w[0] + w[1], total;
-      block_scan(sh, none, at, &ntot, &total);
-      const u64 target = top_p < 1.0f ? ceil_part(top_p, total) : ~0ull;
-      // Those that stay, back in index order.
-      int pad = 2;
-      while (pad < kept) pad <<= 1;
-      for (int e = 0; e < 2; ++e) {
-        const int i = 2 * tid + e;
-        if (i < pad) {
-          const bool stays = i < kept && at < target && static_cast<double>(w[e]) >= min_w;
-          const u64 idx = sh.l.comp[i] & 0xffffffffu;
-          sh.l.comp[i] = stays ? (idx << 32) | i : ~0ull;
-          sh.l.w[i] = w[e];
-        }
-        at += w[e];
-      }
-      __syncthreads();
-      sort_list(sh, pad);
-      u64 c[2];
-      for (int e = 0; e < 2; ++e) {
-        const int i = 2 * tid + e;
-        c[e] = i < pad ? sh.l.comp[i] : ~0ull;
-        w[e] = c[e] != ~0ull ? sh.l.w[c[e] & 0xffffffffu] : 0;
-      }
-      at = w[0] + w[1];
-      none = 0;
-      block_scan(sh, none, at, &ntot, &total);
-      const u64 draw = floor_part(u, total);
-      for (int e = 0; e < 2; ++e) {
-        if (at <= draw && at + w[e] > draw) finish(static_cast<int>(c[e] >> 32), w[e], total);
-        at += w[e];
-      }
+  // From a sorted list in the first CTA of which the first `kept` that lie
+  // before `target` of the running mass stay (0: top_p of the list's).
+  auto finish_list = [&](int kept, u64 target) INLINE {
+    u64 w[kEach];
+    u64 at = 0, total;
+    unsigned none = 0, ntot;
+    for (int e = 0; e < kEach; ++e) {
+      const int i = kEach * tid + e;
+      w[e] = i < kept ? list_weight(sh.l.comp[i]) : 0;
+      at += w[e];
     }
-    cluster.sync();
-    return;
-  }
-  u64 limit = ~0ull;
-  int listed;
-  if (k != INT_MAX) limit = search(false, k, limit, false, &listed);
-  if (top_p < 1.0f) limit = search(true, 0, limit, false, &listed);
+    block_scan(sh, none, at, &ntot, &total);
+    if (target == 0) target = top_p < 1.0f ? ceil_part(top_p, total) : ~0ull;
+    // Those that stay, back in index order.
+    for (int e = 0; e < kEach; ++e) {
+      const int i = kEach * tid + e;
+      if (i < kept) {
+        const bool stays = at < target && static_cast<double>(w[e]) >= min_w;
+        const u64 idx = sh.l.comp[i] & 0xffffffffu;
+        sh.l.comp[i] = stays ? (idx << 32) | i : ~0ull;
+        sh.l.w[i] = w[e];
+      }
+      at += w[e];
+    }
+    __syncthreads();
+    sort_list(sh, kept);
+    u64 c[kEach];
+    at = 0;
+    for (int e = 0; e < kEach; ++e) {
+      const int i = kEach * tid + e;
+      c[e] = i < kept ? sh.l.comp[i] : ~0ull;
+      w[e] = c[e] != ~0ull ? sh.l.w[c[e] & 0xffffffffu] : 0;
+      at += w[e];
+    }
+    none = 0;
+    block_scan(sh, none, at, &ntot, &total);
+    const u64 draw = floor_part(u, total);
+    for (int e = 0; e < kEach; ++e) {
+      if (at <= draw && at + w[e] > draw) finish(static_cast<int>(c[e] >> 32), w[e], total);
+      at += w[e];
+    }
+  };
 
-  // The draw: every warp sums a run of consecutive elements, the one whose
-  // run holds the drawn mass goes through it again.
-  auto weight_at = [&](int i) -> u64 {
-    if (limit != ~0ull && comp_at(i) > limit) return 0;
-    double y;
-    if (bin_at(i, &y) < 0) return 0;
-    const u64 w = wt.weight(y);
+  u64 limit = ~0ull, goal = 0;
+  int listed = -1;
+  if (k != INT_MAX) {
+    limit = search(false, k, limit, &listed, &goal);
+    if (listed >= 0) {
+      if (rank == 0) finish_list(min(listed, k), 0);
+      cluster.sync();
+      return;
+    }
+  }
+  if (top_p < 1.0f) {
+    limit = search(true, UINT_MAX, limit, &listed, &goal);
+    if (listed >= 0) {
+      if (rank == 0) finish_list(listed, goal);
+      cluster.sync();
+      return;
+    }
+  }
+
+  // The draw: every warp sums a run of consecutive blocks; the run that holds
+  // the drawn mass is then shared out over all warps of its CTA and gone
+  // through again. Lanes queue the values they keep and weigh them together
+  // once one of them has more than 4; nothing is queued when all are kept.
+  const float edge = limit == ~0ull ? -INFINITY : value_of(limit);
+  const int edge_idx = static_cast<int>(limit & 0x7fffffffu);
+  auto kept = [&](float v, int i) INLINE {
+    // What lies before the last kept element has weight, as that one has.
+    if (limit == ~0ull) return bin_of(v) >= 0;
+    return v > edge || (v == edge && i <= edge_idx);
+  };
+  auto weigh = [&](float v) INLINE -> u64 {
+    const u64 w = weight_of(v, bin_of(v));
     return static_cast<double>(w) >= min_w ? w : 0;
   };
-  const int run = ((n + kWarps - 1) / kWarps + 31) / 32 * 32;
-  const int r0 = min(warp * run, n), r1 = min(r0 + run, n);
+  const int run = (blocks + kWarps - 1) / kWarps;
+  const int r0 = min(warp * run, blocks), r1 = min(r0 + run, blocks);
+  float* queue = sh.queue[warp][0];
   u64 mine = 0;
-  for (int i = r0 + lane; i < r1; i += 32) mine += weight_at(i);
+  int waiting = 0;
+  auto flush = [&]() INLINE {
+#pragma unroll 1
+    for (int e = 0; __any_sync(0xffffffffu, e < waiting); ++e)
+      if (e < waiting) mine += weigh(queue[e * 32 + lane]);
+    waiting = 0;
+  };
+  __syncthreads();  // the queues take the histograms' place
+  if (limit == ~0ull)
+    sweep_run(r0, r1, 32, heavy, [&](int i, const float(&v)[kVec]) INLINE {
+#pragma unroll
+      for (int q = 0; q < kVec; ++q) mine += bin_of(v[q]) >= 0 ? weigh(v[q]) : 0;
+    });
+  else
+    sweep_run(r0, r1, 32, heavy, [&](int i, const float(&v)[kVec]) INLINE {
+#pragma unroll
+      for (int q = 0; q < kVec; ++q) {
+        if (kept(v[q], i + q)) queue[waiting++ * 32 + lane] = v[q];
+        if (q % 4 == 3 && __any_sync(0xffffffffu, waiting > 4)) flush();
+      }
+    });
+  flush();
   mine = warp_sum64(mine);
-  __syncthreads();
   if (lane == 0) sh.red[warp] = mine;
   __syncthreads();
-  u64 before = 0, total = 0;
-  for (int wq = 0; wq < kWarps; ++wq) {
-    if (wq < warp) before += sh.red[wq];
-    total += sh.red[wq];
-  }
+  const u64 of_warp = sh.red[lane];
+  u64 total = warp_sum64(of_warp);
   if (tid == 0) sh.part_mass = total;
   cluster.sync();
-  total = 0;
-  for (int r = 0; r < C; ++r) {
-    const u64 p = peer(r).part_mass;
-    if (r < rank) before += p;
-    total += p;
-  }
+  const u64 part = lane < C ? peer(lane).part_mass : 0;
+  u64 before = warp_sum64(lane < rank ? part : 0);
+  const u64 here = total;
+  total = warp_sum64(part);
   const u64 draw = floor_part(u, total);
-  if (before <= draw && draw < before + mine) {
-    for (int i = r0; i < r1; i += 32) {
-      const u64 w = i + lane < r1 ? weight_at(i + lane) : 0;
-      u64 sum = w;
+  if (before <= draw && draw < before + here) {
+    u64 scan = of_warp;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const u64 v = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += v;
-      }
-      const bool hit = before + sum - w <= draw && draw < before + sum;
-      if (hit) finish(i0 + i + lane, w, total);
-      if (__any_sync(0xffffffffu, hit)) break;
-      before += __shfl_sync(0xffffffffu, sum, 31);
+    for (int o = 1; o < 32; o <<= 1) {
+      const u64 v = __shfl_up_sync(0xffffffffu, scan, o);
+      if (lane >= o) scan += v;
+    }
+    const int whose = __ffs(__ballot_sync(0xffffffffu, draw < before + scan)) - 1;
+    before += __shfl_sync(0xffffffffu, scan - of_warp, whose);
+    const int s0 = min(whose * run, blocks), s1 = min(s0 + run, blocks);
+    const int piece = (s1 - s0 + kWarps - 1) / kWarps;
+    const int p0 = min(s0 + warp * piece, s1), p1 = min(p0 + piece, s1);
+    u64 sum = 0;
+    sweep_run(p0, p1, 32, one, [&](int i, const float(&v)[kVec]) INLINE {
+#pragma unroll
+      for (int q = 0; q < kVec; ++q) sum += kept(v[q], i + q) ? weigh(v[q]) : 0;
+    });
+    sum = warp_sum64(sum);
+    __syncthreads();
+    if (lane == 0) sh.red[warp] = sum;
+    __syncthreads();
+    before += warp_sum64(lane < warp ? sh.red[lane] : 0);
+    if (before <= draw && draw < before + sum) {
+      sweep_run(p0, p1, 32, one, [&](int i, const float(&v)[kVec]) INLINE {
+        u64 w[kVec], all = 0;
+#pragma unroll
+        for (int q = 0; q < kVec; ++q) {
+          w[q] = kept(v[q], i + q) ? weigh(v[q]) : 0;
+          all += w[q];
+        }
+        u64 upto = all;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const u64 y = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += y;
+        }
+        u64 at = before + upto - all;
+#pragma unroll
+        for (int q = 0; q < kVec; ++q) {
+          if (at <= draw && draw < at + w[q]) finish(i + q, w[q], total);
+          at += w[q];
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+      });
     }
   }
   cluster.sync();
@@ -671,14 +878,11 @@ constexpr int kShared = (sizeof(Shared) + 15) / 16 * 16;
 
 template <class T>
 void launch(const SampleArgs& a, int num_sms, cudaStream_t s) {
-  // CTAs per row: enough that a slice fits shared memory, then more while
-  // there are SMs without a row.
+  // CTAs per row: more than one only while there are SMs without a row.
   int c = 1;
-  while (c < kMaxCluster &&
-         ((static_cast<int64_t>(a.vocab) + c - 1) / c * sizeof(T) > kSliceBytes ||
-          static_cast<int64_t>(a.rows) * c * 2 <= num_sms))
-    c *= 2;
+  while (c < kMaxCluster && static_cast<int64_t>(a.rows) * c * 2 <= num_sms) c *= 2;
   const int slice = (a.vocab + c - 1) / c * static_cast<int>(sizeof(T)) + 16;
+  const bool staged = slice <= kSliceBytes;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = c;
@@ -686,30 +890,36 @@ void launch(const SampleArgs& a, int num_sms, cudaStream_t s) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(a.rows) * c);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = kShared + (slice + 15) / 16 * 16;
+  cfg.dynamicSmemBytes = kShared + (staged ? (slice + 15) / 16 * 16 : 0);
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, sample_kernel<T>, a);
+  if (staged)
+    cudaLaunchKernelEx(&cfg, sample_kernel<T, true>, a);
+  else
+    cudaLaunchKernelEx(&cfg, sample_kernel<T, false>, a);
 }
 
-template <class T>
-void set_smem() {
-  cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                       kShared + kSliceBytes + 32);
+static_assert(kShared + kSliceBytes + 16 <= 227 * 1024, "shared memory");
+
+template <class T, bool STAGED>
+void set_attributes() {
+  cudaFuncSetAttribute(sample_kernel<T, STAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                       kShared + (STAGED ? kSliceBytes + 16 : 0));
+  cudaFuncSetAttribute(sample_kernel<T, STAGED>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
 }
 
 }  // namespace
 
-int sample_max_vocab(int dtype) {
-  // Slices in shared memory; and sums of 2^19 weights of 2^44 fit 64 bits.
-  return std::min(kMaxCluster * kSliceBytes / (dtype == kOpF32 ? 4 : 2), 1 << 19);
-}
+int sample_max_vocab(int) { return 1 << 19; }  // sums of 2^19 weights of 2^44 fit 64 bits
 
 void sample_setup_device() {
-  set_smem<float>();
-  set_smem<__half>();
-  set_smem<__nv_bfloat16>();
+  set_attributes<float, true>();
+  set_attributes<float, false>();
+  set_attributes<__half, true>();
+  set_attributes<__half, false>();
+  set_attributes<__nv_bfloat16, true>();
+  set_attributes<__nv_bfloat16, false>();
 }
 
 void launch_sample(const SampleArgs& a, int num_sms, cudaStream_t s) {

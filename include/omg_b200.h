@@ -562,7 +562,7 @@ typedef struct {
   const void* logits;      /* [rows] rows of vocab values, any element alignment */
   int64_t stride;          /* elements between rows */
   int32_t dtype;           /* OMG_TYPE_* */
-  int32_t rows, vocab;     /* vocab up to 327,680 (f32) or 524,288 (f16, bf16) */
+  int32_t rows, vocab;     /* vocab up to 524,288 */
   const float* u;          /* [rows] uniform numbers in [0, 1) */
   /* [rows] settings, or NULL and the one value after them for every row. */
   const float* temperature;

@@ -70,11 +70,19 @@ def test_settings(device, torch, ops, dtype, vocab, kw):
     check(torch, ops, x, uniforms(6, vocab), **kw)
 
 
-@pytest.mark.parametrize("dtype,vocab", [("f32", 327680), ("bf16", 524288), ("f16", 262144)])
+@pytest.mark.parametrize("dtype,vocab", [("f32", 327680), ("f32", 524288), ("bf16", 524288), ("f16", 262144)])
 def test_largest_vocabularies(device, torch, ops, dtype, vocab):
-    x = logits(torch, 4, vocab, 1, device, dtype)
-    for kw in (dict(), dict(top_p=0.9), dict(top_k=100000, top_p=0.95), dict(top_k=50)):
-        check(torch, ops, x, uniforms(4, 2), **kw)
+    # 4 rows: clusters of CTAs; 90: one CTA per row, which reads it three times.
+    for rows in (4, 90):
+        x = logits(torch, rows, vocab, 1, device, dtype)
+        for kw in (dict(), dict(top_p=0.9), dict(top_k=100000, top_p=0.95), dict(top_k=50)):
+            check(torch, ops, x[:90:23] if rows == 90 else x, uniforms(4, 2), **kw)
+        if rows == 90:
+            u = torch.tensor(uniforms(90, 2), device=x.device)
+            whole = ops.sample(x, u, top_p=0.9)
+            for r in range(0, 90, 29):
+                one = ops.sample(x[r:r + 1], u[r:r + 1], top_p=0.9)
+                assert one[0] == whole[0][r] and one[1] == whole[1][r]
 
 
 @pytest.mark.parametrize("rows", [1, 3, 40, 75, 200])

@@ -197,7 +197,7 @@ def test_rope_frequencies():
     (dict(dtype=3), "dtype 3"),
     (dict(rows=-1), "-1 rows"),
     (dict(vocab=0), "vocabulary of 0"),
-    (dict(vocab=327681, stride=1 << 20), "vocabulary of 327681"),
+    (dict(vocab=524289, stride=1 << 20), "vocabulary of 524289"),
     (dict(dtype=1, vocab=524289, stride=1 << 20), "vocabulary of 524289"),
     (dict(stride=99), "stride 99 < vocabulary 100"),
     (dict(logits=0), "logits is null"),
