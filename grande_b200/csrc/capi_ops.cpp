@@ -224,11 +224,11 @@ int omg_paged_attention(int device, const omg_paged_cache* cache, const omg_page
     a.scale_log2 = p->scale * 1.4426950408889634f;
     paged_attention_workspace(&a, workspace);
     DeviceScope on(device);
-    CUtensorMap tq, tkv;
+    PagedMaps maps;
     char err[256];
-    if (!paged_attention_maps(a, p->q, p->q_stride, &tq, &tkv, err, sizeof err))
+    if (!paged_attention_maps(a, p->q, p->q_stride, &maps, err, sizeof err))
       fail("%s: %s", op, err);
-    launch_paged_attention(a, tq, tkv, static_cast<cudaStream_t>(stream));
+    launch_paged_attention(a, maps, static_cast<cudaStream_t>(stream));
     CUDA_TRY(cudaGetLastError());
     return 0;
   });

@@ -72,29 +72,30 @@ void launch_paged_append(const PagedAppendArgs& a, int num_sms, cudaStream_t s);
 constexpr int kPagedTileRows = 128;
 constexpr int kPagedTileKeys = 64;
 
-// Sequence `s` in row tile `rt` (index s + rt: both ascend along the line).
-struct PagedSeg {
-  int s, rt;
-  int rows;        // r0 | r1 << 16: its rows of the tile; 0: no such pair
-  int i0;          // own index of its first token in the tile
-  int own0;        // first of its own key tiles
-  int n_own;       // their number
-  int kend;        // own keys that exist and are seen by any of its rows
-  int pad;
+// A run of key tiles of one row tile: its group's prefix, or one sequence's
+// own keys.
+struct PagedRun {
+  int cum;         // first tile on the line (of one KV head)
+  int rt;          // row tile
+  int rows;        // r0 | r1 << 16: the rows that see it
+  int i0;          // own index of row r0's token
+  int tile0, n;    // key tiles [tile0, tile0 + n) of its list of pages
+  int kend;        // keys of the list that exist (and, own: that any row sees)
+  int owner;       // the sequence; of a prefix ~group
 };
 
 struct PagedTile {
   int tok0, ntok;
-  int group, prefix_len;
-  int pre0, npre;    // prefix key tiles
+  int prefix_len;
   int cum, ntiles;   // its range of the line of one KV head
-  int seg0, nseg;    // its segments are seg0 .. seg0 + nseg
+  int run0, nruns;
   int imin, imax;    // own indices of its rows
+  int pad[3];
 };
 
 struct PagedPlan {
   int n_tiles;    // row tiles
-  int n_segs;
+  int n_runs;
   int line;       // key tiles of one KV head
   int pad;
 };
@@ -109,25 +110,28 @@ struct PagedAttnArgs {
   float scale_log2;     // score scale x log2(e)
   // Workspace.
   PagedPlan* plan;
-  int* seg_cum;         // [max_segs + 1] first line tile of each segment
-  PagedSeg* segs;       // [max_segs]
+  int* run_cum;         // [max_runs + 1] first line tile of each run
+  PagedRun* runs;       // [max_runs + 1]
   PagedTile* tiles;     // [max_tiles]
   float* part_o;        // [2 * ctas][128][hd]
   float2* part_ml;      // [2 * ctas][128]
-  int max_tiles, max_segs;
+  int max_tiles, max_segs, max_runs;  // segments: (sequence, row tile) pairs
   int ctas, min_tiles;  // grid of the attention kernel; least line tiles per CTA
 };
 
-// Sizes of a call: fills max_tiles, max_segs, ctas, min_tiles of `a` from its
+// Sizes of a call: fills max_tiles .. max_runs, ctas, min_tiles of `a` from its
 // batch and shape and returns the workspace bytes (0: more sequences and row
 // tiles than the plan kernel holds).
 size_t paged_attention_layout(PagedAttnArgs* a, int num_sms);
 // Point the workspace members of `a` into `ws`.
 void paged_attention_workspace(PagedAttnArgs* a, void* ws);
-bool paged_attention_maps(const PagedAttnArgs& a, const void* q, int64_t q_stride,
-                          CUtensorMap* tq, CUtensorMap* tkv, char* err, size_t errlen);
-void launch_paged_attention(const PagedAttnArgs& a, const CUtensorMap& tq, const CUtensorMap& tkv,
-                            cudaStream_t s);
+// Tensor maps: q, and the cache in boxes of up to 64 rows and of 16.
+struct PagedMaps {
+  CUtensorMap q, kv, kv16;
+};
+bool paged_attention_maps(const PagedAttnArgs& a, const void* q, int64_t q_stride, PagedMaps* m,
+                          char* err, size_t errlen);
+void launch_paged_attention(const PagedAttnArgs& a, const PagedMaps& m, cudaStream_t s);
 // Shared-memory limits of its kernels (once per device).
 void paged_attention_setup_device();
 

@@ -67,32 +67,35 @@ struct Shape {
 
 struct PlanSmem {
   int *gs, *gtok, *gtile;                // [groups + 1]: first sequence, token, row tile
-  int *imin, *imax, *own, *seg0, *seg1;  // [max_tiles]
-  int* cnt;                              // [max_segs] line tiles of each segment
+  int *imin, *imax, *npre, *seg0, *seg1; // [max_tiles]
+  int *seg_rt, *seg_n;                   // [max_segs]: row tile (-1: none), own key tiles
 };
 
-__host__ __device__ inline size_t plan_smem_ints(int groups, int max_tiles, int max_segs) {
-  return 3 * (static_cast<size_t>(groups) + 1) + 5 * static_cast<size_t>(max_tiles) + max_segs;
+// Arrays of 2 * max_segs first (they become 64-bit scan results).
+__host__ __device__ inline size_t plan_smem_ints(int64_t groups, int64_t max_tiles,
+                                                 int64_t max_segs) {
+  return 3 * (groups + 1) + 5 * max_tiles + 2 * max_segs;
 }
 
 // Exclusive scan of v over the block, plus `carry`; returns the block's total.
-__device__ __forceinline__ int block_scan(int v, int* excl) {
-  __shared__ int ws[32];
-  __shared__ int total;
+template <class N>
+__device__ __forceinline__ N block_scan(N v, N* excl) {
+  __shared__ N ws[32];
+  __shared__ N total;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int x = v;
+  N x = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    const N y = __shfl_up_sync(0xffffffffu, x, o);
     if (lane >= o) x += y;
   }
   if (lane == 31) ws[warp] = x;
   __syncthreads();
   if (warp == 0) {
-    int w = ws[lane];
+    N w = ws[lane];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, w, o);
+      const N y = __shfl_up_sync(0xffffffffu, w, o);
       if (lane >= o) w += y;
     }
     if (lane == 31) total = w;
@@ -100,7 +103,7 @@ __device__ __forceinline__ int block_scan(int v, int* excl) {
   }
   __syncthreads();
   *excl = x - v + (warp ? ws[warp - 1] : 0);
-  const int t = total;
+  const N t = total;
   __syncthreads();
   return t;
 }
@@ -118,19 +121,42 @@ __device__ __forceinline__ int last_le(const int* a, int n, int v) {
   return lo - 1;
 }
 
+// Sequence s in row tile k of its group (token range [t0, t0 + tpt)).
+struct Seg {
+  int r0, r1;     // rows
+  int i0, i1;     // own indices of its first and last token there
+  int tile0, n;   // own key tiles
+  int kend;
+};
+__device__ __forceinline__ Seg segment(const PagedAttnArgs& a, int s, int q0, int q1, int t0,
+                                       int own_cap) {
+  Seg g;
+  const int ta = max(q0, t0), tb = min(q1, t0 + a.tpt);
+  g.i0 = a.b.lens[s] - (a.b.q_start[s + 1] - ta);
+  g.i1 = g.i0 + (tb - ta) - 1;
+  g.r0 = (ta - t0) * a.hpg;
+  g.r1 = (tb - t0) * a.hpg;
+  g.kend = min(g.i1 + 1, own_cap);
+  const int lo = a.window > 0 ? max(0, g.i0 - a.window + 1) : 0;
+  g.tile0 = lo / kKeys;
+  g.n = g.kend > lo ? (g.kend + kKeys - 1) / kKeys - g.tile0 : 0;
+  return g;
+}
+
 __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedAttnArgs a) {
-  extern __shared__ int sm[];
+  extern __shared__ __align__(16) int sm[];
   const int groups = max(a.b.n_groups, 1), S = a.b.n_seqs, T = a.b.tokens;
   PlanSmem m;
-  m.gs = sm;
+  m.seg_rt = sm;
+  m.seg_n = m.seg_rt + a.max_segs;
+  m.gs = m.seg_n + a.max_segs;
   m.gtok = m.gs + groups + 1;
   m.gtile = m.gtok + groups + 1;
   m.imin = m.gtile + groups + 1;
   m.imax = m.imin + a.max_tiles;
-  m.own = m.imax + a.max_tiles;
-  m.seg0 = m.own + a.max_tiles;
+  m.npre = m.imax + a.max_tiles;
+  m.seg0 = m.npre + a.max_tiles;
   m.seg1 = m.seg0 + a.max_tiles;
-  m.cnt = m.seg1 + a.max_tiles;
   const int tid = threadIdx.x;
   griddep_wait();
   griddep_launch();
@@ -143,13 +169,13 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedAttnArgs 
     m.gtok[g] = min(max(a.b.q_start[s], 0), T);
   }
   for (int i = tid; i < a.max_segs; i += kPlanThreads) {
-    m.cnt[i] = 0;
-    a.segs[i].rows = 0;
+    m.seg_rt[i] = -1;
+    m.seg_n[i] = 0;
   }
   for (int i = tid; i < a.max_tiles; i += kPlanThreads) {
     m.imin[i] = INT_MAX;
     m.imax[i] = INT_MIN;
-    m.own[i] = 0;
+    m.npre[i] = 0;  // until the prefix's are known: the own tiles
     m.seg0[i] = INT_MAX;
     m.seg1[i] = -1;
   }
@@ -167,144 +193,167 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedAttnArgs 
   if (tid == 0) m.gtile[groups] = n_tiles;
   __syncthreads();
 
-  // (sequence, row tile) pairs.
   const int own_cap = a.b.max_pages << a.c.page_log2;
-  for (int s = tid; s < S; s += kPlanThreads) {
-    const int g = last_le(m.gs, groups + 1, s);
-    if (g < 0 || g >= groups) continue;
-    const int q0 = max(a.b.q_start[s], m.gtok[g]);
-    const int q1 = min(a.b.q_start[s + 1], m.gtok[g + 1]);
-    if (q0 >= q1) continue;
-    const int len = a.b.lens[s];
-    const int first = len - (a.b.q_start[s + 1] - q0);  // own index of token q0
-    for (int k = (q0 - m.gtok[g]) / a.tpt; k <= (q1 - 1 - m.gtok[g]) / a.tpt; ++k) {
-      const int rt = m.gtile[g] + k;
-      const int t0 = m.gtok[g] + k * a.tpt;
-      if (rt >= n_tiles) break;
-      const int ta = max(q0, t0), tb = min(q1, t0 + a.tpt);
-      const int i0 = first + (ta - q0), i1 = i0 + (tb - ta) - 1;
-      PagedSeg sg;
-      sg.s = s;
-      sg.rt = rt;
-      sg.rows = ((ta - t0) * a.hpg) | (((tb - t0) * a.hpg) << 16);
-      sg.i0 = i0;
-      sg.kend = min(i1 + 1, own_cap);
-      const int lo = a.window > 0 ? max(0, i0 - a.window + 1) : 0;
-      sg.own0 = lo / kKeys;
-      sg.n_own = max(0, (sg.kend + kKeys - 1) / kKeys - sg.own0);
-      if (sg.kend <= lo) sg.n_own = 0;
-      sg.pad = 0;
-      const int at = s + rt;
-      a.segs[at] = sg;
-      m.cnt[at] = sg.n_own;
-      atomicMin(&m.imin[rt], i0);
-      atomicMax(&m.imax[rt], i1);
-      atomicAdd(&m.own[rt], sg.n_own);
-      atomicMin(&m.seg0[rt], at);
-      atomicMax(&m.seg1[rt], at);
+  const int pre_cap = a.b.n_groups > 0 ? a.b.max_prefix_pages << a.c.page_log2 : 0;
+  // f(sequence, row tile, segment) for every pair that shares tokens.
+  auto each_segment = [&](auto f) {
+    for (int s = tid; s < S; s += kPlanThreads) {
+      const int g = last_le(m.gs, groups + 1, s);
+      if (g < 0 || g >= groups) continue;
+      const int q0 = max(a.b.q_start[s], m.gtok[g]);
+      const int q1 = min(a.b.q_start[s + 1], m.gtok[g + 1]);
+      if (q0 >= q1) continue;
+      for (int k = (q0 - m.gtok[g]) / a.tpt; k <= (q1 - 1 - m.gtok[g]) / a.tpt; ++k) {
+        const int rt = m.gtile[g] + k;
+        if (rt >= n_tiles) break;
+        f(s, rt, segment(a, s, q0, q1, m.gtok[g] + k * a.tpt, own_cap));
+      }
     }
+  };
+  each_segment([&](int s, int rt, const Seg& sg) {
+    m.seg_rt[s + rt] = rt;
+    m.seg_n[s + rt] = sg.n;
+    atomicMin(&m.imin[rt], sg.i0);
+    atomicMax(&m.imax[rt], sg.i1);
+    atomicAdd(&m.npre[rt], sg.n);
+    atomicMin(&m.seg0[rt], s + rt);
+    atomicMax(&m.seg1[rt], s + rt);
+  });
+  __syncthreads();
+
+  // The prefix's key tiles come before the first segment's own. Rows that see
+  // nothing at all still get their zeros: one key tile, all of it masked.
+  auto prefix_range = [&](int rt, int* tile0, int* end) -> int {
+    const int g = last_le(m.gtile, groups, rt);
+    const int plen = a.b.n_groups > 0 ? max(a.b.prefix_lens[g], 0) : 0;
+    *end = min(plen, pre_cap);
+    const int lo = a.window > 0 ? max(0, plen + m.imin[rt] - a.window + 1) : 0;
+    *tile0 = lo / kKeys;
+    return lo < *end ? (*end + kKeys - 1) / kKeys - *tile0 : 0;
+  };
+  for (int rt = tid; rt < n_tiles; rt += kPlanThreads) {
+    int tile0, end;
+    const int pre = m.seg1[rt] >= 0 ? prefix_range(rt, &tile0, &end) : 0;
+    m.npre[rt] = m.seg1[rt] < 0 ? 0 : pre + m.npre[rt] == 0 ? 1 : pre;
   }
   __syncthreads();
 
-  // Row tiles: the prefix's key tiles come before the first segment's own.
-  const int pre_cap = a.b.n_groups > 0 ? a.b.max_prefix_pages << a.c.page_log2 : 0;
+  // Places of the runs, and of their tiles on the line.
+  using u64 = unsigned long long;
+  const int n_segs = S + n_tiles;
+  u64 carry = 0;  // tiles << 32 | runs
+  for (int i0 = 0; i0 < n_segs; i0 += kPlanThreads) {
+    const int i = i0 + tid;
+    u64 v = 0;
+    if (i < n_segs && m.seg_rt[i] >= 0) {
+      const int rt = m.seg_rt[i], own = m.seg_n[i], pre = m.seg0[rt] == i ? m.npre[rt] : 0;
+      v = (static_cast<u64>(own + pre) << 32) | ((own > 0) + (pre > 0));
+    }
+    u64 at;
+    const u64 total = block_scan(v, &at);
+    at += carry;
+    if (i < n_segs) {
+      // (In place: nothing else reads entry i any more.)
+      m.seg_rt[i] = static_cast<int>(at);
+      m.seg_n[i] = static_cast<int>(at >> 32);
+    }
+    carry += total;
+  }
+  const int n_runs = static_cast<int>(carry & 0xffffffffu), line = static_cast<int>(carry >> 32);
+  __syncthreads();
+
+  each_segment([&](int s, int rt, const Seg& sg) {
+    if (sg.n == 0) return;
+    const int pre = m.seg0[rt] == s + rt ? m.npre[rt] : 0;
+    const int at = m.seg_rt[s + rt] + (pre > 0), cum = m.seg_n[s + rt] + pre;
+    a.runs[at] = PagedRun{cum, rt, sg.r0 | (sg.r1 << 16), sg.i0, sg.tile0, sg.n, sg.kend, s};
+    a.run_cum[at] = cum;
+  });
   for (int rt = tid; rt < n_tiles; rt += kPlanThreads) {
     const int g = last_le(m.gtile, groups, rt);
-    PagedTile t;
+    PagedTile t{};
     t.tok0 = m.gtok[g] + (rt - m.gtile[g]) * a.tpt;
     t.ntok = min(a.tpt, m.gtok[g + 1] - t.tok0);
-    t.group = g;
     t.prefix_len = a.b.n_groups > 0 ? max(a.b.prefix_lens[g], 0) : 0;
-    t.seg0 = m.seg0[rt];
-    t.nseg = m.seg1[rt] - m.seg0[rt] + 1;
     t.imin = m.imin[rt];
     t.imax = m.imax[rt];
-    t.pre0 = t.npre = t.cum = t.ntiles = 0;
     if (m.seg1[rt] >= 0) {
-      const int end = min(t.prefix_len, pre_cap);
-      const int lo = a.window > 0 ? max(0, t.prefix_len + t.imin - a.window + 1) : 0;
-      if (lo < end) {
-        t.pre0 = lo / kKeys;
-        t.npre = (end + kKeys - 1) / kKeys - t.pre0;
+      const int first = m.seg0[rt], last = m.seg1[rt] + 1;
+      t.run0 = m.seg_rt[first];
+      t.cum = m.seg_n[first];
+      t.nruns = (last < n_segs ? m.seg_rt[last] : n_runs) - t.run0;
+      t.ntiles = (last < n_segs ? m.seg_n[last] : line) - t.cum;
+      if (m.npre[rt] > 0) {
+        int tile0, end;
+        const int pre = prefix_range(rt, &tile0, &end);
+        a.runs[t.run0] = PagedRun{t.cum, rt, (t.ntok * a.hpg) << 16, 0, pre ? tile0 : 0,
+                                  m.npre[rt], pre ? end : 0, ~g};
+        a.run_cum[t.run0] = t.cum;
       }
-      // Rows that see nothing at all still get their zeros: one key tile,
-      // all of it masked.
-      if (t.npre + m.own[rt] == 0) t.npre = 1;
-      t.ntiles = t.npre + m.own[rt];
-      m.cnt[t.seg0] += t.npre;
     }
     a.tiles[rt] = t;
   }
-  __syncthreads();
-
-  const int n_segs = S + n_tiles;
-  int line = 0;
-  for (int i0 = 0; i0 < n_segs; i0 += kPlanThreads) {
-    const int i = i0 + tid;
-    int at;
-    const int total = block_scan(i < n_segs ? m.cnt[i] : 0, &at);
-    if (i < n_segs) {
-      a.seg_cum[i] = line + at;
-      const int rt = a.segs[i].rows ? a.segs[i].rt : -1;
-      if (rt >= 0 && m.seg0[rt] == i) a.tiles[rt].cum = line + at;
-    }
-    line += total;
-  }
   if (tid == 0) {
-    a.seg_cum[n_segs] = line;
-    *a.plan = PagedPlan{n_tiles, n_segs, line, 0};
+    a.run_cum[n_runs] = line;
+    *a.plan = PagedPlan{n_tiles, n_runs, line, 0};
   }
 }
 
 // ---- attention ----------------------------------------------------------------
 
-// A position on the line, walked tile by tile by each role.
-struct Walk {
-  PagedTile t;   // row tile
-  PagedSeg sg;   // segment whose own keys come next or are being read
-  int kv, rt;    // KV head, row tile
-  int pos, end;  // tile of the row tile, and where this CTA's range leaves it
-  int seg, sub;  // segment index; own tile within it
-
-  __device__ __forceinline__ void load_seg(const PagedAttnArgs& a) {
-    while (a.segs[seg].rows == 0 || a.segs[seg].n_own == 0) {
-      if (seg + 1 >= t.seg0 + t.nseg) break;
-      ++seg;
+// A ring position and the parity of its current use.
+template <int N>
+struct Ring {
+  int s = 0;
+  uint32_t ph = 0;
+  __device__ __forceinline__ void next() {
+    if (++s == N) {
+      s = 0;
+      ph ^= 1;
     }
-    sg = a.segs[seg];
   }
-  // Enter the line at tile w of [w, w1); a full warp calls it.
-  __device__ __forceinline__ void enter(const PagedAttnArgs& a, const PagedPlan& p, int w, int w1,
+};
+
+// The runs of a CTA's range [w, w1) of the line, in order. Each role walks
+// them by itself; the next run's record is asked for while the current one is
+// worked on (a record is an L2 latency away, a run can be one tile).
+struct Runs {
+  PagedRun run, next;
+  int kv, r;
+  int off;       // first tile of the run that is this CTA's
+  int w, w1;
+
+  // A full warp calls it, with w < w1.
+  __device__ __forceinline__ void enter(const PagedAttnArgs& a, const PagedPlan& p, int w_, int w1_,
                                         int lane) {
+    w = w_;
+    w1 = w1_;
     kv = w / p.line;
     const int wl = w - kv * p.line;
-    seg = warp_count_le(a.seg_cum, p.n_segs, wl, lane) - 1;
-    rt = a.segs[seg].rt;
-    t = a.tiles[rt];
-    pos = wl - t.cum;
-    end = min(t.ntiles, pos + (w1 - w));
-    if (pos < t.npre) {
-      seg = t.seg0;
-      sub = 0;
-    } else {
-      sub = wl - a.seg_cum[seg] - (seg == t.seg0 ? t.npre : 0);
-    }
-    load_seg(a);
+    r = warp_count_le(a.run_cum, p.n_runs, wl, lane) - 1;
+    run = a.runs[r];
+    off = wl - run.cum;
+    fetch(a, p);
   }
-  __device__ __forceinline__ bool prefix() const { return pos < t.npre; }
-  // Key tile number in its list of pages.
-  __device__ __forceinline__ int key_tile() const {
-    return prefix() ? t.pre0 + pos : sg.own0 + sub;
+  __device__ __forceinline__ void fetch(const PagedAttnArgs& a, const PagedPlan& p) {
+    next = a.runs[r + 1 == p.n_runs ? 0 : r + 1];
   }
-  __device__ __forceinline__ void next(const PagedAttnArgs& a) {
-    if (!prefix()) {
-      if (++sub == sg.n_own && pos + 1 < t.ntiles) {
-        ++seg;
-        sub = 0;
-        load_seg(a);
-      }
+  // Tiles of the run that are this CTA's.
+  __device__ __forceinline__ int count() const { return min(run.n - off, w1 - w); }
+  // Whether more of the same row tile and KV head follows the run.
+  __device__ __forceinline__ bool more(const PagedPlan& p, int n) const {
+    return w + n < w1 && off + n == run.n && r + 1 < p.n_runs && next.rt == run.rt;
+  }
+  // Past the run's n tiles.
+  __device__ __forceinline__ void step(const PagedAttnArgs& a, const PagedPlan& p, int n) {
+    w += n;
+    off = 0;
+    run = next;
+    if (++r == p.n_runs) {
+      r = 0;
+      ++kv;
     }
-    ++pos;
+    if (w < w1) fetch(a, p);
   }
 };
 
@@ -323,11 +372,11 @@ __device__ __forceinline__ uint64_t bits_between(int a, int b) {
   return hi & ~((1ull << a) - 1);
 }
 
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
-                                          int lane) {
-  int ok = 0;
-  if (lane == 0) ok = mbar_wait(bar, parity, abort_flag, nullptr) ? 1 : 0;
-  return __shfl_sync(0xffffffffu, ok, 0) != 0;
+// Every lane waits: a warp that is not split needs no broadcast.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity,
+                                          volatile int* abort_flag) {
+  const bool ok = mbar_wait(bar, parity, abort_flag, nullptr);
+  return __all_sync(0xffffffffu, ok);
 }
 
 template <class T>
@@ -360,8 +409,7 @@ constexpr long long kDrainClocks = 1ll << 28;
 
 template <int HD, class T>
 __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
-    paged_attention_kernel(const __grid_constant__ CUtensorMap tq,
-                           const __grid_constant__ CUtensorMap tkv, PagedAttnArgs a) {
+    paged_attention_kernel(const __grid_constant__ PagedMaps maps, PagedAttnArgs a) {
   using Sh = Shape<HD>;
   constexpr int VD = Sh::kV, NST = Sh::kStages, CH = Sh::kChunks;
   extern __shared__ uint8_t smem_raw[];
@@ -391,8 +439,9 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
     *abort_flag = 0;
     for (int i = 0; i < 8; ++i) bad_keys[i] = 0;
     fence_barrier_init();
-    prefetch_tmap(&tq);
-    prefetch_tmap(&tkv);
+    prefetch_tmap(&maps.q);
+    prefetch_tmap(&maps.kv);
+    prefetch_tmap(&maps.kv16);
   }
   if (warp == 1) tmem_alloc(tmem_slot, Sh::kTmemCols);
   tc_fence_before();
@@ -407,158 +456,227 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
   const int per = max((total + a.ctas - 1) / a.ctas, a.min_tiles);
   const int w0 = min(static_cast<int>(blockIdx.x) * per, total);
   const int w1 = min(w0 + per, total);
-  const int pre_cap = a.b.n_groups > 0 ? a.b.max_prefix_pages << a.c.page_log2 : 0;
   constexpr int KST = Sh::kHalves;  // ring stages of a K tile (V: one)
 
-  if (warp == 0) {
-    // ---- loads: Q of each row tile; per tile K then, one tile behind, V.
-    const int box = min(1 << a.c.page_log2, kKeys);  // rows per TMA box
-    const int nbox = kKeys / box;
-    const int lb = lane % nbox, lc = lane / nbox;
-    int it = 0, nk = 0, nv = 0, nq = 0;
-    bool ok = true;
-    // First cache row of this lane's box of the walk's tile (-1: past the
-    // keys that exist, nothing to load; a page outside the pool lies past
-    // the map's end, where TMA fills zeros).
-    auto box_row = [&](const Walk& w) -> int {
-      const int key = w.key_tile() * kKeys + lb * box;
-      const bool pre = w.prefix();
-      const int kend = pre ? min(w.t.prefix_len, pre_cap) : w.sg.kend;
-      if (key >= kend) return -1;
-      const int pi = key >> a.c.page_log2;
-      const int* table =
-          pre ? a.b.prefix_pages + static_cast<int64_t>(w.t.group) * a.b.max_prefix_pages
-              : a.b.pages + static_cast<int64_t>(w.sg.s) * a.b.max_pages;
-      int page = table[pi];
-      if (page < 0 || page >= a.c.n_pages) page = static_cast<int>(a.c.n_pages);
-      return (page << a.c.page_log2) + (key & ((1 << a.c.page_log2) - 1));
-    };
-    // One ring stage: dims [x, x + kV) of the tile's keys.
-    auto load_stage = [&](int row, int x, bool is_v) {
-      const int s = it % NST, n = it / NST;
-      if (n > 0 && !warp_wait(&empty[s], (n - 1) & 1, abort_flag, lane)) {
+  if (w0 >= w1) {
+    // Nothing of the line: on to the end.
+  } else if (warp == 0) {
+    // ---- loads: Q of each row tile; per tile K and then V of the one before.
+    Ring<NST> slot, kr, vr;
+    uint32_t qphase = 0;
+    int issued_k = 0, issued_v = 0;  // for the drain
+    bool ok = true, first_q = true;
+    const int lg = a.c.page_log2, full_box = min(1 << lg, kKeys);
+    const int full_log2 = min(lg, 6);
+    // One ring stage: dims [x, x + kV) of `row`'s boxes.
+    auto load_stage = [&](int row, int box, int lb, int lc, int x, bool is_v) {
+      if (!warp_wait(&empty[slot.s], slot.ph ^ 1, abort_flag)) {
         ok = false;
         return;
       }
-      ++it;
-      uint64_t* full = is_v ? &vfull[nv++ % NST] : &kfull[nk++ % NST];
-      const uint32_t live = __popc(__ballot_sync(0xffffffffu, row >= 0 && lc < CH));
+      uint64_t* full = is_v ? &vfull[vr.s] : &kfull[kr.s];
+      const bool on = row >= 0 && lc < CH;
+      const uint32_t live = __popc(__ballot_sync(0xffffffffu, on));
       if (lane == 0) mbar_arrive_expect_tx(full, live * box * 128);
       __syncwarp();
-      if (row >= 0 && lc < CH)
-        tma_load_2d(ring + s * Sh::kStage + lc * kKvChunk + lb * box * 128, &tkv, full,
-                    x + lc * 64, row);
+      if (on)
+        tma_load_2d(ring + slot.s * Sh::kStage + lc * kKvChunk + lb * box * 128,
+                    box == full_box ? &maps.kv : &maps.kv16, full, x + lc * 64, row);
+      slot.next();
+      if (is_v) {
+        vr.next();
+        ++issued_v;
+      } else {
+        kr.next();
+        ++issued_k;
+      }
     };
-    for (int w = w0; w < w1 && ok;) {
-      Walk wk;
-      wk.enter(a, plan, w, w1, lane);
-      if (nq > 0 && !warp_wait(&bars[B_QFREE], (nq - 1) & 1, abort_flag, lane)) break;
+    Runs u;
+    u.enter(a, plan, w0, w1, lane);
+    while (u.w < w1 && ok) {
+      // One row tile's share.
+      const int rt = u.run.rt, kv = u.kv;
+      const int kx = kv * HD, vx = (a.c.kv_heads + kv) * HD + vhalf * VD;
+      if (!first_q) {
+        if (!warp_wait(&bars[B_QFREE], qphase, abort_flag)) break;
+        qphase ^= 1;
+      }
+      first_q = false;
       if (lane == 0) {
+        const int tok0 = a.tiles[rt].tok0;
         mbar_arrive_expect_tx(&bars[B_Q], HD * 2u * static_cast<uint32_t>(a.hpg * a.tpt));
 #pragma unroll 1
         for (int c = 0; c < HD / 64; ++c)
-          tma_load_4d(qs + c * kQChunk, &tq, &bars[B_Q], c * 64, 0, wk.kv, wk.t.tok0);
+          tma_load_4d(qs + c * kQChunk, &maps.q, &bars[B_Q], c * 64, 0, kv, tok0);
       }
       __syncwarp();
-      ++nq;
-      const int n = wk.end - wk.pos;
-      const int kx = wk.kv * HD, vx = (a.c.kv_heads + wk.kv) * HD + vhalf * VD;
-      int row = box_row(wk);
-      for (int u = 0; u < KST && ok; ++u) load_stage(row, kx + u * VD, false);
-      for (int j = 0; j < n && ok; ++j) {
-        int ahead = -1;
-        if (j + 1 < n) {
-          wk.next(a);
-          ahead = box_row(wk);
-          for (int u = 0; u < KST && ok; ++u) load_stage(ahead, kx + u * VD, false);
+      // The tile before, whose V is still to be loaded.
+      int prow = -1, pbox = full_box, plb = 0, plc = 0;
+      bool pending = false, more = true;
+      while (more && ok) {
+        const int n = u.count();
+        more = u.more(plan, n);
+        const int* table =
+            u.run.owner < 0
+                ? a.b.prefix_pages + static_cast<int64_t>(~u.run.owner) * a.b.max_prefix_pages
+                : a.b.pages + static_cast<int64_t>(u.run.owner) * a.b.max_pages;
+        const int kend = u.run.kend;
+        // This lane's box of a tile: its cache row (-1: past the keys that
+        // exist; a page outside the pool lies past the map's end, where TMA
+        // fills zeros). A tile that is not full takes boxes of 16 rows, so
+        // that keys past the end cost at most 15 rows of traffic.
+        auto box_row = [&](int k0, int box_log2, int* lb, int* lc) -> int {
+          const int nlog = 6 - box_log2;
+          *lb = lane & ((1 << nlog) - 1);
+          *lc = lane >> nlog;
+          const int key = k0 + (*lb << box_log2);
+          if (key >= kend) return -1;
+          int page = table[key >> lg];
+          if (page < 0 || page >= a.c.n_pages) page = static_cast<int>(a.c.n_pages);
+          return (page << lg) + (key & ((1 << lg) - 1));
+        };
+        int k0 = (u.run.tile0 + u.off) * kKeys;
+        int blog = k0 + kKeys <= kend ? full_log2 : 4, lb, lc;
+        int row = box_row(k0, blog, &lb, &lc);
+        for (int t = 0; t < n && ok; ++t) {
+          // The next tile's pages are looked up before this one's waits.
+          const int k1 = k0 + kKeys, blog1 = k1 + kKeys <= kend ? full_log2 : 4;
+          int lb1 = 0, lc1 = 0;
+          const int row1 = t + 1 < n ? box_row(k1, blog1, &lb1, &lc1) : -1;
+#pragma unroll
+          for (int h = 0; h < KST; ++h)
+            if (ok) load_stage(row, 1 << blog, lb, lc, kx + h * VD, false);
+          if (pending && ok) load_stage(prow, pbox, plb, plc, vx, true);
+          pending = true;
+          prow = row;
+          pbox = 1 << blog;
+          plb = lb;
+          plc = lc;
+          row = row1;
+          blog = blog1;
+          lb = lb1;
+          lc = lc1;
+          k0 = k1;
         }
-        if (ok) load_stage(row, vx, true);
-        row = ahead;
+        u.step(a, plan, n);
       }
-      w += n;
+      if (ok) load_stage(prow, pbox, plb, plc, vx, true);
     }
     if (*abort_flag && lane == 0) {
       // Gave up: wait (bounded) for the copies in flight into this CTA.
-      for (int i = max(0, nk - NST); i < nk; ++i)
+      for (int i = max(0, issued_k - NST); i < issued_k; ++i)
         mbar_drain(&kfull[i % NST], (i / NST) & 1, kDrainClocks);
-      for (int i = max(0, nv - NST); i < nv; ++i)
+      for (int i = max(0, issued_v - NST); i < issued_v; ++i)
         mbar_drain(&vfull[i % NST], (i / NST) & 1, kDrainClocks);
-      if (nq > 0) mbar_drain(&bars[B_Q], (nq - 1) & 1, kDrainClocks);
+      mbar_drain(&bars[B_Q], 0, kDrainClocks);
+      mbar_drain(&bars[B_Q], 1, kDrainClocks);
     }
     __syncwarp();
   } else if (warp == 1) {
-    // ---- MMA issue.
+    // ---- MMA issue: S of a tile, then P V of the one before. The whole warp
+    // runs the loop, one lane issues.
     constexpr uint32_t fs = idesc_f16_f32(kRows, kKeys), fo = idesc_f16_f32_bmn(kRows, VD);
     constexpr bool f16 = std::is_same<T, __half>::value;
     constexpr uint32_t idesc_s = f16 ? fs : idesc_bf16(fs);
     constexpr uint32_t idesc_o = f16 ? fo : idesc_bf16(fo);
-    int it = 0, nk = 0, jt = 0, nq = 0;
+    const uint64_t dq = sw128_desc(qs), dk = sw128_desc(ring), dp = sw128_desc(ps),
+                   dv = sw128_mn_desc(ring, kKvChunk);
+    Ring<NST> slot, kr, vr;
+    uint32_t qphase = 0;
+    int g = 0;  // tiles so far
     bool ok = true;
-    for (int w = w0; w < w1 && ok;) {
-      Walk wk;
-      wk.enter(a, plan, w, w1, lane);
-      const int n = wk.end - wk.pos;
+    // O += P V of tile `at` for the lanes not in `off`, its first `steps` x 16 keys.
+    auto issue_pv = [&](int at, const uint32_t (&off)[4], int steps) -> bool {
+      const int b = at & 1;
+      if (!warp_wait(&bars[B_P0 + b], (at >> 1) & 1, abort_flag) ||
+          !warp_wait(&vfull[vr.s], vr.ph, abort_flag))
+        return false;
+      tc_fence_after();
       if (lane == 0) {
-        auto issue_s = [&](int j) -> bool {
-          const int b = (jt + j) & 1;
-#pragma unroll 1
-          for (int u = 0; u < KST; ++u, ++it, ++nk) {
-            const int s = it % NST;
-            if (!mbar_wait(&kfull[nk % NST], (nk / NST) & 1, abort_flag, nullptr)) return false;
-            tc_fence_after();
+        const uint64_t pa = dp + b * (kPBytes >> 4), vb = dv + slot.s * (Sh::kStage >> 4);
 #pragma unroll
-            for (int c = 0; c < CH; ++c) {
-              const uint64_t da = sw128_desc(qs + (u * CH + c) * kQChunk);
-              const uint64_t db = sw128_desc(ring + s * Sh::kStage + c * kKvChunk);
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                umma_f16(tmem + b * kKeys, da + 2 * k, db + 2 * k, idesc_s, (u | c | k) ? 1u : 0u);
-            }
-            umma_commit(&empty[s]);
-          }
-          umma_commit(&bars[B_S0 + b]);
-          if (j + 1 == n) umma_commit(&bars[B_QFREE]);
-          return true;
-        };
-        ok = mbar_wait(&bars[B_Q], nq & 1, abort_flag, nullptr) && issue_s(0);
-        for (int j = 0; ok && j < n; ++j) {
-          // S one tile ahead; its buffer's last reader finished before the P
-          // of two tiles back, waited for below.
-          if (j + 1 < n && !issue_s(j + 1)) {
-            ok = false;
-            break;
-          }
-          const int g = jt + j, b = g & 1;
-          const int s = it % NST;
-          if (!mbar_wait(&bars[B_P0 + b], (g >> 1) & 1, abort_flag, nullptr) ||
-              !mbar_wait(&vfull[g % NST], (g / NST) & 1, abort_flag, nullptr)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          uint32_t off[4] = {0, 0, 0, 0};
-          if (!wk.prefix()) {
-            const int r0 = wk.sg.rows & 0xffff, r1 = wk.sg.rows >> 16;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              off[i] = ~static_cast<uint32_t>(bits_between(r0 - 32 * i, min(r1 - 32 * i, 32)));
-          }
-#pragma unroll
-          for (int kk = 0; kk < kKeys / 16; ++kk) {
-            const uint64_t pa = sw128_desc(ps + b * kPBytes) + 2 * kk;
-            const uint64_t vb = sw128_mn_desc(ring + s * Sh::kStage + kk * 2048, kKvChunk);
-            umma_f16_lanes(tmem + Sh::kTmemO, pa, vb, idesc_o, 1u, off);
-          }
-          umma_commit(&bars[B_O0 + b]);
-          umma_commit(&empty[s]);
-          ++it;
-          if (j + 1 < n) wk.next(a);
-        }
+        for (int kk = 0; kk < kKeys / 16; ++kk)
+          if (kk < steps)
+            umma_f16_lanes(tmem + Sh::kTmemO, pa + 2 * kk, vb + kk * (2048 >> 4), idesc_o, 1u, off);
+        umma_commit(&bars[B_O0 + b]);
+        umma_commit(&empty[slot.s]);
       }
-      ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-      ++nq;
-      jt += n;
-      w += n;
+      __syncwarp();
+      slot.next();
+      vr.next();
+      return true;
+    };
+    Runs u;
+    u.enter(a, plan, w0, w1, lane);
+    while (u.w < w1 && ok) {
+      if (!warp_wait(&bars[B_Q], qphase, abort_flag)) {
+        ok = false;
+        break;
+      }
+      qphase ^= 1;
+      bool pending = false, more = true;
+      uint32_t poff[4] = {0, 0, 0, 0};
+      int psteps = 4;
+      while (more && ok) {
+        const int n = u.count();
+        more = u.more(plan, n);
+        uint32_t off[4] = {0, 0, 0, 0};
+        if (u.run.owner >= 0) {
+          const int r0 = u.run.rows & 0xffff, r1 = u.run.rows >> 16;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int lo = min(max(r0 - 32 * i, 0), 32), hi = min(max(r1 - 32 * i, 0), 32);
+            // Lanes [lo, hi) stay on.
+            const uint32_t below_hi = hi == 32 ? ~0u : (1u << hi) - 1;
+            const uint32_t below_lo = lo == 32 ? ~0u : (1u << lo) - 1;
+            off[i] = ~(below_hi & ~below_lo);
+          }
+        }
+        int left = u.run.kend - (u.run.tile0 + u.off) * kKeys;
+        for (int t = 0; t < n; ++t, left -= kKeys) {
+          const int b = g & 1;
+          // The score buffer's last reader finished before the P of two tiles
+          // back, waited for with that tile's P V.
+#pragma unroll
+          for (int h = 0; h < KST; ++h) {
+            if (!warp_wait(&kfull[kr.s], kr.ph, abort_flag)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            if (lane == 0) {
+              const uint64_t kd = dk + slot.s * (Sh::kStage >> 4);
+#pragma unroll
+              for (int c = 0; c < CH; ++c)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  umma_f16(tmem + b * kKeys, dq + (h * CH + c) * (kQChunk >> 4) + 2 * k,
+                           kd + c * (kKvChunk >> 4) + 2 * k, idesc_s, (h | c | k) ? 1u : 0u);
+              umma_commit(&empty[slot.s]);
+              if (h == KST - 1) umma_commit(&bars[B_S0 + b]);
+            }
+            __syncwarp();
+            slot.next();
+            kr.next();
+          }
+          if (!ok) break;
+          if (pending && !issue_pv(g - 1, poff, psteps)) {
+            ok = false;
+            break;
+          }
+          pending = true;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) poff[i] = off[i];
+          psteps = left >= kKeys ? 4 : (max(left, 1) + 15) >> 4;
+          ++g;
+        }
+        u.step(a, plan, n);
+      }
+      if (ok) {
+        if (lane == 0) umma_commit(&bars[B_QFREE]);
+        __syncwarp();
+        ok = issue_pv(g - 1, poff, psteps);
+      }
     }
     if (!ok && lane == 0) {
       // Gave up: let the MMAs in flight finish (bounded).
@@ -573,29 +691,36 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
     const int tid = threadIdx.x - 64;
     const uint32_t trow = tmem + (static_cast<uint32_t>(32 * q4) << 16);
     uint8_t* my_stage[2] = {ps + 32 * q4 * 128, ps + kPBytes + 32 * q4 * 128};
-    int it = 0, jt = 0, cleans = 0;
+    int it = 0;  // ring stages before the row tile's
+    int g = 0;   // tiles so far
+    Ring<NST> vr;
+    uint32_t clean_phase = 0;
     bool ok = true;
     // All four softmax warps meet (a bounded wait, unlike a named barrier).
     auto meet = [&]() -> bool {
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars[B_CLEAN]);
-      return warp_wait(&bars[B_CLEAN], cleans++ & 1, abort_flag, lane);
+      const bool met = warp_wait(&bars[B_CLEAN], clean_phase, abort_flag);
+      clean_phase ^= 1;
+      return met;
     };
-    for (int w = w0; w < w1;) {
-      Walk wk;
-      wk.enter(a, plan, w, w1, lane);
-      const int n = wk.end - wk.pos;
-      const int nrows = wk.t.ntok * a.hpg;
-      const bool whole = n == wk.t.ntiles;
-      // The row's own index, from its sequence's segment.
-      int own = INT_MIN / 2;
+    Runs u;
+    u.enter(a, plan, w0, w1, lane);
+    while (u.w < w1) {
+      const int kv = u.kv;
+      const bool first = u.w == w0;
+      const PagedTile tile = a.tiles[u.run.rt];
+      const int nrows = tile.ntok * a.hpg;
+      const int begin = u.w;
       const bool valid = r < nrows;
-      for (int i = wk.t.seg0; i < wk.t.seg0 + wk.t.nseg; ++i) {
-        const int rows = a.segs[i].rows, i0 = a.segs[i].i0;
+      // The row's own index, from its sequence's run.
+      int own = INT_MIN / 2;
+#pragma unroll 4
+      for (int i = tile.run0; i < tile.run0 + tile.nruns; ++i) {
+        const int rows = a.runs[i].rows, i0 = a.runs[i].i0, owner = a.runs[i].owner;
         const int r0 = rows & 0xffff;
-        if (valid && r >= r0 && r < (rows >> 16)) own = i0 + (r - r0) / a.hpg;
+        if (owner >= 0 && valid && r >= r0 && r < (rows >> 16)) own = i0 + (r - r0) / a.hpg;
       }
-      const int nstart = it;
       float m_ref = -INFINITY, l = 0.f;
       if (ok && 32 * q4 < nrows) {
         // O starts from zero: an own tile only ever touches its rows' lanes.
@@ -606,230 +731,243 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
         for (int c = 0; c < VD / 32; ++c) tmem_st32(trow + Sh::kTmemO + c * 32, z);
         tmem_st_wait();
       }
-      for (int j = 0; ok && j < n; ++j) {
-        const int g = jt + j, b = g & 1;
-        const bool pre = wk.prefix();
-        const int k0 = wk.key_tile() * kKeys;
-        const int r0 = pre ? 0 : wk.sg.rows & 0xffff, r1 = pre ? nrows : wk.sg.rows >> 16;
-        const bool mine = r >= r0 && r < r1;
-        // The row's keys of this tile; those of the tile's first and last
-        // row bound what any and what all of its rows see.
-        const int plen = wk.t.prefix_len;
-        const int cap = pre ? min(plen, pre_cap) : wk.sg.kend;
-        const int shift = pre ? plen : 0;
-        const int ifirst = pre ? wk.t.imin : wk.sg.i0;
-        const int ilast = pre ? wk.t.imax : wk.sg.i0 + (r1 - r0) / a.hpg - 1;
-        auto sees = [&](int i) -> uint64_t {
-          const int p = shift + i;
-          return bits_between((a.window > 0 ? p - a.window + 1 : 0) - k0, min(p + 1, cap) - k0);
-        };
-        const uint64_t vis = mine ? sees(own) : 0;
-        const uint64_t any =
-            bits_between((a.window > 0 ? shift + ifirst - a.window + 1 : 0) - k0,
-                         min(shift + ilast + 1, cap) - k0);
-        const uint64_t all =
-            bits_between((a.window > 0 ? shift + ilast - a.window + 1 : 0) - k0,
-                         min(shift + ifirst + 1, cap) - k0);
-        // FIFO place of this tile's V: K of tile j + 1 was loaded before it.
-        const int vi = nstart + (j + 1 < n ? 2 * KST + j * (KST + 1) : n * (KST + 1) - 1);
-        if (!warp_wait(&bars[B_S0 + b], (g >> 1) & 1, abort_flag, lane)) {
-          ok = false;
-          break;
-        }
-        uint64_t bad = 0;
-        if (any != ~0ull || all != ~0ull) {
-          // Keys that no row sees may hold anything: their V rows become
-          // zeros. Of those that only some rows see, V rows with infinities
-          // or NaN are taken out of the product and added by hand to the rows
-          // that see them, so that a masked key never reaches a row.
-          uint8_t* v = ring + (vi % NST) * Sh::kStage;
-          if (!warp_wait(&vfull[g % NST], (g / NST) & 1, abort_flag, lane)) {
+      int done = 0;  // tiles of this row tile
+      bool more = true;
+      while (more) {
+        const int n = u.count();
+        more = u.more(plan, n);
+        const bool pre = u.run.owner < 0;
+        const int r0 = u.run.rows & 0xffff, r1 = u.run.rows >> 16;
+        // (A row without own keys, whose length is short of its query rows,
+        // sees nothing.)
+        const bool mine = r >= r0 && r < r1 && own > INT_MIN / 2;
+        const bool my_warp = 32 * q4 < r1 && 32 * q4 + 32 > r0;
+        // The keys of the run that its first and last row see bound what any
+        // and what all of its rows see.
+        const int shift = pre ? tile.prefix_len : 0, cap = u.run.kend;
+        const int ifirst = shift + (pre ? tile.imin : u.run.i0);
+        const int ilast = shift + (pre ? tile.imax : u.run.i0 + (r1 - r0) / a.hpg - 1);
+        const int wlo = a.window > 0 ? a.window - 1 : INT_MAX / 2;
+        const int any_lo = max(ifirst - wlo, 0), any_hi = min(ilast + 1, cap);
+        const int all_lo = max(ilast - wlo, 0), all_hi = min(ifirst + 1, cap);
+        int k0 = (u.run.tile0 + u.off) * kKeys;
+        for (int t = 0; ok && t < n; ++t, k0 += kKeys) {
+          const int b = g & 1;
+          const bool last = !more && t + 1 == n;
+          // Ring place of this tile's V: the next tile's K was loaded before it.
+          const int vi = it + done * (KST + 1) + (last ? KST : 2 * KST);
+          if (!warp_wait(&bars[B_S0 + b], (g >> 1) & 1, abort_flag)) {
             ok = false;
             break;
           }
-          const uint64_t part = any & ~all;
-          for (int i = tid; i < kKeys * CH * 8; i += 128) {
-            const int key = (i >> 3) & (kKeys - 1), chunk = i >> 9;
-            uint4* p = reinterpret_cast<uint4*>(v + chunk * kKvChunk + key * 128 + (i & 7) * 16);
-            if (!((any >> key) & 1)) {
-              *p = make_uint4(0, 0, 0, 0);
-            } else if ((part >> key) & 1) {
-              const uint4 x = *p;
-              if (nonfinite2<T>(x.x) || nonfinite2<T>(x.y) || nonfinite2<T>(x.z) ||
-                  nonfinite2<T>(x.w))
-                atomicOr(&bad_keys[2 * (g & 3) + (key >> 5)], 1u << (key & 31));
+          uint64_t bad = 0;
+          uint64_t vis = mine ? ~0ull : 0;
+          const bool edge = k0 < all_lo || k0 + kKeys > all_hi;
+          if (edge) {
+            if (mine) {
+              const int p = shift + own;
+              vis = bits_between(max(p - wlo, 0) - k0, min(p + 1, cap) - k0);
             }
-          }
-          if (part) {
-            if (!meet()) {
+            // Keys that no row sees may hold anything: their V rows, as far
+            // as the product reads them, become zeros. Of those that only
+            // some rows see, V rows with infinities or NaN are taken out of
+            // the product and added by hand to the rows that see them, so
+            // that a masked key never reaches a row.
+            uint8_t* v = ring + (vi % NST) * Sh::kStage;
+            if (!warp_wait(&vfull[vr.s], vr.ph, abort_flag)) {
               ok = false;
               break;
             }
-            const volatile uint32_t* bk = bad_keys + 2 * (g & 3);
-            bad = static_cast<uint64_t>(bk[0]) | (static_cast<uint64_t>(bk[1]) << 32);
-          }
-          if (bad) {
-            for (int i = tid; i < kKeys * CH * 8; i += 128) {
-              const int key = (i >> 3) & (kKeys - 1), chunk = i >> 9;
-              if ((bad >> key) & 1)
-                *reinterpret_cast<uint4*>(v + chunk * kKvChunk + key * 128 + (i & 7) * 16) =
-                    make_uint4(0, 0, 0, 0);
+            // f(first piece of 16 bytes, key) over the V rows of keys [lo, hi).
+            auto each_piece = [&](int lo, int hi, auto f) {
+              constexpr int kPieces = CH * 8;
+              for (int i = lo * kPieces + tid; i < hi * kPieces; i += 128) {
+                const int key = i / kPieces, pc = i % kPieces;
+                f(reinterpret_cast<uint4*>(v + (pc >> 3) * kKvChunk + key * 128 + (pc & 7) * 16),
+                  key);
+              }
+            };
+            const int lo = min(max(any_lo - k0, 0), kKeys), hi = min(max(any_hi - k0, lo), kKeys);
+            // The product reads whole steps of 16 keys, at least one.
+            const int read = cap - k0 >= kKeys ? kKeys : (max(cap - k0, 1) + 15) / 16 * 16;
+            auto zero = [](uint4* p, int) { *p = make_uint4(0, 0, 0, 0); };
+            each_piece(0, lo, zero);
+            each_piece(hi, read, zero);
+            const int alo = min(max(all_lo - k0, lo), hi), ahi = min(max(all_hi - k0, alo), hi);
+            if (alo > lo || ahi < hi) {
+              auto look = [&](uint4* p, int key) {
+                const uint4 x = *p;
+                if (nonfinite2<T>(x.x) || nonfinite2<T>(x.y) || nonfinite2<T>(x.z) ||
+                    nonfinite2<T>(x.w))
+                  atomicOr(&bad_keys[2 * (g & 3) + (key >> 5)], 1u << (key & 31));
+              };
+              each_piece(lo, alo, look);
+              each_piece(ahi, hi, look);
+              if (!meet()) {
+                ok = false;
+                break;
+              }
+              const volatile uint32_t* bk = bad_keys + 2 * (g & 3);
+              bad = static_cast<uint64_t>(bk[0]) | (static_cast<uint64_t>(bk[1]) << 32);
+              if (bad) {
+                each_piece(lo, hi, [&](uint4* p, int key) {
+                  if ((bad >> key) & 1) *p = make_uint4(0, 0, 0, 0);
+                });
+                if (!meet()) {
+                  ok = false;
+                  break;
+                }
+                if (tid < 2) bad_keys[2 * (g & 3) + tid] = 0;
+              }
             }
-            if (!meet()) {
-              ok = false;
-              break;
-            }
-            if (tid < 2) bad_keys[2 * (g & 3) + tid] = 0;
           }
-        }
-        const bool active = __any_sync(0xffffffffu, vis != 0);
-        uint8_t* pj = ps + b * kPBytes;
-        if (active || (32 * q4 < r1 && 32 * q4 + 32 > r0)) {
-          tc_fence_after();
-          float s[kKeys];
-          {
-            uint32_t raw0[32], raw1[32];
-            tmem_ld32_nowait(trow + b * kKeys, raw0);
-            tmem_ld32_nowait(trow + b * kKeys + 32, raw1);
-            tmem_ld_wait();
+          uint8_t* pj = ps + b * kPBytes;
+          if (my_warp) {
+            tc_fence_after();
+            float s[kKeys];
+            {
+              uint32_t raw0[32], raw1[32];
+              tmem_ld32_nowait(trow + b * kKeys, raw0);
+              tmem_ld32_nowait(trow + b * kKeys + 32, raw1);
+              tmem_ld_wait();
 #pragma unroll
-            for (int c = 0; c < 32; ++c) {
-              s[c] = __uint_as_float(raw0[c]);
-              s[32 + c] = __uint_as_float(raw1[c]);
+              for (int c = 0; c < 32; ++c) {
+                s[c] = __uint_as_float(raw0[c]);
+                s[32 + c] = __uint_as_float(raw1[c]);
+              }
             }
-          }
-          if (__any_sync(0xffffffffu, vis != ~0ull)) {
-            const uint32_t vlo = static_cast<uint32_t>(vis), vhi = static_cast<uint32_t>(vis >> 32);
+            // Rows that are not this run's see nothing; in an own tile their
+            // lanes are off in the product, so only their (max, sum) must not
+            // move and their scores need no mask.
+            if (__any_sync(0xffffffffu, vis != ~0ull && (mine || pre))) {
+              const uint32_t vlo = static_cast<uint32_t>(vis), vhi = static_cast<uint32_t>(vis >> 32);
 #pragma unroll
-            for (int c = 0; c < kKeys; ++c) {
-              const uint32_t m = c < 32 ? vlo : vhi;
-              s[c] = ((m >> (c & 31)) & 1u) ? s[c] : -INFINITY;
+              for (int c = 0; c < kKeys; ++c) {
+                const uint32_t m = c < 32 ? vlo : vhi;
+                s[c] = ((m >> (c & 31)) & 1u) ? s[c] : -INFINITY;
+              }
             }
-          }
-          float mx[8];
+            float mx[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) mx[e] = s[e];
+            for (int e = 0; e < 8; ++e) mx[e] = s[e];
 #pragma unroll
-          for (int c = 8; c < kKeys; ++c) mx[c & 7] = fmaxf(mx[c & 7], s[c]);
-          const float mt = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])),
-                                 fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7]))) *
-                           a.scale_log2;
-          float alpha = 1.f;
-          bool rescale = false;
-          if (mt > m_ref + kTau * kLog2e) {
-            rescale = m_ref != -INFINITY;
-            alpha = rescale ? exp2_fast(m_ref - mt) : 0.f;
-            m_ref = mt;
-          }
-          float sum = 0.f;
-          if (m_ref == -INFINITY) {
-            // Nothing seen so far. A NaN score (fmaxf drops it) still counts.
-#pragma unroll
-            for (int c = 0; c < kKeys; ++c) {
-              s[c] = s[c] != s[c] ? s[c] : 0.f;
-              sum += s[c];
+            for (int c = 8; c < kKeys; ++c) mx[c & 7] = fmaxf(mx[c & 7], s[c]);
+            const float mt = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])),
+                                   fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7]))) *
+                             a.scale_log2;
+            float alpha = 1.f;
+            bool rescale = false;
+            if (mine && mt > m_ref + kTau * kLog2e) {
+              rescale = m_ref != -INFINITY;
+              alpha = rescale ? exp2_fast(m_ref - mt) : 0.f;
+              m_ref = mt;
             }
-          } else {
+            // A row that has seen nothing yet has no reference: its scores are
+            // all -infinity, or NaN, which counts (fmaxf drops it).
+            const float ref = m_ref == -INFINITY ? 0.f : m_ref;
             float psum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int c = 0; c < kKeys; ++c) {
-              s[c] = exp2_fast(fmaf(s[c], a.scale_log2, -m_ref));
+              s[c] = exp2_fast(fmaf(s[c], a.scale_log2, -ref));
               psum[c & 7] += s[c];
             }
-            sum = ((psum[0] + psum[1]) + (psum[2] + psum[3])) +
-                  ((psum[4] + psum[5]) + (psum[6] + psum[7]));
-          }
-          l = l * alpha + sum;
-          const bool any_rescale = __any_sync(0xffffffffu, rescale);
-          // Rescaling O needs the P V before this one done; slot b was read by
-          // the one before that.
-          if (j > 0 && any_rescale) {
-            if (!warp_wait(&bars[B_O0 + ((g - 1) & 1)], ((g - 1) >> 1) & 1, abort_flag, lane)) {
-              ok = false;
-              break;
+            const float sum = ((psum[0] + psum[1]) + (psum[2] + psum[3])) +
+                              ((psum[4] + psum[5]) + (psum[6] + psum[7]));
+            if (mine) l = l * alpha + sum;
+            const bool any_rescale = __any_sync(0xffffffffu, rescale);
+            // Rescaling O needs the P V before this one done; slot b was read
+            // by the one before that.
+            if (done > 0 && any_rescale) {
+              if (!warp_wait(&bars[B_O0 + ((g - 1) & 1)], ((g - 1) >> 1) & 1, abort_flag)) {
+                ok = false;
+                break;
+              }
             }
-          }
-          if (j > 1) {
-            if (!warp_wait(&bars[B_O0 + b], ((g - 2) >> 1) & 1, abort_flag, lane)) {
-              ok = false;
-              break;
+            if (done > 1) {
+              if (!warp_wait(&bars[B_O0 + b], ((g - 2) >> 1) & 1, abort_flag)) {
+                ok = false;
+                break;
+              }
             }
-          }
-          if (any_rescale) {
-            tc_fence_after();
-            const float f = rescale ? alpha : 1.0f;
-#pragma unroll 1
-            for (int c = 0; c < VD / 32; ++c) {
-              uint32_t o[32];
-              tmem_ld32_nowait(trow + Sh::kTmemO + c * 32, o);
-              tmem_ld_wait();
-#pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-              tmem_st32(trow + Sh::kTmemO + c * 32, o);
-            }
-            tmem_st_wait();
-          }
-#pragma unroll
-          for (int pw = 0; pw < kKeys / 8; ++pw) {
-            uint32_t h[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) h[e] = pack2<T>(s[pw * 8 + 2 * e], s[pw * 8 + 2 * e + 1]);
-            *reinterpret_cast<uint4*>(pj + r * 128 + ((pw ^ (r & 7)) << 4)) =
-                make_uint4(h[0], h[1], h[2], h[3]);
-          }
-        }
-        fence_proxy_async();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars[B_P0 + b]);
-        if (bad) {
-          // The taken-out keys, for the rows that see them.
-          if (!warp_wait(&bars[B_O0 + b], (g >> 1) & 1, abort_flag, lane)) {
-            ok = false;
-            break;
-          }
-          if (__any_sync(0xffffffffu, (vis & bad) != 0)) {
-            tc_fence_after();
-            for (uint64_t todo = bad; todo; todo &= todo - 1) {
-              const int key = __ffsll(static_cast<long long>(todo)) - 1;
-              const int pi = (k0 + key) >> a.c.page_log2;
-              const int page =
-                  pre ? a.b.prefix_pages[static_cast<int64_t>(wk.t.group) * a.b.max_prefix_pages + pi]
-                      : a.b.pages[static_cast<int64_t>(wk.sg.s) * a.b.max_pages + pi];
-              const int64_t row = (static_cast<int64_t>(page) << a.c.page_log2) +
-                                  ((k0 + key) & ((1 << a.c.page_log2) - 1));
-              const uint16_t* vrow = static_cast<const uint16_t*>(a.c.rows) +
-                                     (row * 2 * a.c.kv_heads + a.c.kv_heads + wk.kv) * HD +
-                                     vhalf * VD;
-              const bool add = (vis >> key) & 1;
-              const float p = to_float<T>(*reinterpret_cast<const uint16_t*>(
-                  pj + r * 128 + (((key >> 3) ^ (r & 7)) << 4) + (key & 7) * 2));
+            if (any_rescale) {
+              tc_fence_after();
+              const float f = rescale ? alpha : 1.0f;
 #pragma unroll 1
               for (int c = 0; c < VD / 32; ++c) {
                 uint32_t o[32];
                 tmem_ld32_nowait(trow + Sh::kTmemO + c * 32, o);
                 tmem_ld_wait();
 #pragma unroll
-                for (int e = 0; e < 32; ++e)
-                  if (add)
-                    o[e] = __float_as_uint(
-                        fmaf(p, to_float<T>(vrow[c * 32 + e]), __uint_as_float(o[e])));
+                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
                 tmem_st32(trow + Sh::kTmemO + c * 32, o);
               }
               tmem_st_wait();
             }
-            tc_fence_before();
+#pragma unroll
+            for (int pw = 0; pw < kKeys / 8; ++pw) {
+              uint32_t h[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) h[e] = pack2<T>(s[pw * 8 + 2 * e], s[pw * 8 + 2 * e + 1]);
+              *reinterpret_cast<uint4*>(pj + r * 128 + ((pw ^ (r & 7)) << 4)) =
+                  make_uint4(h[0], h[1], h[2], h[3]);
+            }
           }
+          if (my_warp || edge) fence_proxy_async();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars[B_P0 + b]);
+          if (bad) {
+            // The taken-out keys, for the rows that see them.
+            if (!warp_wait(&bars[B_O0 + b], (g >> 1) & 1, abort_flag)) {
+              ok = false;
+              break;
+            }
+            if (__any_sync(0xffffffffu, (vis & bad) != 0)) {
+              tc_fence_after();
+              for (uint64_t todo = bad; todo; todo &= todo - 1) {
+                const int key = __ffsll(static_cast<long long>(todo)) - 1;
+                const int pi = (k0 + key) >> a.c.page_log2;
+                const int page =
+                    pre ? a.b.prefix_pages[static_cast<int64_t>(~u.run.owner) *
+                                               a.b.max_prefix_pages + pi]
+                        : a.b.pages[static_cast<int64_t>(u.run.owner) * a.b.max_pages + pi];
+                const int64_t row = (static_cast<int64_t>(page) << a.c.page_log2) +
+                                    ((k0 + key) & ((1 << a.c.page_log2) - 1));
+                const uint16_t* vrow = static_cast<const uint16_t*>(a.c.rows) +
+                                       (row * 2 * a.c.kv_heads + a.c.kv_heads + kv) * HD +
+                                       vhalf * VD;
+                const bool add = (vis >> key) & 1;
+                const float p = to_float<T>(*reinterpret_cast<const uint16_t*>(
+                    pj + r * 128 + (((key >> 3) ^ (r & 7)) << 4) + (key & 7) * 2));
+#pragma unroll 1
+                for (int c = 0; c < VD / 32; ++c) {
+                  uint32_t o[32];
+                  tmem_ld32_nowait(trow + Sh::kTmemO + c * 32, o);
+                  tmem_ld_wait();
+#pragma unroll
+                  for (int e = 0; e < 32; ++e)
+                    if (add)
+                      o[e] = __float_as_uint(
+                          fmaf(p, to_float<T>(vrow[c * 32 + e]), __uint_as_float(o[e])));
+                  tmem_st32(trow + Sh::kTmemO + c * 32, o);
+                }
+                tmem_st_wait();
+              }
+              tc_fence_before();
+            }
+          }
+          ++g;
+          ++done;
+          vr.next();
         }
-        if (j + 1 < n) wk.next(a);
+        u.step(a, plan, n);
       }
-      it += n * (KST + 1);
-      jt += n;
+      const int count = u.w - begin;
+      const bool whole = count == tile.ntiles;
+      it += count * (KST + 1);
       // O of the row tile, or this range's share of it.
-      if (ok && !warp_wait(&bars[B_O0 + ((jt - 1) & 1)], ((jt - 1) >> 1) & 1, abort_flag, lane))
-        ok = false;
+      if (ok && !warp_wait(&bars[B_O0 + ((g - 1) & 1)], ((g - 1) >> 1) & 1, abort_flag)) ok = false;
       tc_fence_after();
-      const bool first = w == w0;
       const size_t slot = 2 * static_cast<size_t>(blockIdx.x) + (first ? 0 : 1);
       float keep = 0.f;
       if (whole) {
@@ -873,8 +1011,8 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
               const uint4 v =
                   *reinterpret_cast<const uint4*>(st + i * 128 + (((lane & 7) ^ (i & 7)) << 4));
               const int row = 32 * q4 + i, tok = row / a.hpg;
-              T* o = static_cast<T*>(a.out) + (wk.t.tok0 + tok) * a.out_stride +
-                     (wk.kv * a.hpg + row - tok * a.hpg) * HD + vhalf * VD + c * kPass;
+              T* o = static_cast<T*>(a.out) + (tile.tok0 + tok) * a.out_stride +
+                     (kv * a.hpg + row - tok * a.hpg) * HD + vhalf * VD + c * kPass;
               reinterpret_cast<uint4*>(o)[lane & 7] = v;
             }
             __syncwarp();
@@ -906,7 +1044,6 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
         }
       }
       tc_fence_before();
-      w += n;
     }
   }
   tc_fence_before();
@@ -940,8 +1077,8 @@ __global__ void __launch_bounds__(32 * kMergeWarps) paged_merge_kernel(PagedAttn
   const int w = i * per;
   if (w >= total) return;
   const int kv = w / plan.line, wl = w - kv * plan.line;
-  const int seg = warp_count_le(a.seg_cum, plan.n_segs, wl, lane) - 1;
-  const PagedTile t = a.tiles[a.segs[seg].rt];
+  const int run = warp_count_le(a.run_cum, plan.n_runs, wl, lane) - 1;
+  const PagedTile t = a.tiles[a.runs[run].rt];
   const int e0 = kv * plan.line + t.cum;
   if (e0 == w || (i - 1) * per > e0) return;
   const int c0 = i - 1, c1 = (e0 + t.ntiles - 1) / per;
@@ -1014,13 +1151,12 @@ __global__ void __launch_bounds__(32 * kMergeWarps) paged_merge_kernel(PagedAttn
 }
 
 template <int HD, class T>
-void launch(const PagedAttnArgs& a, const CUtensorMap& tq, const CUtensorMap& tkv,
-            cudaStream_t s) {
+void launch(const PagedAttnArgs& a, const PagedMaps& m, cudaStream_t s) {
   const int groups = std::max(a.b.n_groups, 1);
   launch_pdl(paged_plan_kernel, dim3(1), dim3(kPlanThreads),
              plan_smem_ints(groups, a.max_tiles, a.max_segs) * 4, s, a);
   launch_pdl(paged_attention_kernel<HD, T>, dim3(a.ctas, Shape<HD>::kHalves), dim3(192),
-             Shape<HD>::kSmem, s, tq, tkv, a);
+             Shape<HD>::kSmem, s, m, a);
   if (a.ctas > 1) {
     const int rows = std::min<int64_t>(kRows, static_cast<int64_t>(a.b.tokens) * a.hpg);
     constexpr int kRowsHere = kMergeWarps / (HD < 128 ? 1 : HD / 128);
@@ -1059,17 +1195,17 @@ size_t paged_attention_layout(PagedAttnArgs* a, int num_sms) {
   a->tpt = kRows / a->hpg;
   const int64_t tiles = (static_cast<int64_t>(a->b.tokens) + a->tpt - 1) / a->tpt +
                         std::min<int64_t>(groups, a->b.tokens);
-  const int64_t segs = tiles + a->b.n_seqs;
-  if (plan_smem_ints(groups, 0, 0) * 4 > kPlanSmemMax || (5 * tiles + segs) * 4 > kPlanSmemMax ||
-      plan_smem_ints(groups, static_cast<int>(tiles), static_cast<int>(segs)) * 4 > kPlanSmemMax)
-    return 0;
+  const int64_t segs = tiles + a->b.n_seqs, runs = segs + tiles;
+  if (plan_smem_ints(groups, tiles, segs) * 4 > kPlanSmemMax) return 0;
+  a->max_runs = static_cast<int>(runs);
   a->max_tiles = static_cast<int>(tiles);
   a->max_segs = static_cast<int>(segs);
   const int per_sm = a->c.hd == 64 ? Shape<64>::kCtasPerSm : 1;
   a->ctas = std::max(num_sms * per_sm / (a->c.hd == 512 ? 2 : 1), 1);
   a->min_tiles = 2;
   const size_t slots = 2 * static_cast<size_t>(a->ctas) * kRows;
-  return align_up(sizeof(PagedPlan)) + align_up((segs + 1) * 4) + align_up(segs * sizeof(PagedSeg)) +
+  return align_up(sizeof(PagedPlan)) + align_up((runs + 1) * 4) +
+         align_up((runs + 1) * sizeof(PagedRun)) +
          align_up(tiles * sizeof(PagedTile)) + align_up(slots * 8) + slots * a->c.hd * 4;
 }
 
@@ -1082,37 +1218,43 @@ void paged_attention_workspace(PagedAttnArgs* a, void* ws) {
   };
   const size_t slots = 2 * static_cast<size_t>(a->ctas) * kRows;
   a->plan = static_cast<PagedPlan*>(take(sizeof(PagedPlan)));
-  a->seg_cum = static_cast<int*>(take((static_cast<size_t>(a->max_segs) + 1) * 4));
-  a->segs = static_cast<PagedSeg*>(take(static_cast<size_t>(a->max_segs) * sizeof(PagedSeg)));
+  const size_t runs = static_cast<size_t>(a->max_runs) + 1;
+  a->run_cum = static_cast<int*>(take(runs * 4));
+  a->runs = static_cast<PagedRun*>(take(runs * sizeof(PagedRun)));
   a->tiles = static_cast<PagedTile*>(take(static_cast<size_t>(a->max_tiles) * sizeof(PagedTile)));
   a->part_ml = static_cast<float2*>(take(slots * 8));
   a->part_o = static_cast<float*>(take(slots * a->c.hd * 4));
 }
 
-bool paged_attention_maps(const PagedAttnArgs& a, const void* q, int64_t q_stride,
-                          CUtensorMap* tq, CUtensorMap* tkv, char* err, size_t errlen) {
+bool paged_attention_maps(const PagedAttnArgs& a, const void* q, int64_t q_stride, PagedMaps* m,
+                          char* err, size_t errlen) {
   const uint64_t hd = a.c.hd, kvh = a.c.kv_heads;
   const uint64_t qd[4] = {hd, static_cast<uint64_t>(a.hpg), kvh, static_cast<uint64_t>(a.b.tokens)};
   const uint64_t qst[3] = {hd * 2, a.hpg * hd * 2, static_cast<uint64_t>(q_stride) * 2};
   const uint32_t qb[4] = {64, static_cast<uint32_t>(a.hpg), 1, static_cast<uint32_t>(a.tpt)};
-  if (!make_tmap_f16(tq, q, 4, qd, qst, qb, err, errlen)) return false;
+  if (!make_tmap_f16(&m->q, q, 4, qd, qst, qb, err, errlen)) return false;
   const uint64_t d[2] = {2 * kvh * hd, static_cast<uint64_t>(a.c.n_pages) << a.c.page_log2};
   const uint64_t st[1] = {2 * kvh * hd * 2};
   const uint32_t b[2] = {64, static_cast<uint32_t>(std::min(1 << a.c.page_log2, kKeys))};
-  return make_tmap_f16(tkv, a.c.rows, 2, d, st, b, err, errlen);
+  const uint32_t b16[2] = {64, 16};
+  return make_tmap_f16(&m->kv, a.c.rows, 2, d, st, b, err, errlen) &&
+         make_tmap_f16(&m->kv16, a.c.rows, 2, d, st, b16, err, errlen);
 }
 
-void launch_paged_attention(const PagedAttnArgs& a, const CUtensorMap& tq, const CUtensorMap& tkv,
-                            cudaStream_t s) {
-  const bool f16 = a.c.dtype == kOpF16;
+template <int HD>
+static void launch_type(const PagedAttnArgs& a, const PagedMaps& m, cudaStream_t s) {
+  if (a.c.dtype == kOpF16)
+    launch<HD, __half>(a, m, s);
+  else
+    launch<HD, __nv_bfloat16>(a, m, s);
+}
+
+void launch_paged_attention(const PagedAttnArgs& a, const PagedMaps& m, cudaStream_t s) {
   switch (a.c.hd) {
-    case 64: return f16 ? launch<64, __half>(a, tq, tkv, s) : launch<64, __nv_bfloat16>(a, tq, tkv, s);
-    case 128:
-      return f16 ? launch<128, __half>(a, tq, tkv, s) : launch<128, __nv_bfloat16>(a, tq, tkv, s);
-    case 256:
-      return f16 ? launch<256, __half>(a, tq, tkv, s) : launch<256, __nv_bfloat16>(a, tq, tkv, s);
-    default:
-      return f16 ? launch<512, __half>(a, tq, tkv, s) : launch<512, __nv_bfloat16>(a, tq, tkv, s);
+    case 64: return launch_type<64>(a, m, s);
+    case 128: return launch_type<128>(a, m, s);
+    case 256: return launch_type<256>(a, m, s);
+    default: return launch_type<512>(a, m, s);
   }
 }
 
