@@ -74,7 +74,7 @@ constexpr int kPagedTileKeys = 64;
 
 // A run of key tiles of one row tile: its group's prefix, or one sequence's
 // own keys.
-struct PagedRun {
+struct alignas(16) PagedRun {
   int cum;         // first tile on the line (of one KV head)
   int rt;          // row tile
   int rows;        // r0 | r1 << 16: the rows that see it
@@ -84,7 +84,7 @@ struct PagedRun {
   int owner;       // the sequence; of a prefix ~group
 };
 
-struct PagedTile {
+struct alignas(16) PagedTile {
   int tok0, ntok;
   int prefix_len;
   int cum, ntiles;   // its range of the line of one KV head
@@ -106,6 +106,7 @@ struct PagedAttnArgs {
   void* out;
   int64_t out_stride;
   int heads, hpg, tpt;  // query heads, per KV head, tokens per row tile
+  int hpg_recip;        // ceil(2^16 / hpg): r / hpg = r hpg_recip >> 16 for r <= 128
   int window;           // 0: all keys
   float scale_log2;     // score scale x log2(e)
   // Workspace.

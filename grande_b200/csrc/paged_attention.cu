@@ -56,11 +56,11 @@ struct Shape {
   static constexpr int kStage = kChunks * kKvChunk; // 64 keys x kV dims
   static constexpr int kQ = HD / 64 * kQChunk;
   static constexpr int kPSlots = 2;
-  static constexpr int kCtasPerSm = HD <= 64 ? 2 : 1;
-  static constexpr int kStages = HD == 512 ? 2 : HD == 256 ? 4 : HD == 128 ? 8 : 6;
+  static constexpr int kCtasPerSm = HD <= 128 ? 2 : 1;
+  static constexpr int kStages = HD == 512 ? 2 : HD == 256 ? 4 : HD == 128 ? 3 : 6;
   static constexpr int kTmemO = 128;                // S buffers at columns 0 and 64
   static constexpr uint32_t kTmemCols = HD >= 256 ? 512 : 256;
-  static constexpr int kSmem = 1024 + kQ + kStages * kStage + kPSlots * kPBytes + 512;
+  static constexpr int kSmem = kQ + kStages * kStage + kPSlots * kPBytes + 512;
 };
 
 // ---- plan -------------------------------------------------------------------
@@ -314,6 +314,12 @@ struct Ring {
   }
 };
 
+template <int N>
+__device__ __forceinline__ int ring_add(int s, int n) {
+  s += n;
+  return s >= N ? s - N : s;
+}
+
 // The runs of a CTA's range [w, w1) of the line, in order. Each role walks
 // them by itself; the next run's record is asked for while the current one is
 // worked on (a record is an L2 latency away, a run can be one tile).
@@ -412,9 +418,7 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
     paged_attention_kernel(const __grid_constant__ PagedMaps maps, PagedAttnArgs a) {
   using Sh = Shape<HD>;
   constexpr int VD = Sh::kV, NST = Sh::kStages, CH = Sh::kChunks;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* qs = reinterpret_cast<uint8_t*>(
-      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  extern __shared__ __align__(1024) uint8_t qs[];  // (the swizzle's atoms)
   uint8_t* ring = qs + Sh::kQ;
   uint8_t* ps = ring + NST * Sh::kStage;
   uint64_t* bars = reinterpret_cast<uint64_t*>(ps + Sh::kPSlots * kPBytes);
@@ -461,7 +465,9 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
   if (w0 >= w1) {
     // Nothing of the line: on to the end.
   } else if (warp == 0) {
-    // ---- loads: Q of each row tile; per tile K and then V of the one before.
+    // ---- loads: Q of each row tile; K and V of each tile. At head_dim 512 V
+    // comes after the next tile's K: the two stages that hold a K tile are all
+    // the ring has, and S is issued a tile ahead.
     Ring<NST> slot, kr, vr;
     uint32_t qphase = 0;
     int issued_k = 0, issued_v = 0;  // for the drain
@@ -546,12 +552,16 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
 #pragma unroll
           for (int h = 0; h < KST; ++h)
             if (ok) load_stage(row, 1 << blog, lb, lc, kx + h * VD, false);
-          if (pending && ok) load_stage(prow, pbox, plb, plc, vx, true);
-          pending = true;
-          prow = row;
-          pbox = 1 << blog;
-          plb = lb;
-          plc = lc;
+          if constexpr (KST == 1) {
+            if (ok) load_stage(row, 1 << blog, lb, lc, vx, true);
+          } else {
+            if (pending && ok) load_stage(prow, pbox, plb, plc, vx, true);
+            pending = true;
+            prow = row;
+            pbox = 1 << blog;
+            plb = lb;
+            plc = lc;
+          }
           row = row1;
           blog = blog1;
           lb = lb1;
@@ -560,7 +570,7 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
         }
         u.step(a, plan, n);
       }
-      if (ok) load_stage(prow, pbox, plb, plc, vx, true);
+      if (KST == 2 && ok) load_stage(prow, pbox, plb, plc, vx, true);
     }
     if (*abort_flag && lane == 0) {
       // Gave up: wait (bounded) for the copies in flight into this CTA.
@@ -581,7 +591,11 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
     constexpr uint32_t idesc_o = f16 ? fo : idesc_bf16(fo);
     const uint64_t dq = sw128_desc(qs), dk = sw128_desc(ring), dp = sw128_desc(ps),
                    dv = sw128_mn_desc(ring, kKvChunk);
-    Ring<NST> slot, kr, vr;
+    // Ring places: at head_dim 512 in the order of use, otherwise K and V of a
+    // tile side by side.
+    Ring<NST> slot;
+    int kslot = 0, vslot = 1;
+    Ring<NST> kr, vr;
     uint32_t qphase = 0;
     int g = 0;  // tiles so far
     bool ok = true;
@@ -592,17 +606,19 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
           !warp_wait(&vfull[vr.s], vr.ph, abort_flag))
         return false;
       tc_fence_after();
+      const int vs = KST == 1 ? vslot : slot.s;
       if (lane == 0) {
-        const uint64_t pa = dp + b * (kPBytes >> 4), vb = dv + slot.s * (Sh::kStage >> 4);
+        const uint64_t pa = dp + b * (kPBytes >> 4), vb = dv + vs * (Sh::kStage >> 4);
 #pragma unroll
         for (int kk = 0; kk < kKeys / 16; ++kk)
           if (kk < steps)
             umma_f16_lanes(tmem + Sh::kTmemO, pa + 2 * kk, vb + kk * (2048 >> 4), idesc_o, 1u, off);
         umma_commit(&bars[B_O0 + b]);
-        umma_commit(&empty[slot.s]);
+        umma_commit(&empty[vs]);
       }
       __syncwarp();
       slot.next();
+      vslot = ring_add<NST>(vslot, 2);
       vr.next();
       return true;
     };
@@ -644,19 +660,21 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
               break;
             }
             tc_fence_after();
+            const int ks = KST == 1 ? kslot : slot.s;
             if (lane == 0) {
-              const uint64_t kd = dk + slot.s * (Sh::kStage >> 4);
+              const uint64_t kd = dk + ks * (Sh::kStage >> 4);
 #pragma unroll
               for (int c = 0; c < CH; ++c)
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
                   umma_f16(tmem + b * kKeys, dq + (h * CH + c) * (kQChunk >> 4) + 2 * k,
                            kd + c * (kKvChunk >> 4) + 2 * k, idesc_s, (h | c | k) ? 1u : 0u);
-              umma_commit(&empty[slot.s]);
+              umma_commit(&empty[ks]);
               if (h == KST - 1) umma_commit(&bars[B_S0 + b]);
             }
             __syncwarp();
             slot.next();
+            kslot = ring_add<NST>(kslot, 2);
             kr.next();
           }
           if (!ok) break;
@@ -691,7 +709,8 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
     const int tid = threadIdx.x - 64;
     const uint32_t trow = tmem + (static_cast<uint32_t>(32 * q4) << 16);
     uint8_t* my_stage[2] = {ps + 32 * q4 * 128, ps + kPBytes + 32 * q4 * 128};
-    int it = 0;  // ring stages before the row tile's
+    int it = 0;     // ring stages before the row tile's (head_dim 512)
+    int vslot = 1;  // ring place of the next V (otherwise)
     int g = 0;   // tiles so far
     Ring<NST> vr;
     uint32_t clean_phase = 0;
@@ -713,13 +732,25 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
       const int nrows = tile.ntok * a.hpg;
       const int begin = u.w;
       const bool valid = r < nrows;
-      // The row's own index, from its sequence's run.
+      // The row's own index, from its sequence's run: a lane per run, and a
+      // search over the lanes for the last run that starts at or before the
+      // row (own runs ascend by row; a prefix run comes first).
       int own = INT_MIN / 2;
-#pragma unroll 4
-      for (int i = tile.run0; i < tile.run0 + tile.nruns; ++i) {
-        const int rows = a.runs[i].rows, i0 = a.runs[i].i0, owner = a.runs[i].owner;
-        const int r0 = rows & 0xffff;
-        if (owner >= 0 && valid && r >= r0 && r < (rows >> 16)) own = i0 + (r - r0) / a.hpg;
+      for (int c = 0; c < tile.nruns; c += 32) {
+        int start = kRows + 1, stop = 0, i0 = 0;
+        if (c + lane < tile.nruns) {
+          const PagedRun w = a.runs[tile.run0 + c + lane];
+          start = w.owner < 0 ? -1 : w.rows & 0xffff;
+          stop = w.owner < 0 ? 0 : w.rows >> 16;
+          i0 = w.i0;
+        }
+        int at = 0;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+          if (__shfl_sync(0xffffffffu, start, at + o) <= r) at += o;
+        const int s0 = __shfl_sync(0xffffffffu, start, at), s1 = __shfl_sync(0xffffffffu, stop, at),
+                  si = __shfl_sync(0xffffffffu, i0, at);
+        if (valid && r >= s0 && r < s1) own = si + ((r - s0) * a.hpg_recip >> 16);
       }
       float m_ref = -INFINITY, l = 0.f;
       if (ok && 32 * q4 < nrows) {
@@ -746,7 +777,8 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
         // and what all of its rows see.
         const int shift = pre ? tile.prefix_len : 0, cap = u.run.kend;
         const int ifirst = shift + (pre ? tile.imin : u.run.i0);
-        const int ilast = shift + (pre ? tile.imax : u.run.i0 + (r1 - r0) / a.hpg - 1);
+        const int ilast =
+            shift + (pre ? tile.imax : u.run.i0 + ((r1 - r0) * a.hpg_recip >> 16) - 1);
         const int wlo = a.window > 0 ? a.window - 1 : INT_MAX / 2;
         const int any_lo = max(ifirst - wlo, 0), any_hi = min(ilast + 1, cap);
         const int all_lo = max(ilast - wlo, 0), all_hi = min(ifirst + 1, cap);
@@ -754,8 +786,8 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
         for (int t = 0; ok && t < n; ++t, k0 += kKeys) {
           const int b = g & 1;
           const bool last = !more && t + 1 == n;
-          // Ring place of this tile's V: the next tile's K was loaded before it.
-          const int vi = it + done * (KST + 1) + (last ? KST : 2 * KST);
+          // Ring place of this tile's V.
+          const int vs = KST == 1 ? vslot : (it + done * (KST + 1) + (last ? KST : 2 * KST)) % NST;
           if (!warp_wait(&bars[B_S0 + b], (g >> 1) & 1, abort_flag)) {
             ok = false;
             break;
@@ -773,7 +805,7 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
             // some rows see, V rows with infinities or NaN are taken out of
             // the product and added by hand to the rows that see them, so
             // that a masked key never reaches a row.
-            uint8_t* v = ring + (vi % NST) * Sh::kStage;
+            uint8_t* v = ring + vs * Sh::kStage;
             if (!warp_wait(&vfull[vr.s], vr.ph, abort_flag)) {
               ok = false;
               break;
@@ -958,6 +990,7 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
           }
           ++g;
           ++done;
+          vslot = ring_add<NST>(vslot, 2);
           vr.next();
         }
         u.step(a, plan, n);
@@ -1006,14 +1039,19 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
               }
             }
             __syncwarp();
-#pragma unroll 1
-            for (int i = lane >> 3; i < rows_here; i += 4) {
-              const uint4 v =
-                  *reinterpret_cast<const uint4*>(st + i * 128 + (((lane & 7) ^ (i & 7)) << 4));
-              const int row = 32 * q4 + i, tok = row / a.hpg;
+            uint4 v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int i = (lane >> 3) + 4 * e;
+              v[e] = *reinterpret_cast<const uint4*>(st + i * 128 + (((lane & 7) ^ (i & 7)) << 4));
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int i = (lane >> 3) + 4 * e, row = 32 * q4 + i;
+              const int tok = row * a.hpg_recip >> 16;
               T* o = static_cast<T*>(a.out) + (tile.tok0 + tok) * a.out_stride +
                      (kv * a.hpg + row - tok * a.hpg) * HD + vhalf * VD + c * kPass;
-              reinterpret_cast<uint4*>(o)[lane & 7] = v;
+              if (i < rows_here) reinterpret_cast<uint4*>(o)[lane & 7] = v[e];
             }
             __syncwarp();
           }
@@ -1031,13 +1069,18 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
                   make_uint4(__float_as_uint(o[4 * e]), __float_as_uint(o[4 * e + 1]),
                              __float_as_uint(o[4 * e + 2]), __float_as_uint(o[4 * e + 3]));
             __syncwarp();
-#pragma unroll 1
-            for (int i = lane >> 3; i < rows_here; i += 4) {
-              if (!((live >> i) & 1)) continue;
-              const uint4 v =
-                  *reinterpret_cast<const uint4*>(st + i * 128 + (((lane & 7) ^ (i & 7)) << 4));
-              reinterpret_cast<uint4*>(po + static_cast<size_t>(32 * q4 + i) * HD + c * 32)[lane & 7] =
-                  v;
+            uint4 v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int i = (lane >> 3) + 4 * e;
+              v[e] = *reinterpret_cast<const uint4*>(st + i * 128 + (((lane & 7) ^ (i & 7)) << 4));
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int i = (lane >> 3) + 4 * e;
+              if ((live >> i) & 1)
+                reinterpret_cast<uint4*>(po + static_cast<size_t>(32 * q4 + i) * HD +
+                                         c * 32)[lane & 7] = v[e];
             }
             __syncwarp();
           }
@@ -1171,7 +1214,7 @@ void set_smem() {
                        cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<HD>::kSmem);
   cudaFuncSetAttribute(paged_attention_kernel<HD, __nv_bfloat16>,
                        cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<HD>::kSmem);
-  static_assert(Shape<HD>::kSmem * Shape<HD>::kCtasPerSm <= 227 * 1024, "shared memory");
+  static_assert((Shape<HD>::kSmem + 1024) * Shape<HD>::kCtasPerSm <= 228 * 1024, "shared memory");
 }
 
 constexpr size_t kPlanSmemMax = 200 * 1024;
@@ -1193,6 +1236,7 @@ size_t paged_attention_layout(PagedAttnArgs* a, int num_sms) {
   const int groups = std::max(a->b.n_groups, 1);
   a->hpg = a->heads / a->c.kv_heads;
   a->tpt = kRows / a->hpg;
+  a->hpg_recip = (65536 + a->hpg - 1) / a->hpg;
   const int64_t tiles = (static_cast<int64_t>(a->b.tokens) + a->tpt - 1) / a->tpt +
                         std::min<int64_t>(groups, a->b.tokens);
   const int64_t segs = tiles + a->b.n_seqs, runs = segs + tiles;
@@ -1200,7 +1244,7 @@ size_t paged_attention_layout(PagedAttnArgs* a, int num_sms) {
   a->max_runs = static_cast<int>(runs);
   a->max_tiles = static_cast<int>(tiles);
   a->max_segs = static_cast<int>(segs);
-  const int per_sm = a->c.hd == 64 ? Shape<64>::kCtasPerSm : 1;
+  const int per_sm = a->c.hd <= 128 ? 2 : 1;
   a->ctas = std::max(num_sms * per_sm / (a->c.hd == 512 ? 2 : 1), 1);
   a->min_tiles = 2;
   const size_t slots = 2 * static_cast<size_t>(a->ctas) * kRows;
