@@ -55,9 +55,9 @@ struct Shape {
   static constexpr int kChunks = kV / 64;           // 64-dim chunks of a ring stage
   static constexpr int kStage = kChunks * kKvChunk; // 64 keys x kV dims
   static constexpr int kQ = HD / 64 * kQChunk;
-  static constexpr int kPSlots = 2;
+  static constexpr int kPSlots = HD == 128 ? 1 : 2;  // one: a ring of two whole tiles instead
   static constexpr int kCtasPerSm = HD <= 128 ? 2 : 1;
-  static constexpr int kStages = HD == 512 ? 2 : HD == 256 ? 4 : HD == 128 ? 3 : 6;
+  static constexpr int kStages = HD == 512 ? 2 : HD == 64 ? 6 : 4;
   static constexpr int kTmemO = 128;                // S buffers at columns 0 and 64
   static constexpr uint32_t kTmemCols = HD >= 256 ? 512 : 256;
   static constexpr int kSmem = kQ + kStages * kStage + kPSlots * kPBytes + 512;
@@ -608,7 +608,7 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
       tc_fence_after();
       const int vs = KST == 1 ? vslot : slot.s;
       if (lane == 0) {
-        const uint64_t pa = dp + b * (kPBytes >> 4), vb = dv + vs * (Sh::kStage >> 4);
+        const uint64_t pa = dp + (b & (Sh::kPSlots - 1)) * (kPBytes >> 4), vb = dv + vs * (Sh::kStage >> 4);
 #pragma unroll
         for (int kk = 0; kk < kKeys / 16; ++kk)
           if (kk < steps)
@@ -708,7 +708,8 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
     const int r = 32 * q4 + lane;
     const int tid = threadIdx.x - 64;
     const uint32_t trow = tmem + (static_cast<uint32_t>(32 * q4) << 16);
-    uint8_t* my_stage[2] = {ps + 32 * q4 * 128, ps + kPBytes + 32 * q4 * 128};
+    uint8_t* my_stage[2] = {ps + 32 * q4 * 128,
+                            ps + (Sh::kPSlots - 1) * kPBytes + 32 * q4 * 128};
     int it = 0;     // ring stages before the row tile's (head_dim 512)
     int vslot = 1;  // ring place of the next V (otherwise)
     int g = 0;   // tiles so far
@@ -853,7 +854,7 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
               }
             }
           }
-          uint8_t* pj = ps + b * kPBytes;
+          uint8_t* pj = ps + (b & (Sh::kPSlots - 1)) * kPBytes;
           if (my_warp) {
             tc_fence_after();
             float s[kKeys];
@@ -909,13 +910,13 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
             const bool any_rescale = __any_sync(0xffffffffu, rescale);
             // Rescaling O needs the P V before this one done; slot b was read
             // by the one before that.
-            if (done > 0 && any_rescale) {
+            if (done > 0 && (any_rescale || Sh::kPSlots == 1)) {
               if (!warp_wait(&bars[B_O0 + ((g - 1) & 1)], ((g - 1) >> 1) & 1, abort_flag)) {
                 ok = false;
                 break;
               }
             }
-            if (done > 1) {
+            if (Sh::kPSlots == 2 && done > 1) {
               if (!warp_wait(&bars[B_O0 + b], ((g - 2) >> 1) & 1, abort_flag)) {
                 ok = false;
                 break;
