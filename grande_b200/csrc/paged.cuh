@@ -63,34 +63,35 @@ void launch_paged_append(const PagedAppendArgs& a, int num_sms, cudaStream_t s);
 // ---- attention ---------------------------------------------------------------
 //
 // A row tile is up to 128 / (query heads per KV head) consecutive query tokens
-// of one group, all heads of one KV head: 128 query rows. It meets 64-key
-// tiles: first its group's prefix, which all of its rows see, then the own
-// keys of each of its sequences, which that sequence's rows see. The key
-// tiles of all (KV head, row tile) entries, in that order, form one line that
-// the CTAs cut into equal ranges.
+// of one group, all heads of one KV head: 128 query rows. It meets slots of 16
+// keys: first its group's prefix, which all of its rows see, then the own keys
+// of each of its sequences, which that sequence's rows see. Four slots in a
+// row make a key tile, whosever they are; the key tiles of all (KV head, row
+// tile) entries, in that order, form one line that the CTAs cut into equal
+// ranges.
 
 constexpr int kPagedTileRows = 128;
 constexpr int kPagedTileKeys = 64;
+constexpr int kPagedSlotKeys = 16;  // the K step of the P V product, the smallest page
 
-// A run of key tiles of one row tile: its group's prefix, or one sequence's
-// own keys.
+// A run of slots of one row tile: its group's prefix, or one sequence's own
+// keys.
 struct alignas(16) PagedRun {
-  int cum;         // first tile on the line (of one KV head)
   int rt;          // row tile
+  int slot0, n;    // slots [slot0, slot0 + n) of the row tile
+  int key0;        // first key (a multiple of 16) of its list of pages
+  int kend;        // keys of the list that exist (and, own: that any row sees)
   int rows;        // r0 | r1 << 16: the rows that see it
   int i0;          // own index of row r0's token
-  int tile0, n;    // key tiles [tile0, tile0 + n) of its list of pages
-  int kend;        // keys of the list that exist (and, own: that any row sees)
   int owner;       // the sequence; of a prefix ~group
 };
 
 struct alignas(16) PagedTile {
   int tok0, ntok;
   int prefix_len;
-  int cum, ntiles;   // its range of the line of one KV head
+  int ntiles;        // key tiles
   int run0, nruns;
   int imin, imax;    // own indices of its rows
-  int pad[3];
 };
 
 struct PagedPlan {
@@ -111,7 +112,7 @@ struct PagedAttnArgs {
   float scale_log2;     // score scale x log2(e)
   // Workspace.
   PagedPlan* plan;
-  int* run_cum;         // [max_runs + 1] first line tile of each run
+  int* tile_cum;        // [max_tiles + 1] first line tile of each row tile
   PagedRun* runs;       // [max_runs + 1]
   PagedTile* tiles;     // [max_tiles]
   float* part_o;        // [2 * ctas][128][hd]
@@ -126,9 +127,9 @@ struct PagedAttnArgs {
 size_t paged_attention_layout(PagedAttnArgs* a, int num_sms);
 // Point the workspace members of `a` into `ws`.
 void paged_attention_workspace(PagedAttnArgs* a, void* ws);
-// Tensor maps: q, and the cache in boxes of up to 64 rows and of 16.
+// Tensor maps: q, and the cache in boxes of a slot.
 struct PagedMaps {
-  CUtensorMap q, kv, kv16;
+  CUtensorMap q, kv;
 };
 bool paged_attention_maps(const PagedAttnArgs& a, const void* q, int64_t q_stride, PagedMaps* m,
                           char* err, size_t errlen);
@@ -137,14 +138,15 @@ void launch_paged_attention(const PagedAttnArgs& a, const PagedMaps& m, cudaStre
 void paged_attention_setup_device();
 
 #ifdef __CUDACC__
-// Entries of the ascending array a[0..n) that are <= t; a full warp calls it
-// (each round every lane probes the last entry of its share).
-__device__ __forceinline__ int warp_count_le(const int* __restrict__ a, int n, int t, int lane) {
+// Entries of the ascending array a[0], a[stride] .. (n of them) that are <= t;
+// a full warp calls it (each round every lane probes the last of its share).
+__device__ __forceinline__ int warp_count_le(const int* __restrict__ a, int n, int t, int lane,
+                                             int stride = 1) {
   int lo = 0;
   while (n > 0) {
     const int step = (n + 31) >> 5;
     const int e = (lane + 1) * step;
-    const bool le = e <= n && a[lo + e - 1] <= t;
+    const bool le = e <= n && a[static_cast<int64_t>(lo + e - 1) * stride] <= t;
     const int c = __popc(__ballot_sync(0xffffffffu, le));
     lo += c * step;
     if (step == 1) break;

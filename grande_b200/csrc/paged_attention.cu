@@ -40,6 +40,8 @@ namespace omg {
 namespace {
 
 constexpr int kKeys = kPagedTileKeys;
+constexpr int kSlot = kPagedSlotKeys;
+constexpr int kSlots = kKeys / kSlot;
 constexpr int kRows = kPagedTileRows;
 constexpr int kQChunk = kRows * 128;   // [128 rows][64 dims]
 constexpr int kKvChunk = kKeys * 128;  // [64 keys][64 dims]
@@ -68,7 +70,7 @@ struct Shape {
 struct PlanSmem {
   int *gs, *gtok, *gtile;                // [groups + 1]: first sequence, token, row tile
   int *imin, *imax, *npre, *seg0, *seg1; // [max_tiles]
-  int *seg_rt, *seg_n;                   // [max_segs]: row tile (-1: none), own key tiles
+  int *seg_rt, *seg_n;                   // [max_segs]: row tile (-1: none), own slots
 };
 
 // Arrays of 2 * max_segs first (they become 64-bit scan results).
@@ -125,7 +127,7 @@ __device__ __forceinline__ int last_le(const int* a, int n, int v) {
 struct Seg {
   int r0, r1;     // rows
   int i0, i1;     // own indices of its first and last token there
-  int tile0, n;   // own key tiles
+  int key0, n;    // own slots, from key0
   int kend;
 };
 __device__ __forceinline__ Seg segment(const PagedAttnArgs& a, int s, int q0, int q1, int t0,
@@ -138,8 +140,8 @@ __device__ __forceinline__ Seg segment(const PagedAttnArgs& a, int s, int q0, in
   g.r1 = (tb - t0) * a.hpg;
   g.kend = min(g.i1 + 1, own_cap);
   const int lo = a.window > 0 ? max(0, g.i0 - a.window + 1) : 0;
-  g.tile0 = lo / kKeys;
-  g.n = g.kend > lo ? (g.kend + kKeys - 1) / kKeys - g.tile0 : 0;
+  g.key0 = lo / kSlot * kSlot;
+  g.n = g.kend > lo ? (g.kend - g.key0 + kSlot - 1) / kSlot : 0;
   return g;
 }
 
@@ -175,7 +177,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedAttnArgs 
   for (int i = tid; i < a.max_tiles; i += kPlanThreads) {
     m.imin[i] = INT_MAX;
     m.imax[i] = INT_MIN;
-    m.npre[i] = 0;  // until the prefix's are known: the own tiles
+    m.npre[i] = 0;  // until the prefix's are known: the own slots
     m.seg0[i] = INT_MAX;
     m.seg1[i] = -1;
   }
@@ -221,27 +223,38 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedAttnArgs 
   });
   __syncthreads();
 
-  // The prefix's key tiles come before the first segment's own. Rows that see
-  // nothing at all still get their zeros: one key tile, all of it masked.
-  auto prefix_range = [&](int rt, int* tile0, int* end) -> int {
+  // The prefix's slots come before the first segment's own. Rows that see
+  // nothing at all still get their zeros: one slot, all of it masked.
+  auto prefix_slots = [&](int rt, int* key0, int* end) -> int {
     const int g = last_le(m.gtile, groups, rt);
     const int plen = a.b.n_groups > 0 ? max(a.b.prefix_lens[g], 0) : 0;
     *end = min(plen, pre_cap);
     const int lo = a.window > 0 ? max(0, plen + m.imin[rt] - a.window + 1) : 0;
-    *tile0 = lo / kKeys;
-    return lo < *end ? (*end + kKeys - 1) / kKeys - *tile0 : 0;
+    *key0 = lo / kSlot * kSlot;
+    return lo < *end ? (*end - *key0 + kSlot - 1) / kSlot : 0;
   };
-  for (int rt = tid; rt < n_tiles; rt += kPlanThreads) {
-    int tile0, end;
-    const int pre = m.seg1[rt] >= 0 ? prefix_range(rt, &tile0, &end) : 0;
-    m.npre[rt] = m.seg1[rt] < 0 ? 0 : pre + m.npre[rt] == 0 ? 1 : pre;
+  using u64 = unsigned long long;
+  int line = 0;
+  for (int rt0 = 0; rt0 < n_tiles; rt0 += kPlanThreads) {
+    const int rt = rt0 + tid;
+    int n = 0;  // key tiles
+    if (rt < n_tiles) {
+      int key0, end;
+      const int pre = m.seg1[rt] >= 0 ? prefix_slots(rt, &key0, &end) : 0, own = m.npre[rt];
+      m.npre[rt] = m.seg1[rt] < 0 ? 0 : pre + own == 0 ? 1 : pre;
+      n = (m.npre[rt] + own + kSlots - 1) / kSlots;
+    }
+    int at;
+    const int total = block_scan(n, &at);
+    if (rt < n_tiles) a.tile_cum[rt] = line + at;
+    if (rt < n_tiles) a.tiles[rt].ntiles = n;
+    line += total;
   }
   __syncthreads();
 
-  // Places of the runs, and of their tiles on the line.
-  using u64 = unsigned long long;
+  // Places of the runs, and of their slots.
   const int n_segs = S + n_tiles;
-  u64 carry = 0;  // tiles << 32 | runs
+  u64 carry = 0;  // slots << 32 | runs
   for (int i0 = 0; i0 < n_segs; i0 += kPlanThreads) {
     const int i = i0 + tid;
     u64 v = 0;
@@ -259,15 +272,15 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedAttnArgs 
     }
     carry += total;
   }
-  const int n_runs = static_cast<int>(carry & 0xffffffffu), line = static_cast<int>(carry >> 32);
+  const int n_runs = static_cast<int>(carry & 0xffffffffu);
   __syncthreads();
 
   each_segment([&](int s, int rt, const Seg& sg) {
     if (sg.n == 0) return;
-    const int pre = m.seg0[rt] == s + rt ? m.npre[rt] : 0;
-    const int at = m.seg_rt[s + rt] + (pre > 0), cum = m.seg_n[s + rt] + pre;
-    a.runs[at] = PagedRun{cum, rt, sg.r0 | (sg.r1 << 16), sg.i0, sg.tile0, sg.n, sg.kend, s};
-    a.run_cum[at] = cum;
+    const int first = m.seg0[rt], pre = first == s + rt ? m.npre[rt] : 0;
+    a.runs[m.seg_rt[s + rt] + (pre > 0)] =
+        PagedRun{rt,      m.seg_n[s + rt] + pre - m.seg_n[first], sg.n, sg.key0,
+                 sg.kend, sg.r0 | (sg.r1 << 16),                   sg.i0, s};
   });
   for (int rt = tid; rt < n_tiles; rt += kPlanThreads) {
     const int g = last_le(m.gtile, groups, rt);
@@ -275,26 +288,24 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedAttnArgs 
     t.tok0 = m.gtok[g] + (rt - m.gtile[g]) * a.tpt;
     t.ntok = min(a.tpt, m.gtok[g + 1] - t.tok0);
     t.prefix_len = a.b.n_groups > 0 ? max(a.b.prefix_lens[g], 0) : 0;
+    t.ntiles = a.tiles[rt].ntiles;
     t.imin = m.imin[rt];
     t.imax = m.imax[rt];
     if (m.seg1[rt] >= 0) {
-      const int first = m.seg0[rt], last = m.seg1[rt] + 1;
-      t.run0 = m.seg_rt[first];
-      t.cum = m.seg_n[first];
+      const int last = m.seg1[rt] + 1;
+      t.run0 = m.seg_rt[m.seg0[rt]];
       t.nruns = (last < n_segs ? m.seg_rt[last] : n_runs) - t.run0;
-      t.ntiles = (last < n_segs ? m.seg_n[last] : line) - t.cum;
       if (m.npre[rt] > 0) {
-        int tile0, end;
-        const int pre = prefix_range(rt, &tile0, &end);
-        a.runs[t.run0] = PagedRun{t.cum, rt, (t.ntok * a.hpg) << 16, 0, pre ? tile0 : 0,
-                                  m.npre[rt], pre ? end : 0, ~g};
-        a.run_cum[t.run0] = t.cum;
+        int key0, end;
+        const int pre = prefix_slots(rt, &key0, &end);
+        a.runs[t.run0] = PagedRun{rt,          0,                     m.npre[rt], pre ? key0 : 0,
+                                  pre ? end : 0, (t.ntok * a.hpg) << 16, 0,          ~g};
       }
     }
     a.tiles[rt] = t;
   }
   if (tid == 0) {
-    a.run_cum[n_runs] = line;
+    a.tile_cum[n_tiles] = line;
     *a.plan = PagedPlan{n_tiles, n_runs, line, 0};
   }
 }
@@ -320,47 +331,47 @@ __device__ __forceinline__ int ring_add(int s, int n) {
   return s >= N ? s - N : s;
 }
 
-// The runs of a CTA's range [w, w1) of the line, in order. Each role walks
-// them by itself; the next run's record is asked for while the current one is
-// worked on (a record is an L2 latency away, a run can be one tile).
-struct Runs {
-  PagedRun run, next;
-  int kv, r;
-  int off;       // first tile of the run that is this CTA's
-  int w, w1;
+// One row tile's share of a CTA's range [w, w1) of the line, walked tile by
+// tile by each role. Lane i keeps the run that slot i % 4 of the tile lies in.
+struct Share {
+  PagedTile tile;
+  PagedRun run;   // rows 0: no such slot
+  int kv, rt;
+  int pos, end;   // key tiles [pos, end) of the row tile
+  int slot, ri;   // this lane's slot of the row tile, and its run's index
 
   // A full warp calls it, with w < w1.
-  __device__ __forceinline__ void enter(const PagedAttnArgs& a, const PagedPlan& p, int w_, int w1_,
+  __device__ __forceinline__ void enter(const PagedAttnArgs& a, const PagedPlan& p, int w, int w1,
                                         int lane) {
-    w = w_;
-    w1 = w1_;
     kv = w / p.line;
     const int wl = w - kv * p.line;
-    r = warp_count_le(a.run_cum, p.n_runs, wl, lane) - 1;
-    run = a.runs[r];
-    off = wl - run.cum;
-    fetch(a, p);
+    rt = warp_count_le(a.tile_cum, p.n_tiles, wl, lane) - 1;
+    tile = a.tiles[rt];
+    pos = wl - a.tile_cum[rt];
+    end = min(tile.ntiles, pos + (w1 - w));
+    ri = warp_count_le(&a.runs[tile.run0].slot0, tile.nruns, pos * kSlots, lane,
+                       sizeof(PagedRun) / sizeof(int)) - 1;
+    run = a.runs[tile.run0 + ri];
+    slot = pos * kSlots + (lane & (kSlots - 1));
+    settle(a);
   }
-  __device__ __forceinline__ void fetch(const PagedAttnArgs& a, const PagedPlan& p) {
-    next = a.runs[r + 1 == p.n_runs ? 0 : r + 1];
-  }
-  // Tiles of the run that are this CTA's.
-  __device__ __forceinline__ int count() const { return min(run.n - off, w1 - w); }
-  // Whether more of the same row tile and KV head follows the run.
-  __device__ __forceinline__ bool more(const PagedPlan& p, int n) const {
-    return w + n < w1 && off + n == run.n && r + 1 < p.n_runs && next.rt == run.rt;
-  }
-  // Past the run's n tiles.
-  __device__ __forceinline__ void step(const PagedAttnArgs& a, const PagedPlan& p, int n) {
-    w += n;
-    off = 0;
-    run = next;
-    if (++r == p.n_runs) {
-      r = 0;
-      ++kv;
+  __device__ __forceinline__ void settle(const PagedAttnArgs& a) {
+    while (slot >= run.slot0 + run.n) {
+      if (++ri >= tile.nruns) {
+        run.rows = 0;
+        run.n = INT_MAX / 2;  // stays
+        run.slot0 = 0;
+        break;
+      }
+      run = a.runs[tile.run0 + ri];
     }
-    if (w < w1) fetch(a, p);
   }
+  __device__ __forceinline__ void next(const PagedAttnArgs& a) {
+    ++pos;
+    slot += kSlots;
+    settle(a);
+  }
+  __device__ __forceinline__ int key() const { return run.key0 + (slot - run.slot0) * kSlot; }
 };
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -445,7 +456,6 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
     fence_barrier_init();
     prefetch_tmap(&maps.q);
     prefetch_tmap(&maps.kv);
-    prefetch_tmap(&maps.kv16);
   }
   if (warp == 1) tmem_alloc(tmem_slot, Sh::kTmemCols);
   tc_fence_before();
@@ -472,10 +482,12 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
     uint32_t qphase = 0;
     int issued_k = 0, issued_v = 0;  // for the drain
     bool ok = true, first_q = true;
-    const int lg = a.c.page_log2, full_box = min(1 << lg, kKeys);
-    const int full_log2 = min(lg, 6);
-    // One ring stage: dims [x, x + kV) of `row`'s boxes.
-    auto load_stage = [&](int row, int box, int lb, int lc, int x, bool is_v) {
+    const int lg = a.c.page_log2;
+    // A lane per box: slot lane % 4, 64-dim chunk lane / 4.
+    const int lb = lane & (kSlots - 1), lc = lane / kSlots;
+    // One ring stage: dims [x, x + kV) of the slots, whose first cache rows
+    // are `row` (-1: no such keys).
+    auto load_stage = [&](int row, int x, bool is_v) {
       if (!warp_wait(&empty[slot.s], slot.ph ^ 1, abort_flag)) {
         ok = false;
         return;
@@ -483,11 +495,11 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
       uint64_t* full = is_v ? &vfull[vr.s] : &kfull[kr.s];
       const bool on = row >= 0 && lc < CH;
       const uint32_t live = __popc(__ballot_sync(0xffffffffu, on));
-      if (lane == 0) mbar_arrive_expect_tx(full, live * box * 128);
+      if (lane == 0) mbar_arrive_expect_tx(full, live * kSlot * 128);
       __syncwarp();
       if (on)
-        tma_load_2d(ring + slot.s * Sh::kStage + lc * kKvChunk + lb * box * 128,
-                    box == full_box ? &maps.kv : &maps.kv16, full, x + lc * 64, row);
+        tma_load_2d(ring + slot.s * Sh::kStage + lc * kKvChunk + lb * kSlot * 128, &maps.kv, full,
+                    x + lc * 64, row);
       slot.next();
       if (is_v) {
         vr.next();
@@ -497,80 +509,58 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
         ++issued_k;
       }
     };
-    Runs u;
-    u.enter(a, plan, w0, w1, lane);
-    while (u.w < w1 && ok) {
-      // One row tile's share.
-      const int rt = u.run.rt, kv = u.kv;
-      const int kx = kv * HD, vx = (a.c.kv_heads + kv) * HD + vhalf * VD;
+    // First cache row of this lane's slot; a page outside the pool lies past
+    // the map's end, where TMA fills zeros.
+    auto slot_row = [&](const Share& u) -> int {
+      const int key = u.key();
+      if (u.run.rows == 0 || key >= u.run.kend) return -1;
+      const int* table =
+          u.run.owner < 0
+              ? a.b.prefix_pages + static_cast<int64_t>(~u.run.owner) * a.b.max_prefix_pages
+              : a.b.pages + static_cast<int64_t>(u.run.owner) * a.b.max_pages;
+      int page = table[key >> lg];
+      if (page < 0 || page >= a.c.n_pages) page = static_cast<int>(a.c.n_pages);
+      return (page << lg) + (key & ((1 << lg) - 1));
+    };
+    for (int w = w0; w < w1 && ok;) {
+      Share u;
+      u.enter(a, plan, w, w1, lane);
+      const int n = u.end - u.pos;
+      const int kx = u.kv * HD, vx = (a.c.kv_heads + u.kv) * HD + vhalf * VD;
       if (!first_q) {
         if (!warp_wait(&bars[B_QFREE], qphase, abort_flag)) break;
         qphase ^= 1;
       }
       first_q = false;
       if (lane == 0) {
-        const int tok0 = a.tiles[rt].tok0;
         mbar_arrive_expect_tx(&bars[B_Q], HD * 2u * static_cast<uint32_t>(a.hpg * a.tpt));
 #pragma unroll 1
         for (int c = 0; c < HD / 64; ++c)
-          tma_load_4d(qs + c * kQChunk, &maps.q, &bars[B_Q], c * 64, 0, kv, tok0);
+          tma_load_4d(qs + c * kQChunk, &maps.q, &bars[B_Q], c * 64, 0, u.kv, u.tile.tok0);
       }
       __syncwarp();
-      // The tile before, whose V is still to be loaded.
-      int prow = -1, pbox = full_box, plb = 0, plc = 0;
-      bool pending = false, more = true;
-      while (more && ok) {
-        const int n = u.count();
-        more = u.more(plan, n);
-        const int* table =
-            u.run.owner < 0
-                ? a.b.prefix_pages + static_cast<int64_t>(~u.run.owner) * a.b.max_prefix_pages
-                : a.b.pages + static_cast<int64_t>(u.run.owner) * a.b.max_pages;
-        const int kend = u.run.kend;
-        // This lane's box of a tile: its cache row (-1: past the keys that
-        // exist; a page outside the pool lies past the map's end, where TMA
-        // fills zeros). A tile that is not full takes boxes of 16 rows, so
-        // that keys past the end cost at most 15 rows of traffic.
-        auto box_row = [&](int k0, int box_log2, int* lb, int* lc) -> int {
-          const int nlog = 6 - box_log2;
-          *lb = lane & ((1 << nlog) - 1);
-          *lc = lane >> nlog;
-          const int key = k0 + (*lb << box_log2);
-          if (key >= kend) return -1;
-          int page = table[key >> lg];
-          if (page < 0 || page >= a.c.n_pages) page = static_cast<int>(a.c.n_pages);
-          return (page << lg) + (key & ((1 << lg) - 1));
-        };
-        int k0 = (u.run.tile0 + u.off) * kKeys;
-        int blog = k0 + kKeys <= kend ? full_log2 : 4, lb, lc;
-        int row = box_row(k0, blog, &lb, &lc);
-        for (int t = 0; t < n && ok; ++t) {
-          // The next tile's pages are looked up before this one's waits.
-          const int k1 = k0 + kKeys, blog1 = k1 + kKeys <= kend ? full_log2 : 4;
-          int lb1 = 0, lc1 = 0;
-          const int row1 = t + 1 < n ? box_row(k1, blog1, &lb1, &lc1) : -1;
-#pragma unroll
-          for (int h = 0; h < KST; ++h)
-            if (ok) load_stage(row, 1 << blog, lb, lc, kx + h * VD, false);
-          if constexpr (KST == 1) {
-            if (ok) load_stage(row, 1 << blog, lb, lc, vx, true);
-          } else {
-            if (pending && ok) load_stage(prow, pbox, plb, plc, vx, true);
-            pending = true;
-            prow = row;
-            pbox = 1 << blog;
-            plb = lb;
-            plc = lc;
-          }
-          row = row1;
-          blog = blog1;
-          lb = lb1;
-          lc = lc1;
-          k0 = k1;
+      int row = slot_row(u), before = -1;
+      for (int t = 0; t < n && ok; ++t) {
+        // The next tile's pages are looked up before this one's waits.
+        int ahead = -1;
+        if (t + 1 < n) {
+          u.next(a);
+          ahead = slot_row(u);
         }
-        u.step(a, plan, n);
+        __syncwarp();
+#pragma unroll
+        for (int h = 0; h < KST; ++h)
+          if (ok) load_stage(row, kx + h * VD, false);
+        if constexpr (KST == 1) {
+          if (ok) load_stage(row, vx, true);
+        } else {
+          if (t > 0 && ok) load_stage(before, vx, true);
+          before = row;
+        }
+        row = ahead;
       }
-      if (KST == 2 && ok) load_stage(prow, pbox, plb, plc, vx, true);
+      if (KST == 2 && ok) load_stage(before, vx, true);
+      w += n;
     }
     if (*abort_flag && lane == 0) {
       // Gave up: wait (bounded) for the copies in flight into this CTA.
@@ -599,20 +589,38 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
     uint32_t qphase = 0;
     int g = 0;  // tiles so far
     bool ok = true;
-    // O += P V of tile `at` for the lanes not in `off`, its first `steps` x 16 keys.
-    auto issue_pv = [&](int at, const uint32_t (&off)[4], int steps) -> bool {
+    // O += P V of tile `at`: a step per slot, for the lanes of its rows (rows
+    // 0: no such slot).
+    auto issue_pv = [&](int at, const int (&rows)[kSlots]) -> bool {
       const int b = at & 1;
+      uint32_t off[kSlots][4];
+#pragma unroll
+      for (int i = 0; i < kSlots; ++i) {
+        if (i > 0 && rows[i] == rows[i - 1]) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) off[i][e] = off[i > 0 ? i - 1 : 0][e];
+        } else {
+          const int r0 = rows[i] & 0xffff, r1 = rows[i] >> 16;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            // Lanes [lo, hi) stay on.
+            const int lo = min(max(r0 - 32 * e, 0), 32), hi = min(max(r1 - 32 * e, 0), 32);
+            off[i][e] = ~((hi == 32 ? ~0u : (1u << hi) - 1) & ~(lo == 32 ? ~0u : (1u << lo) - 1));
+          }
+        }
+      }
       if (!warp_wait(&bars[B_P0 + b], (at >> 1) & 1, abort_flag) ||
           !warp_wait(&vfull[vr.s], vr.ph, abort_flag))
         return false;
       tc_fence_after();
       const int vs = KST == 1 ? vslot : slot.s;
       if (lane == 0) {
-        const uint64_t pa = dp + (b & (Sh::kPSlots - 1)) * (kPBytes >> 4), vb = dv + vs * (Sh::kStage >> 4);
+        const uint64_t pa = dp + (b & (Sh::kPSlots - 1)) * (kPBytes >> 4),
+                       vb = dv + vs * (Sh::kStage >> 4);
 #pragma unroll
-        for (int kk = 0; kk < kKeys / 16; ++kk)
-          if (kk < steps)
-            umma_f16_lanes(tmem + Sh::kTmemO, pa + 2 * kk, vb + kk * (2048 >> 4), idesc_o, 1u, off);
+        for (int i = 0; i < kSlots; ++i)
+          if (rows[i] != 0)
+            umma_f16_lanes(tmem + Sh::kTmemO, pa + 2 * i, vb + i * (2048 >> 4), idesc_o, 1u, off[i]);
         umma_commit(&bars[B_O0 + b]);
         umma_commit(&empty[vs]);
       }
@@ -622,79 +630,61 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
       vr.next();
       return true;
     };
-    Runs u;
-    u.enter(a, plan, w0, w1, lane);
-    while (u.w < w1 && ok) {
+    for (int w = w0; w < w1 && ok;) {
+      Share u;
+      u.enter(a, plan, w, w1, lane);
+      const int n = u.end - u.pos;
       if (!warp_wait(&bars[B_Q], qphase, abort_flag)) {
         ok = false;
         break;
       }
       qphase ^= 1;
-      bool pending = false, more = true;
-      uint32_t poff[4] = {0, 0, 0, 0};
-      int psteps = 4;
-      while (more && ok) {
-        const int n = u.count();
-        more = u.more(plan, n);
-        uint32_t off[4] = {0, 0, 0, 0};
-        if (u.run.owner >= 0) {
-          const int r0 = u.run.rows & 0xffff, r1 = u.run.rows >> 16;
+      int before[kSlots] = {0, 0, 0, 0};
+      for (int t = 0; t < n; ++t) {
+        int rows[kSlots];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int lo = min(max(r0 - 32 * i, 0), 32), hi = min(max(r1 - 32 * i, 0), 32);
-            // Lanes [lo, hi) stay on.
-            const uint32_t below_hi = hi == 32 ? ~0u : (1u << hi) - 1;
-            const uint32_t below_lo = lo == 32 ? ~0u : (1u << lo) - 1;
-            off[i] = ~(below_hi & ~below_lo);
-          }
-        }
-        int left = u.run.kend - (u.run.tile0 + u.off) * kKeys;
-        for (int t = 0; t < n; ++t, left -= kKeys) {
-          const int b = g & 1;
-          // The score buffer's last reader finished before the P of two tiles
-          // back, waited for with that tile's P V.
+        for (int i = 0; i < kSlots; ++i) rows[i] = __shfl_sync(0xffffffffu, u.run.rows, i);
+        if (t + 1 < n) u.next(a);
+        __syncwarp();
+        const int b = g & 1;
+        // The score buffer's last reader finished before the P of two tiles
+        // back, waited for with that tile's P V.
 #pragma unroll
-          for (int h = 0; h < KST; ++h) {
-            if (!warp_wait(&kfull[kr.s], kr.ph, abort_flag)) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
-            const int ks = KST == 1 ? kslot : slot.s;
-            if (lane == 0) {
-              const uint64_t kd = dk + ks * (Sh::kStage >> 4);
-#pragma unroll
-              for (int c = 0; c < CH; ++c)
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                  umma_f16(tmem + b * kKeys, dq + (h * CH + c) * (kQChunk >> 4) + 2 * k,
-                           kd + c * (kKvChunk >> 4) + 2 * k, idesc_s, (h | c | k) ? 1u : 0u);
-              umma_commit(&empty[ks]);
-              if (h == KST - 1) umma_commit(&bars[B_S0 + b]);
-            }
-            __syncwarp();
-            slot.next();
-            kslot = ring_add<NST>(kslot, 2);
-            kr.next();
-          }
-          if (!ok) break;
-          if (pending && !issue_pv(g - 1, poff, psteps)) {
+        for (int h = 0; h < KST; ++h) {
+          if (!warp_wait(&kfull[kr.s], kr.ph, abort_flag)) {
             ok = false;
             break;
           }
-          pending = true;
+          tc_fence_after();
+          const int ks = KST == 1 ? kslot : slot.s;
+          if (lane == 0) {
+            const uint64_t kd = dk + ks * (Sh::kStage >> 4);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) poff[i] = off[i];
-          psteps = left >= kKeys ? 4 : (max(left, 1) + 15) >> 4;
-          ++g;
+            for (int c = 0; c < CH; ++c)
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                umma_f16(tmem + b * kKeys, dq + (h * CH + c) * (kQChunk >> 4) + 2 * k,
+                         kd + c * (kKvChunk >> 4) + 2 * k, idesc_s, (h | c | k) ? 1u : 0u);
+            umma_commit(&empty[ks]);
+            if (h == KST - 1) umma_commit(&bars[B_S0 + b]);
+          }
+          __syncwarp();
+          slot.next();
+          kslot = ring_add<NST>(kslot, 2);
+          kr.next();
         }
-        u.step(a, plan, n);
+        if (ok && t + 1 == n) {
+          if (lane == 0) umma_commit(&bars[B_QFREE]);
+          __syncwarp();
+        }
+        if (ok && t > 0) ok = issue_pv(g - 1, before);
+        if (!ok) break;
+#pragma unroll
+        for (int i = 0; i < kSlots; ++i) before[i] = rows[i];
+        ++g;
       }
-      if (ok) {
-        if (lane == 0) umma_commit(&bars[B_QFREE]);
-        __syncwarp();
-        ok = issue_pv(g - 1, poff, psteps);
-      }
+      if (ok) ok = issue_pv(g - 1, before);
+      w += n;
     }
     if (!ok && lane == 0) {
       // Gave up: let the MMAs in flight finish (bounded).
@@ -724,14 +714,13 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
       clean_phase ^= 1;
       return met;
     };
-    Runs u;
-    u.enter(a, plan, w0, w1, lane);
-    while (u.w < w1) {
-      const int kv = u.kv;
-      const bool first = u.w == w0;
-      const PagedTile tile = a.tiles[u.run.rt];
+    for (int w = w0; w < w1;) {
+      Share u;
+      u.enter(a, plan, w, w1, lane);
+      const PagedTile tile = u.tile;
+      const int kv = u.kv, n = u.end - u.pos;
+      const bool first = w == w0, whole = n == tile.ntiles;
       const int nrows = tile.ntok * a.hpg;
-      const int begin = u.w;
       const bool valid = r < nrows;
       // The row's own index, from its sequence's run: a lane per run, and a
       // search over the lanes for the last run that starts at or before the
@@ -763,97 +752,114 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
         for (int c = 0; c < VD / 32; ++c) tmem_st32(trow + Sh::kTmemO + c * 32, z);
         tmem_st_wait();
       }
-      int done = 0;  // tiles of this row tile
-      bool more = true;
-      while (more) {
-        const int n = u.count();
-        more = u.more(plan, n);
-        const bool pre = u.run.owner < 0;
-        const int r0 = u.run.rows & 0xffff, r1 = u.run.rows >> 16;
+      const int wlo = a.window > 0 ? a.window - 1 : INT_MAX / 2;
+      for (int done = 0; ok && done < n; ++done) {
+        const int b = g & 1;
+        // This lane's slot: the keys that any of its run's rows sees, and
+        // those that all of them see (bounded by its first and last row).
+        const int rows = u.run.rows, key0 = u.key(), owner = u.run.owner;
+        const int r0 = rows & 0xffff, r1 = rows >> 16;
+        const int shift = owner < 0 ? tile.prefix_len : 0, cap = u.run.kend;
+        const int ifirst = shift + (owner < 0 ? tile.imin : u.run.i0);
+        const int ilast = shift + (owner < 0 ? tile.imax
+                                             : u.run.i0 + ((r1 - r0) * a.hpg_recip >> 16) - 1);
+        const int all_lo = max(ilast - wlo, 0), all_hi = min(ifirst + 1, cap);
+        const int rows0 = __shfl_sync(0xffffffffu, rows, 0);
+        // A tile of one run all of whose rows see all of its keys: no mask.
+        const bool edge = !__all_sync(0xffffffffu, rows == rows0 && rows != 0 && key0 >= all_lo &&
+                                                       key0 + kSlot <= all_hi);
+        // Ring place of this tile's V.
+        const int vs =
+            KST == 1 ? vslot : (it + done * (KST + 1) + (done + 1 == n ? KST : 2 * KST)) % NST;
+        bool mine = r >= (rows0 & 0xffff) && r < (rows0 >> 16);
+        uint64_t vis = ~0ull, any = ~0ull, all = ~0ull, exist = ~0ull;
+        if (edge) {
+          const int any_lo = max(ifirst - wlo, 0), any_hi = min(ilast + 1, cap);
+          auto piece = [&](int lo, int hi) -> uint32_t {
+            lo = min(max(lo - key0, 0), kSlot);
+            hi = min(max(hi - key0, lo), kSlot);
+            return rows ? (1u << hi) - (1u << lo) : 0u;
+          };
+          // Lanes 0 .. 3 hold the tile's four slots.
+          auto whole64 = [&](uint32_t p) -> uint64_t {
+            p <<= kSlot * (lane & 1);
+            const uint32_t lo = __reduce_or_sync(0xffffffffu, lane < 2 ? p : 0u);
+            const uint32_t hi = __reduce_or_sync(0xffffffffu, lane == 2 || lane == 3 ? p : 0u);
+            return static_cast<uint64_t>(hi) << 32 | lo;
+          };
+          any = whole64(piece(any_lo, any_hi));
+          all = whole64(piece(all_lo, all_hi));
+          exist = whole64(rows ? 0xffffu : 0u);
+          mine = false;
+          vis = 0;
+#pragma unroll
+          for (int i = 0; i < kSlots; ++i) {
+            const int ri = __shfl_sync(0xffffffffu, rows, i), ki = __shfl_sync(0xffffffffu, key0, i),
+                      ci = __shfl_sync(0xffffffffu, cap, i), si = __shfl_sync(0xffffffffu, shift, i);
+            if (r >= (ri & 0xffff) && r < (ri >> 16) && own > INT_MIN / 2) {
+              mine = true;
+              const int p = si + own;
+              const int lo = min(max(p - wlo - ki, 0), kSlot), hi = min(max(min(p + 1, ci) - ki, lo), kSlot);
+              vis |= static_cast<uint64_t>((1u << hi) - (1u << lo)) << (kSlot * i);
+            }
+          }
+        }
         // (A row without own keys, whose length is short of its query rows,
         // sees nothing.)
-        const bool mine = r >= r0 && r < r1 && own > INT_MIN / 2;
-        const bool my_warp = 32 * q4 < r1 && 32 * q4 + 32 > r0;
-        // The keys of the run that its first and last row see bound what any
-        // and what all of its rows see.
-        const int shift = pre ? tile.prefix_len : 0, cap = u.run.kend;
-        const int ifirst = shift + (pre ? tile.imin : u.run.i0);
-        const int ilast =
-            shift + (pre ? tile.imax : u.run.i0 + ((r1 - r0) * a.hpg_recip >> 16) - 1);
-        const int wlo = a.window > 0 ? a.window - 1 : INT_MAX / 2;
-        const int any_lo = max(ifirst - wlo, 0), any_hi = min(ilast + 1, cap);
-        const int all_lo = max(ilast - wlo, 0), all_hi = min(ifirst + 1, cap);
-        int k0 = (u.run.tile0 + u.off) * kKeys;
-        for (int t = 0; ok && t < n; ++t, k0 += kKeys) {
-          const int b = g & 1;
-          const bool last = !more && t + 1 == n;
-          // Ring place of this tile's V.
-          const int vs = KST == 1 ? vslot : (it + done * (KST + 1) + (last ? KST : 2 * KST)) % NST;
-          if (!warp_wait(&bars[B_S0 + b], (g >> 1) & 1, abort_flag)) {
+        mine = mine && own > INT_MIN / 2;
+        if (!warp_wait(&bars[B_S0 + b], (g >> 1) & 1, abort_flag)) {
+          ok = false;
+          break;
+        }
+        uint64_t bad = 0;
+        if (edge) {
+          // Keys that no row sees may hold anything: their V rows become
+          // zeros. Of those that only some rows see, V rows with infinities or
+          // NaN are taken out of the product and added by hand to the rows
+          // that see them, so that a masked key never reaches a row. (Other
+          // sequences' keys of the tile cannot: their steps of the product
+          // leave the row's lane alone.)
+          uint8_t* v = ring + vs * Sh::kStage;
+          if (!warp_wait(&vfull[vr.s], vr.ph, abort_flag)) {
             ok = false;
             break;
           }
-          uint64_t bad = 0;
-          uint64_t vis = mine ? ~0ull : 0;
-          const bool edge = k0 < all_lo || k0 + kKeys > all_hi;
-          if (edge) {
-            if (mine) {
-              const int p = shift + own;
-              vis = bits_between(max(p - wlo, 0) - k0, min(p + 1, cap) - k0);
+          // f(16-byte piece, key) over the V rows of `keys`, a key per warp.
+          auto each_piece = [&](uint64_t keys, auto f) {
+            for (keys &= 0x1111111111111111ull << q4; keys; keys &= keys - 1) {
+              const int key = __ffsll(static_cast<long long>(keys)) - 1;
+              if (lane < CH * 8)
+                f(reinterpret_cast<uint4*>(v + (lane >> 3) * kKvChunk + key * 128 + (lane & 7) * 16),
+                  key);
             }
-            // Keys that no row sees may hold anything: their V rows, as far
-            // as the product reads them, become zeros. Of those that only
-            // some rows see, V rows with infinities or NaN are taken out of
-            // the product and added by hand to the rows that see them, so
-            // that a masked key never reaches a row.
-            uint8_t* v = ring + vs * Sh::kStage;
-            if (!warp_wait(&vfull[vr.s], vr.ph, abort_flag)) {
+          };
+          auto zero = [](uint4* p, int) { *p = make_uint4(0, 0, 0, 0); };
+          each_piece(exist & ~any, zero);
+          const uint64_t part = any & ~all;
+          if (part) {
+            each_piece(part, [&](uint4* p, int key) {
+              const uint4 x = *p;
+              if (nonfinite2<T>(x.x) || nonfinite2<T>(x.y) || nonfinite2<T>(x.z) ||
+                  nonfinite2<T>(x.w))
+                atomicOr(&bad_keys[2 * (g & 3) + (key >> 5)], 1u << (key & 31));
+            });
+            if (!meet()) {
               ok = false;
               break;
             }
-            // f(first piece of 16 bytes, key) over the V rows of keys [lo, hi).
-            auto each_piece = [&](int lo, int hi, auto f) {
-              constexpr int kPieces = CH * 8;
-              for (int i = lo * kPieces + tid; i < hi * kPieces; i += 128) {
-                const int key = i / kPieces, pc = i % kPieces;
-                f(reinterpret_cast<uint4*>(v + (pc >> 3) * kKvChunk + key * 128 + (pc & 7) * 16),
-                  key);
-              }
-            };
-            const int lo = min(max(any_lo - k0, 0), kKeys), hi = min(max(any_hi - k0, lo), kKeys);
-            // The product reads whole steps of 16 keys, at least one.
-            const int read = cap - k0 >= kKeys ? kKeys : (max(cap - k0, 1) + 15) / 16 * 16;
-            auto zero = [](uint4* p, int) { *p = make_uint4(0, 0, 0, 0); };
-            each_piece(0, lo, zero);
-            each_piece(hi, read, zero);
-            const int alo = min(max(all_lo - k0, lo), hi), ahi = min(max(all_hi - k0, alo), hi);
-            if (alo > lo || ahi < hi) {
-              auto look = [&](uint4* p, int key) {
-                const uint4 x = *p;
-                if (nonfinite2<T>(x.x) || nonfinite2<T>(x.y) || nonfinite2<T>(x.z) ||
-                    nonfinite2<T>(x.w))
-                  atomicOr(&bad_keys[2 * (g & 3) + (key >> 5)], 1u << (key & 31));
-              };
-              each_piece(lo, alo, look);
-              each_piece(ahi, hi, look);
+            const volatile uint32_t* bk = bad_keys + 2 * (g & 3);
+            bad = static_cast<uint64_t>(bk[0]) | (static_cast<uint64_t>(bk[1]) << 32);
+            if (bad) {
+              each_piece(bad, zero);
               if (!meet()) {
                 ok = false;
                 break;
               }
-              const volatile uint32_t* bk = bad_keys + 2 * (g & 3);
-              bad = static_cast<uint64_t>(bk[0]) | (static_cast<uint64_t>(bk[1]) << 32);
-              if (bad) {
-                each_piece(lo, hi, [&](uint4* p, int key) {
-                  if ((bad >> key) & 1) *p = make_uint4(0, 0, 0, 0);
-                });
-                if (!meet()) {
-                  ok = false;
-                  break;
-                }
-                if (tid < 2) bad_keys[2 * (g & 3) + tid] = 0;
-              }
+              if (tid < 2) bad_keys[2 * (g & 3) + tid] = 0;
             }
           }
+        }
+        const bool my_warp = __any_sync(0xffffffffu, mine);
           uint8_t* pj = ps + (b & (Sh::kPSlots - 1)) * kPBytes;
           if (my_warp) {
             tc_fence_after();
@@ -869,10 +875,10 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
                 s[32 + c] = __uint_as_float(raw1[c]);
               }
             }
-            // Rows that are not this run's see nothing; in an own tile their
-            // lanes are off in the product, so only their (max, sum) must not
-            // move and their scores need no mask.
-            if (__any_sync(0xffffffffu, vis != ~0ull && (mine || pre))) {
+            // Rows without a slot here see nothing: their lanes are off in the
+            // product, so only their (max, sum) must not move and their
+            // scores need no mask.
+            if (__any_sync(0xffffffffu, vis != ~0ull && mine)) {
               const uint32_t vlo = static_cast<uint32_t>(vis), vhi = static_cast<uint32_t>(vis >> 32);
 #pragma unroll
               for (int c = 0; c < kKeys; ++c) {
@@ -959,13 +965,15 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
               tc_fence_after();
               for (uint64_t todo = bad; todo; todo &= todo - 1) {
                 const int key = __ffsll(static_cast<long long>(todo)) - 1;
-                const int pi = (k0 + key) >> a.c.page_log2;
-                const int page =
-                    pre ? a.b.prefix_pages[static_cast<int64_t>(~u.run.owner) *
-                                               a.b.max_prefix_pages + pi]
-                        : a.b.pages[static_cast<int64_t>(u.run.owner) * a.b.max_pages + pi];
+                // (All lanes take part: `todo` is the same in all of them.)
+                const int from = __shfl_sync(0xffffffffu, owner, key / kSlot);
+                const int at = __shfl_sync(0xffffffffu, key0, key / kSlot) + key % kSlot;
+                const int pi = at >> a.c.page_log2;
+                int page = from < 0 ? a.b.prefix_pages[static_cast<int64_t>(~from) *
+                                                           a.b.max_prefix_pages + pi]
+                                    : a.b.pages[static_cast<int64_t>(from) * a.b.max_pages + pi];
                 const int64_t row = (static_cast<int64_t>(page) << a.c.page_log2) +
-                                    ((k0 + key) & ((1 << a.c.page_log2) - 1));
+                                    (at & ((1 << a.c.page_log2) - 1));
                 const uint16_t* vrow = static_cast<const uint16_t*>(a.c.rows) +
                                        (row * 2 * a.c.kv_heads + a.c.kv_heads + kv) * HD +
                                        vhalf * VD;
@@ -989,16 +997,13 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
               tc_fence_before();
             }
           }
-          ++g;
-          ++done;
-          vslot = ring_add<NST>(vslot, 2);
-          vr.next();
-        }
-        u.step(a, plan, n);
+        ++g;
+        vslot = ring_add<NST>(vslot, 2);
+        vr.next();
+        if (done + 1 < n) u.next(a);
+        __syncwarp();
       }
-      const int count = u.w - begin;
-      const bool whole = count == tile.ntiles;
-      it += count * (KST + 1);
+      it += n * (KST + 1);
       // O of the row tile, or this range's share of it.
       if (ok && !warp_wait(&bars[B_O0 + ((g - 1) & 1)], ((g - 1) >> 1) & 1, abort_flag)) ok = false;
       tc_fence_after();
@@ -1088,6 +1093,7 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
         }
       }
       tc_fence_before();
+      w += n;
     }
   }
   tc_fence_before();
@@ -1121,9 +1127,9 @@ __global__ void __launch_bounds__(32 * kMergeWarps) paged_merge_kernel(PagedAttn
   const int w = i * per;
   if (w >= total) return;
   const int kv = w / plan.line, wl = w - kv * plan.line;
-  const int run = warp_count_le(a.run_cum, plan.n_runs, wl, lane) - 1;
-  const PagedTile t = a.tiles[a.runs[run].rt];
-  const int e0 = kv * plan.line + t.cum;
+  const int rt = warp_count_le(a.tile_cum, plan.n_tiles, wl, lane) - 1;
+  const PagedTile t = a.tiles[rt];
+  const int e0 = kv * plan.line + a.tile_cum[rt];
   if (e0 == w || (i - 1) * per > e0) return;
   const int c0 = i - 1, c1 = (e0 + t.ntiles - 1) / per;
   const int r = blockIdx.y * kRowsHere + warp / kRowWarps;
@@ -1249,7 +1255,7 @@ size_t paged_attention_layout(PagedAttnArgs* a, int num_sms) {
   a->ctas = std::max(num_sms * per_sm / (a->c.hd == 512 ? 2 : 1), 1);
   a->min_tiles = 2;
   const size_t slots = 2 * static_cast<size_t>(a->ctas) * kRows;
-  return align_up(sizeof(PagedPlan)) + align_up((runs + 1) * 4) +
+  return align_up(sizeof(PagedPlan)) + align_up((tiles + 1) * 4) +
          align_up((runs + 1) * sizeof(PagedRun)) +
          align_up(tiles * sizeof(PagedTile)) + align_up(slots * 8) + slots * a->c.hd * 4;
 }
@@ -1264,7 +1270,7 @@ void paged_attention_workspace(PagedAttnArgs* a, void* ws) {
   const size_t slots = 2 * static_cast<size_t>(a->ctas) * kRows;
   a->plan = static_cast<PagedPlan*>(take(sizeof(PagedPlan)));
   const size_t runs = static_cast<size_t>(a->max_runs) + 1;
-  a->run_cum = static_cast<int*>(take(runs * 4));
+  a->tile_cum = static_cast<int*>(take((static_cast<size_t>(a->max_tiles) + 1) * 4));
   a->runs = static_cast<PagedRun*>(take(runs * sizeof(PagedRun)));
   a->tiles = static_cast<PagedTile*>(take(static_cast<size_t>(a->max_tiles) * sizeof(PagedTile)));
   a->part_ml = static_cast<float2*>(take(slots * 8));
@@ -1280,10 +1286,8 @@ bool paged_attention_maps(const PagedAttnArgs& a, const void* q, int64_t q_strid
   if (!make_tmap_f16(&m->q, q, 4, qd, qst, qb, err, errlen)) return false;
   const uint64_t d[2] = {2 * kvh * hd, static_cast<uint64_t>(a.c.n_pages) << a.c.page_log2};
   const uint64_t st[1] = {2 * kvh * hd * 2};
-  const uint32_t b[2] = {64, static_cast<uint32_t>(std::min(1 << a.c.page_log2, kKeys))};
-  const uint32_t b16[2] = {64, 16};
-  return make_tmap_f16(&m->kv, a.c.rows, 2, d, st, b, err, errlen) &&
-         make_tmap_f16(&m->kv16, a.c.rows, 2, d, st, b16, err, errlen);
+  const uint32_t b[2] = {64, kSlot};
+  return make_tmap_f16(&m->kv, a.c.rows, 2, d, st, b, err, errlen);
 }
 
 template <int HD>

@@ -135,45 +135,56 @@ def rope_frequencies(theta: float, head_dim: int, rope_dims: Optional[int] = Non
     return (float(theta) ** (-2.0 * d / head_dim) / scale).to(device or "cuda")
 
 
+# The checks below run before every launch: they read each property of a tensor
+# once and build their messages only when they refuse.
+
 def _cache(op: str, cache: torch.Tensor, batch: PagedBatch) -> "_lib.PagedCacheC":
-    if cache.dim() != 5 or cache.shape[2] != 2 or not cache.is_contiguous():
-        _fail(f"{op}: the cache must be a contiguous [pages, page, 2, kv_heads, head_dim] tensor")
-    if cache.dtype not in (torch.float16, torch.bfloat16):
+    code = _TYPES.get(cache.dtype, 2)
+    if code == 2:
         _fail(f"{op}: cache dtype {cache.dtype} (float16 or bfloat16)")
-    if cache.device.type != "cuda":
+    if cache.dim() != 5 or not cache.is_contiguous() or cache.size(2) != 2:
+        _fail(f"{op}: the cache must be a contiguous [pages, page, 2, kv_heads, head_dim] tensor")
+    index = cache.get_device()
+    if index < 0:
         _fail(f"{op}: the cache must be on a GPU")
-    if batch.q_start.device != cache.device:
+    if batch.q_start.get_device() != index:
         _fail(f"{op}: the batch is on {batch.q_start.device}, the cache on {cache.device}")
-    return _lib.PagedCacheC(cache.data_ptr(), cache.shape[0], cache.shape[1], cache.shape[3],
-                            cache.shape[4], _TYPES[cache.dtype])
+    pages, page, _, kv_heads, head_dim = cache.shape
+    return _lib.PagedCacheC(cache.data_ptr(), pages, page, kv_heads, head_dim, code)
 
 
-def _vector(op: str, t, name: str, n: int, dtype, device):
+def _vector(op: str, t, name: str, n: int, dtype, index: int):
     if t is None:
         return None
-    if t.dtype != dtype or t.device != device or t.dim() != 1 or t.numel() != n or (
-            n > 1 and t.stride(0) != 1):
-        _fail(f"{op}: {name} must be {n} contiguous {dtype} values on {device}")
+    if t.dtype is not dtype or t.get_device() != index or t.numel() != n or t.dim() != 1 or (
+            not t.is_contiguous()):
+        _fail(f"{op}: {name} must be {n} contiguous {dtype} values on cuda:{index}")
     return t.data_ptr()
 
 
-def _out(op: str, out, shape, like: torch.Tensor):
+def _out(op: str, out, shape: tuple, like: torch.Tensor):
     if out is None:
-        return torch.empty(shape, dtype=like.dtype, device=like.device)
-    if tuple(out.shape) != tuple(shape) or out.dtype != like.dtype or out.device != like.device:
+        return like.new_empty(shape)
+    if out.shape != shape or out.dtype is not like.dtype or out.get_device() != like.get_device():
         _fail(f"{op}: out must be {list(shape)} {like.dtype} on {like.device}")
     return out
 
 
 def _rows(op: str, t: torch.Tensor, name: str):
     """Row stride of [tokens, heads, head_dim] rows whose heads are packed."""
-    if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
+    n, heads, dim = t.shape
+    if t.is_contiguous():
+        return heads * dim
+    row, head, one = t.stride()
+    if one != 1 or (heads > 1 and head != dim):
         _fail(f"{op}: the heads of {name} must be contiguous")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+    return row if n > 1 else heads * dim
 
 
-def _stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+# The current stream of a device as an integer, without a Stream object.
+_stream = torch._C._cuda_getCurrentRawStream if hasattr(
+    torch._C, "_cuda_getCurrentRawStream") else (
+        lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def paged_append(qkv: torch.Tensor, cache: torch.Tensor, batch: PagedBatch, *, heads: int,
@@ -193,27 +204,26 @@ def paged_append(qkv: torch.Tensor, cache: torch.Tensor, batch: PagedBatch, *, h
     [tokens, heads, head_dim]."""
     op = "paged_append"
     c = _cache(op, cache, batch)
-    kvh, hd = c.kv_heads, c.head_dim
-    dev = cache.device
-    if qkv.device != dev or qkv.dtype not in (torch.float32, cache.dtype):
-        _fail(f"{op}: qkv must be float32 or {cache.dtype} on {dev}")
+    kvh, hd, index = c.kv_heads, c.head_dim, cache.get_device()
+    if qkv.get_device() != index or (qkv.dtype is not torch.float32 and
+                                     qkv.dtype is not cache.dtype):
+        _fail(f"{op}: qkv must be float32 or {cache.dtype} on cuda:{index}")
     width = heads * hd
-    if qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.shape[1] not in (width, width + 2 * kvh * hd):
+    if qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.size(1) not in (width, width + 2 * kvh * hd):
         _fail(f"{op}: qkv is {list(qkv.shape)}, expected [tokens, {width + 2 * kvh * hd}] (q, k, v "
               f"heads) or [tokens, {width}] (q heads), rows contiguous")
-    n = qkv.shape[0]
+    n, have = qkv.shape
     out = _out(op, out, (n, heads, hd), cache)
+    n_freq = 0 if inv_freq is None else inv_freq.numel()
     args = _lib.AppendArgsC(
-        qkv.data_ptr(), qkv.stride(0) if n > 1 else qkv.shape[1], _TYPES[qkv.dtype], n, heads,
-        int(qkv.shape[1] > width), out.data_ptr(), _rows(op, out, "out"),
-        _vector(op, q_norm, "q_norm", hd, torch.float32, dev),
-        _vector(op, k_norm, "k_norm", hd, torch.float32, dev), int(v_norm), norm_offset, eps,
-        q_scale,
-        _vector(op, inv_freq, "inv_freq", 0 if inv_freq is None else inv_freq.numel(),
-                torch.float64, dev),
-        0 if inv_freq is None else inv_freq.numel())
-    check(lib().omg_paged_append(dev.index, C.byref(c), C.byref(batch._c), C.byref(args),
-                                 _stream(dev)))
+        qkv.data_ptr(), qkv.stride(0) if n > 1 else have, _TYPES[qkv.dtype], n, heads,
+        have > width, out.data_ptr(), _rows(op, out, "out"),
+        _vector(op, q_norm, "q_norm", hd, torch.float32, index),
+        _vector(op, k_norm, "k_norm", hd, torch.float32, index), v_norm, norm_offset, eps, q_scale,
+        _vector(op, inv_freq, "inv_freq", n_freq, torch.float64, index), n_freq)
+    if lib().omg_paged_append(index, C.byref(c), C.byref(batch._c), C.byref(args),
+                              _stream(index)) < 0:
+        check(-1)
     return out
 
 
@@ -228,25 +238,29 @@ def paged_attention(q: torch.Tensor, cache: torch.Tensor, batch: PagedBatch, *,
     is allocated from torch's pool when not given."""
     op = "paged_attention"
     c = _cache(op, cache, batch)
-    dev = cache.device
-    if q.device != dev or q.dtype != cache.dtype or q.dim() != 3 or q.shape[2] != c.head_dim:
+    index = cache.get_device()
+    if q.get_device() != index or q.dtype is not cache.dtype or q.dim() != 3 or (
+            q.size(2) != c.head_dim):
         _fail(f"{op}: q is {list(q.shape)} {q.dtype} on {q.device}, expected [tokens, heads, "
-              f"{c.head_dim}] {cache.dtype} on {dev}")
-    n, heads = q.shape[0], q.shape[1]
-    out = _out(op, out, (n, heads, c.head_dim), q)
+              f"{c.head_dim}] {cache.dtype} on cuda:{index}")
+    n, heads, _ = shape = q.shape
+    out = _out(op, out, shape, q)
     if workspace is None:
-        workspace = torch.empty(_workspace(dev, c, batch, n, heads), dtype=torch.uint8, device=dev)
-    elif workspace.device != dev or workspace.dtype != torch.uint8 or not workspace.is_contiguous():
-        _fail(f"{op}: the workspace must be contiguous uint8 on {dev}")
+        workspace = torch.empty(_workspace(index, c, batch, n, heads), dtype=torch.uint8,
+                                device=cache.device)
+    elif workspace.get_device() != index or workspace.dtype is not torch.uint8 or (
+            not workspace.is_contiguous()):
+        _fail(f"{op}: the workspace must be contiguous uint8 on cuda:{index}")
     args = _lib.AttentionArgsC(q.data_ptr(), _rows(op, q, "q"), out.data_ptr(),
                                _rows(op, out, "out"), n, heads, window, scale)
-    check(lib().omg_paged_attention(dev.index, C.byref(c), C.byref(batch._c), C.byref(args),
-                                    workspace.data_ptr(), workspace.numel(), _stream(dev)))
+    if lib().omg_paged_attention(index, C.byref(c), C.byref(batch._c), C.byref(args),
+                                 workspace.data_ptr(), workspace.numel(), _stream(index)) < 0:
+        check(-1)
     return out
 
 
-def _workspace(dev, c, batch, tokens, heads) -> int:
-    n = lib().omg_paged_attention_workspace(dev.index, C.byref(c), C.byref(batch._c), tokens, heads)
+def _workspace(index: int, c, batch, tokens: int, heads: int) -> int:
+    n = lib().omg_paged_attention_workspace(index, C.byref(c), C.byref(batch._c), tokens, heads)
     return n if n else check(-1)
 
 
@@ -255,16 +269,16 @@ def paged_attention_workspace(cache: torch.Tensor, batch: PagedBatch, tokens: in
     """Workspace bytes of a :func:`paged_attention` call with ``tokens`` query
     rows. Calls that may overlap (two streams, two captured graphs) need a
     workspace each."""
-    return _workspace(cache.device, _cache("paged_attention_workspace", cache, batch), batch,
+    return _workspace(cache.get_device(), _cache("paged_attention_workspace", cache, batch), batch,
                       tokens, heads)
 
 
-def _setting(op: str, v, name: str, n: int, dtype, device, off):
+def _setting(op: str, v, name: str, n: int, dtype, index: int, off):
     """(pointer, value): a tensor of one value per row, or one for all."""
     if v is None:
         return None, off
     if isinstance(v, torch.Tensor):
-        return _vector(op, v, name, n, dtype, device), off
+        return _vector(op, v, name, n, dtype, index), off
     return None, v
 
 
@@ -282,26 +296,27 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature=None, to
     the likeliest. Temperature 0 takes the largest logit. A row of nothing but
     -infinity and NaN gets token -1 and probability 0."""
     op = "sample"
-    if logits.device.type != "cuda":
+    index = logits.get_device()
+    if index < 0:
         _fail(f"{op}: logits must be on a GPU")
-    dev = logits.device
-    if logits.dim() != 2 or logits.dtype not in _TYPES or (
-            logits.shape[1] > 1 and logits.stride(1) != 1):
+    code = _TYPES.get(logits.dtype, -1)
+    if code < 0 or logits.dim() != 2 or (logits.stride(1) != 1 and logits.size(1) > 1):
         _fail(f"{op}: logits must be [rows, vocab] float32, float16 or bfloat16, rows contiguous")
     n, vocab = logits.shape
     f32, i32 = torch.float32, torch.int32
     if tokens is None:
-        tokens = torch.empty(n, dtype=i32, device=dev)
+        tokens = logits.new_empty(n, dtype=i32)
     if probs is None:
-        probs = torch.empty(n, dtype=f32, device=dev)
-    temp = _setting(op, temperature, "temperature", n, f32, dev, 1.0)
-    k = _setting(op, top_k, "top_k", n, i32, dev, 0)
-    p = _setting(op, top_p, "top_p", n, f32, dev, 1.0)
-    m = _setting(op, min_p, "min_p", n, f32, dev, 0.0)
+        probs = logits.new_empty(n, dtype=f32)
+    temp = _setting(op, temperature, "temperature", n, f32, index, 1.0)
+    k = _setting(op, top_k, "top_k", n, i32, index, 0)
+    p = _setting(op, top_p, "top_p", n, f32, index, 1.0)
+    m = _setting(op, min_p, "min_p", n, f32, index, 0.0)
     args = _lib.SampleArgsC(
-        logits.data_ptr(), logits.stride(0) if n > 1 else vocab, _TYPES[logits.dtype], n, vocab,
-        _vector(op, uniforms, "uniforms", n, f32, dev), temp[0], k[0], p[0], m[0], temp[1], k[1],
-        p[1], m[1], _vector(op, tokens, "tokens", n, i32, dev),
-        _vector(op, probs, "probs", n, f32, dev))
-    check(lib().omg_sample(dev.index, C.byref(args), _stream(dev)))
+        logits.data_ptr(), logits.stride(0) if n > 1 else vocab, code, n, vocab,
+        _vector(op, uniforms, "uniforms", n, f32, index), temp[0], k[0], p[0], m[0], temp[1], k[1],
+        p[1], m[1], _vector(op, tokens, "tokens", n, i32, index),
+        _vector(op, probs, "probs", n, f32, index))
+    if lib().omg_sample(index, C.byref(args), _stream(index)) < 0:
+        check(-1)
     return tokens, probs
