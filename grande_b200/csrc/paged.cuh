@@ -90,15 +90,20 @@ struct alignas(16) PagedTile {
   int tok0, ntok;
   int prefix_len;
   int ntiles;        // key tiles
-  int run0, nruns;
+  int nruns, pad;
   int imin, imax;    // own indices of its rows
 };
 
-struct PagedPlan {
+struct alignas(16) PagedPlan {
   int n_tiles;    // row tiles
-  int n_runs;
   int line;       // key tiles of one KV head
+  int per;        // key tiles per CTA
   int pad;
+};
+
+// Where a CTA's range of the line begins: tile `pos` of row tile `rt`.
+struct alignas(16) PagedStart {
+  int rt, pos, kv, pad;
 };
 
 struct PagedAttnArgs {
@@ -112,16 +117,17 @@ struct PagedAttnArgs {
   float scale_log2;     // score scale x log2(e)
   // Workspace.
   PagedPlan* plan;
-  int* tile_cum;        // [max_tiles + 1] first line tile of each row tile
-  PagedRun* runs;       // [max_runs + 1]
+  PagedStart* starts;   // [ctas]
+  PagedRun* runs;       // [max_tiles][tpt + 1]
   PagedTile* tiles;     // [max_tiles]
   float* part_o;        // [2 * ctas][128][hd]
   float2* part_ml;      // [2 * ctas][128]
-  int max_tiles, max_segs, max_runs;  // segments: (sequence, row tile) pairs
+  int max_tiles;
   int ctas, min_tiles;  // grid of the attention kernel; least line tiles per CTA
+  bool one_tile;        // a single row tile, which every CTA plans for itself
 };
 
-// Sizes of a call: fills max_tiles .. max_runs, ctas, min_tiles of `a` from its
+// Sizes of a call: fills max_tiles, ctas, min_tiles, one_tile of `a` from its
 // batch and shape and returns the workspace bytes (0: more sequences and row
 // tiles than the plan kernel holds).
 size_t paged_attention_layout(PagedAttnArgs* a, int num_sms);

@@ -49,6 +49,9 @@ constexpr int kPBytes = kRows * kKeys * 2;
 constexpr float kTau = 8.0f;           // slack of the reference max, in log2 units x ln 2
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kPlanThreads = 1024;
+constexpr int kThreads = 192;
+// Runs (the prefix's included) that a CTA plans for itself in shared memory.
+constexpr int one_tile_runs(int hd) { return hd == 128 ? 21 : 33; }
 
 template <int HD>
 struct Shape {
@@ -62,28 +65,18 @@ struct Shape {
   static constexpr int kStages = HD == 512 ? 2 : HD == 64 ? 6 : 4;
   static constexpr int kTmemO = 128;                // S buffers at columns 0 and 64
   static constexpr uint32_t kTmemCols = HD >= 256 ? 512 : 256;
-  static constexpr int kSmem = kQ + kStages * kStage + kPSlots * kPBytes + 512;
+  static constexpr int kSmem = kQ + kStages * kStage + kPSlots * kPBytes + 320 +
+                               (1 + one_tile_runs(HD)) * 32;
 };
 
 // ---- plan -------------------------------------------------------------------
 
-struct PlanSmem {
-  int *gs, *gtok, *gtile;                // [groups + 1]: first sequence, token, row tile
-  int *imin, *imax, *npre, *seg0, *seg1; // [max_tiles]
-  int *seg_rt, *seg_n;                   // [max_segs]: row tile (-1: none), own slots
-};
-
-// Arrays of 2 * max_segs first (they become 64-bit scan results).
-__host__ __device__ inline size_t plan_smem_ints(int64_t groups, int64_t max_tiles,
-                                                 int64_t max_segs) {
-  return 3 * (groups + 1) + 5 * max_tiles + 2 * max_segs;
-}
-
-// Exclusive scan of v over the block, plus `carry`; returns the block's total.
-template <class N>
-__device__ __forceinline__ N block_scan(N v, N* excl) {
-  __shared__ N ws[32];
-  __shared__ N total;
+// Exclusive scan of v over a block of THREADS; returns its total. (Scratch of
+// 64 ints, 8-byte aligned: static shared memory would cost the second CTA of
+// an SM.)
+template <int THREADS, class N>
+__device__ __forceinline__ N block_scan(N v, N* excl, int* scratch) {
+  N* ws = reinterpret_cast<N*>(scratch);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   N x = v;
 #pragma unroll
@@ -93,21 +86,18 @@ __device__ __forceinline__ N block_scan(N v, N* excl) {
   }
   if (lane == 31) ws[warp] = x;
   __syncthreads();
-  if (warp == 0) {
-    N w = ws[lane];
+  // Every warp scans the warps' sums for itself.
+  N w = lane < THREADS / 32 ? ws[lane] : 0;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const N y = __shfl_up_sync(0xffffffffu, w, o);
-      if (lane >= o) w += y;
-    }
-    if (lane == 31) total = w;
-    ws[lane] = w;
+  for (int o = 1; o < 32; o <<= 1) {
+    const N y = __shfl_up_sync(0xffffffffu, w, o);
+    if (lane >= o) w += y;
   }
+  const N before = __shfl_sync(0xffffffffu, w, max(warp - 1, 0));
+  *excl = x - v + (warp ? before : 0);
+  const N total = __shfl_sync(0xffffffffu, w, 31);
   __syncthreads();
-  *excl = x - v + (warp ? ws[warp - 1] : 0);
-  const N t = total;
-  __syncthreads();
-  return t;
+  return total;
 }
 
 // Largest i with a[i] <= v in the ascending a[0..n), -1: none (shared memory).
@@ -123,191 +113,164 @@ __device__ __forceinline__ int last_le(const int* a, int n, int v) {
   return lo - 1;
 }
 
-// Sequence s in row tile k of its group (token range [t0, t0 + tpt)).
-struct Seg {
-  int r0, r1;     // rows
-  int i0, i1;     // own indices of its first and last token there
-  int key0, n;    // own slots, from key0
-  int kend;
-};
-__device__ __forceinline__ Seg segment(const PagedAttnArgs& a, int s, int q0, int q1, int t0,
-                                       int own_cap) {
-  Seg g;
-  const int ta = max(q0, t0), tb = min(q1, t0 + a.tpt);
-  g.i0 = a.b.lens[s] - (a.b.q_start[s + 1] - ta);
-  g.i1 = g.i0 + (tb - ta) - 1;
-  g.r0 = (ta - t0) * a.hpg;
-  g.r1 = (tb - t0) * a.hpg;
-  g.kend = min(g.i1 + 1, own_cap);
-  const int lo = a.window > 0 ? max(0, g.i0 - a.window + 1) : 0;
-  g.key0 = lo / kSlot * kSlot;
-  g.n = g.kend > lo ? (g.kend - g.key0 + kSlot - 1) / kSlot : 0;
-  return g;
+// Row tile `rt`, tokens [t0, t1) of group g: its record and its runs. A full
+// warp calls it, a lane per sequence; `s` is the first sequence that may have
+// tokens there, `s_end` the group's end.
+__device__ void plan_tile(const PagedAttnArgs& a, const int* q, const int* lens, int rt, int g,
+                          int plen, int t0, int t1, int s, int s_end, PagedRun* runs,
+                          PagedTile* out) {
+  const int lane = threadIdx.x & 31;
+  const int own_cap = a.b.max_pages << a.c.page_log2;
+  const int pre_cap = a.b.n_groups > 0 ? a.b.max_prefix_pages << a.c.page_log2 : 0;
+  // The own runs, placed as if no prefix came before them.
+  int imin = INT_MAX, imax = INT_MIN, slots = 0, n_runs = 0;
+  for (; s < s_end; s += 32) {
+    const int me = s + lane;
+    int n = 0, ta = 0, tb = 0, key0 = 0, kend = 0, i0 = 0, q0 = t1;
+    if (me < s_end) {
+      q0 = q[me];
+      const int q1 = q[me + 1];
+      ta = max(q0, t0);
+      tb = min(q1, t1);
+      if (ta < tb) {
+        i0 = lens[me] - (q1 - ta);
+        const int i1 = i0 + (tb - ta) - 1;
+        imin = min(imin, i0);
+        imax = max(imax, i1);
+        kend = min(i1 + 1, own_cap);
+        const int lo = a.window > 0 ? max(0, i0 - a.window + 1) : 0;
+        key0 = lo / kSlot * kSlot;
+        n = kend > lo ? (kend - key0 + kSlot - 1) / kSlot : 0;
+      }
+    }
+    int upto = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += y;
+    }
+    const unsigned have = __ballot_sync(0xffffffffu, n > 0);
+    const int at = n_runs + __popc(have & ((1u << lane) - 1));
+    // (No more runs than tokens in a tile, but for tables out of order.)
+    if (n > 0 && at < a.tpt)
+      runs[1 + at] = PagedRun{rt,   slots + upto - n,
+                              n,    key0,
+                              kend, ((ta - t0) * a.hpg) | (((tb - t0) * a.hpg) << 16),
+                              i0,   me};
+    n_runs = min(n_runs + __popc(have), a.tpt);
+    slots += __shfl_sync(0xffffffffu, upto, 31);
+    if (__any_sync(0xffffffffu, me < s_end && q0 >= t1)) break;
+  }
+  imin = __reduce_min_sync(0xffffffffu, imin);
+  imax = __reduce_max_sync(0xffffffffu, imax);
+  // The prefix's slots. Rows that see nothing at all still get their zeros:
+  // one slot, all of it masked.
+  const int end = min(plen, pre_cap);
+  const int lo = a.window > 0 && imin != INT_MAX ? max(0, plen + imin - a.window + 1) : 0;
+  int key0 = lo / kSlot * kSlot, kend = end, pre = lo < end ? (end - key0 + kSlot - 1) / kSlot : 0;
+  if (pre + slots == 0) {
+    pre = 1;
+    key0 = kend = 0;
+  }
+  __syncwarp();
+  for (int i = lane; i < n_runs; i += 32) runs[1 + i].slot0 += pre;
+  if (lane == 0) {
+    runs[0] = PagedRun{rt, 0, pre, key0, kend, ((t1 - t0) * a.hpg) << 16, 0, ~g};
+    PagedTile t{};
+    t.tok0 = t0;
+    t.ntok = t1 - t0;
+    t.prefix_len = plen;
+    t.ntiles = (pre + slots + kSlots - 1) / kSlots;
+    t.nruns = 1 + n_runs;
+    t.imin = imin;
+    t.imax = imax;
+    *out = t;
+  }
+  __syncwarp();
 }
 
+__device__ __forceinline__ int tiles_per_cta(const PagedAttnArgs& a, int line) {
+  return max((line * a.c.kv_heads + a.ctas - 1) / a.ctas, a.min_tiles);
+}
+
+__host__ __device__ inline size_t plan_smem_ints(int64_t seqs, int64_t groups, int64_t max_tiles) {
+  return 64 + 2 * (seqs + 1) + 4 * (groups + 1) + max_tiles + 1;
+}
+
+// One block: groups to row tiles, a warp per row tile, and the CTAs' places on
+// the line.
 __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedAttnArgs a) {
   extern __shared__ __align__(16) int sm[];
   const int groups = max(a.b.n_groups, 1), S = a.b.n_seqs, T = a.b.tokens;
-  PlanSmem m;
-  m.seg_rt = sm;
-  m.seg_n = m.seg_rt + a.max_segs;
-  m.gs = m.seg_n + a.max_segs;
-  m.gtok = m.gs + groups + 1;
-  m.gtile = m.gtok + groups + 1;
-  m.imin = m.gtile + groups + 1;
-  m.imax = m.imin + a.max_tiles;
-  m.npre = m.imax + a.max_tiles;
-  m.seg0 = m.npre + a.max_tiles;
-  m.seg1 = m.seg0 + a.max_tiles;
-  const int tid = threadIdx.x;
+  int* q = sm + 64;            // [S + 1]
+  int* len = q + S + 1;        // [S + 1]
+  int* gs = len + S + 1;       // [groups + 1] first sequence, token, row tile; prefix length
+  int* gtok = gs + groups + 1;
+  int* gtile = gtok + groups + 1;
+  int* plen = gtile + groups + 1;
+  int* cum = plen + groups + 1;  // [max_tiles + 1] key tiles, then their running sum
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   griddep_wait();
   griddep_launch();
-
-  // Groups: first sequence and token, clipped to what exists.
+  for (int s = tid; s <= S; s += kPlanThreads) {
+    q[s] = min(max(a.b.q_start[s], 0), T);
+    len[s] = s < S ? a.b.lens[s] : 0;
+  }
   for (int g = tid; g <= groups; g += kPlanThreads) {
-    int s = a.b.n_groups > 0 ? a.b.group_start[g] : g * S;
-    s = min(max(s, 0), S);
-    m.gs[g] = s;
-    m.gtok[g] = min(max(a.b.q_start[s], 0), T);
-  }
-  for (int i = tid; i < a.max_segs; i += kPlanThreads) {
-    m.seg_rt[i] = -1;
-    m.seg_n[i] = 0;
-  }
-  for (int i = tid; i < a.max_tiles; i += kPlanThreads) {
-    m.imin[i] = INT_MAX;
-    m.imax[i] = INT_MIN;
-    m.npre[i] = 0;  // until the prefix's are known: the own slots
-    m.seg0[i] = INT_MAX;
-    m.seg1[i] = -1;
+    const int s = a.b.n_groups > 0 ? a.b.group_start[g] : g * S;
+    gs[g] = min(max(s, 0), S);
+    plen[g] = a.b.n_groups > 0 && g < groups ? max(a.b.prefix_lens[g], 0) : 0;
   }
   __syncthreads();
   int n_tiles = 0;
   for (int g0 = 0; g0 < groups; g0 += kPlanThreads) {
     const int g = g0 + tid;
-    const int n = g < groups ? (max(m.gtok[g + 1] - m.gtok[g], 0) + a.tpt - 1) / a.tpt : 0;
+    int n = 0;
+    if (g < groups) {
+      const int t0 = q[gs[g]], t1 = q[gs[g + 1]];
+      gtok[g] = t0;
+      n = (max(t1 - t0, 0) + a.tpt - 1) / a.tpt;
+    }
     int at;
-    const int total = block_scan(n, &at);
-    if (g < groups) m.gtile[g] = n_tiles + at;
+    const int total = block_scan<kPlanThreads>(n, &at, sm);
+    if (g < groups) gtile[g] = n_tiles + at;
     n_tiles += total;
   }
   n_tiles = min(n_tiles, a.max_tiles);  // only tables out of order make more
-  if (tid == 0) m.gtile[groups] = n_tiles;
   __syncthreads();
-
-  const int own_cap = a.b.max_pages << a.c.page_log2;
-  const int pre_cap = a.b.n_groups > 0 ? a.b.max_prefix_pages << a.c.page_log2 : 0;
-  // f(sequence, row tile, segment) for every pair that shares tokens.
-  auto each_segment = [&](auto f) {
-    for (int s = tid; s < S; s += kPlanThreads) {
-      const int g = last_le(m.gs, groups + 1, s);
-      if (g < 0 || g >= groups) continue;
-      const int q0 = max(a.b.q_start[s], m.gtok[g]);
-      const int q1 = min(a.b.q_start[s + 1], m.gtok[g + 1]);
-      if (q0 >= q1) continue;
-      for (int k = (q0 - m.gtok[g]) / a.tpt; k <= (q1 - 1 - m.gtok[g]) / a.tpt; ++k) {
-        const int rt = m.gtile[g] + k;
-        if (rt >= n_tiles) break;
-        f(s, rt, segment(a, s, q0, q1, m.gtok[g] + k * a.tpt, own_cap));
-      }
-    }
-  };
-  each_segment([&](int s, int rt, const Seg& sg) {
-    m.seg_rt[s + rt] = rt;
-    m.seg_n[s + rt] = sg.n;
-    atomicMin(&m.imin[rt], sg.i0);
-    atomicMax(&m.imax[rt], sg.i1);
-    atomicAdd(&m.npre[rt], sg.n);
-    atomicMin(&m.seg0[rt], s + rt);
-    atomicMax(&m.seg1[rt], s + rt);
-  });
+  for (int rt = warp; rt < n_tiles; rt += kPlanThreads / 32) {
+    const int g = last_le(gtile, groups, rt);
+    const int t0 = gtok[g] + (rt - gtile[g]) * a.tpt;
+    const int t1 = min(t0 + a.tpt, q[gs[g + 1]]);
+    // The last sequence that starts at or before the first token.
+    const int s = max(gs[g], warp_count_le(q + gs[g], gs[g + 1] - gs[g], t0, lane) - 1 + gs[g]);
+    plan_tile(a, q, len, rt, g, plen[g], t0, t1, s, gs[g + 1],
+              a.runs + static_cast<int64_t>(rt) * (a.tpt + 1), a.tiles + rt);
+    if (lane == 0) cum[rt] = a.tiles[rt].ntiles;
+  }
   __syncthreads();
-
-  // The prefix's slots come before the first segment's own. Rows that see
-  // nothing at all still get their zeros: one slot, all of it masked.
-  auto prefix_slots = [&](int rt, int* key0, int* end) -> int {
-    const int g = last_le(m.gtile, groups, rt);
-    const int plen = a.b.n_groups > 0 ? max(a.b.prefix_lens[g], 0) : 0;
-    *end = min(plen, pre_cap);
-    const int lo = a.window > 0 ? max(0, plen + m.imin[rt] - a.window + 1) : 0;
-    *key0 = lo / kSlot * kSlot;
-    return lo < *end ? (*end - *key0 + kSlot - 1) / kSlot : 0;
-  };
-  using u64 = unsigned long long;
   int line = 0;
   for (int rt0 = 0; rt0 < n_tiles; rt0 += kPlanThreads) {
     const int rt = rt0 + tid;
-    int n = 0;  // key tiles
-    if (rt < n_tiles) {
-      int key0, end;
-      const int pre = m.seg1[rt] >= 0 ? prefix_slots(rt, &key0, &end) : 0, own = m.npre[rt];
-      m.npre[rt] = m.seg1[rt] < 0 ? 0 : pre + own == 0 ? 1 : pre;
-      n = (m.npre[rt] + own + kSlots - 1) / kSlots;
-    }
     int at;
-    const int total = block_scan(n, &at);
-    if (rt < n_tiles) a.tile_cum[rt] = line + at;
-    if (rt < n_tiles) a.tiles[rt].ntiles = n;
+    const int total = block_scan<kPlanThreads>(rt < n_tiles ? cum[rt] : 0, &at, sm);
+    if (rt < n_tiles) cum[rt] = line + at;
     line += total;
   }
   __syncthreads();
-
-  // Places of the runs, and of their slots.
-  const int n_segs = S + n_tiles;
-  u64 carry = 0;  // slots << 32 | runs
-  for (int i0 = 0; i0 < n_segs; i0 += kPlanThreads) {
-    const int i = i0 + tid;
-    u64 v = 0;
-    if (i < n_segs && m.seg_rt[i] >= 0) {
-      const int rt = m.seg_rt[i], own = m.seg_n[i], pre = m.seg0[rt] == i ? m.npre[rt] : 0;
-      v = (static_cast<u64>(own + pre) << 32) | ((own > 0) + (pre > 0));
+  const int per = tiles_per_cta(a, line);
+  for (int i = tid; i < a.ctas; i += kPlanThreads) {
+    const int w = i * per;
+    PagedStart st{0, 0, 0, 0};
+    if (w < line * a.c.kv_heads) {
+      st.kv = w / line;
+      const int wl = w - st.kv * line;
+      st.rt = last_le(cum, n_tiles, wl);
+      st.pos = wl - cum[st.rt];
     }
-    u64 at;
-    const u64 total = block_scan(v, &at);
-    at += carry;
-    if (i < n_segs) {
-      // (In place: nothing else reads entry i any more.)
-      m.seg_rt[i] = static_cast<int>(at);
-      m.seg_n[i] = static_cast<int>(at >> 32);
-    }
-    carry += total;
+    a.starts[i] = st;
   }
-  const int n_runs = static_cast<int>(carry & 0xffffffffu);
-  __syncthreads();
-
-  each_segment([&](int s, int rt, const Seg& sg) {
-    if (sg.n == 0) return;
-    const int first = m.seg0[rt], pre = first == s + rt ? m.npre[rt] : 0;
-    a.runs[m.seg_rt[s + rt] + (pre > 0)] =
-        PagedRun{rt,      m.seg_n[s + rt] + pre - m.seg_n[first], sg.n, sg.key0,
-                 sg.kend, sg.r0 | (sg.r1 << 16),                   sg.i0, s};
-  });
-  for (int rt = tid; rt < n_tiles; rt += kPlanThreads) {
-    const int g = last_le(m.gtile, groups, rt);
-    PagedTile t{};
-    t.tok0 = m.gtok[g] + (rt - m.gtile[g]) * a.tpt;
-    t.ntok = min(a.tpt, m.gtok[g + 1] - t.tok0);
-    t.prefix_len = a.b.n_groups > 0 ? max(a.b.prefix_lens[g], 0) : 0;
-    t.ntiles = a.tiles[rt].ntiles;
-    t.imin = m.imin[rt];
-    t.imax = m.imax[rt];
-    if (m.seg1[rt] >= 0) {
-      const int last = m.seg1[rt] + 1;
-      t.run0 = m.seg_rt[m.seg0[rt]];
-      t.nruns = (last < n_segs ? m.seg_rt[last] : n_runs) - t.run0;
-      if (m.npre[rt] > 0) {
-        int key0, end;
-        const int pre = prefix_slots(rt, &key0, &end);
-        a.runs[t.run0] = PagedRun{rt,          0,                     m.npre[rt], pre ? key0 : 0,
-                                  pre ? end : 0, (t.ntok * a.hpg) << 16, 0,          ~g};
-      }
-    }
-    a.tiles[rt] = t;
-  }
-  if (tid == 0) {
-    a.tile_cum[n_tiles] = line;
-    *a.plan = PagedPlan{n_tiles, n_runs, line, 0};
-  }
+  if (tid == 0) *a.plan = PagedPlan{n_tiles, line, per, 0};
 }
 
 // ---- attention ----------------------------------------------------------------
@@ -331,31 +294,51 @@ __device__ __forceinline__ int ring_add(int s, int n) {
   return s >= N ? s - N : s;
 }
 
-// One row tile's share of a CTA's range [w, w1) of the line, walked tile by
-// tile by each role. Lane i keeps the run that slot i % 4 of the tile lies in.
+// One row tile's share of a CTA's range of the line, walked tile by tile by
+// each role. Lane i keeps the run that slot i % 4 of the tile lies in.
 struct Share {
+  const PagedRun* runs;
   PagedTile tile;
   PagedRun run;   // rows 0: no such slot
   int kv, rt;
   int pos, end;   // key tiles [pos, end) of the row tile
   int slot, ri;   // this lane's slot of the row tile, and its run's index
 
-  // A full warp calls it, with w < w1.
-  __device__ __forceinline__ void enter(const PagedAttnArgs& a, const PagedPlan& p, int w, int w1,
-                                        int lane) {
-    kv = w / p.line;
-    const int wl = w - kv * p.line;
-    rt = warp_count_le(a.tile_cum, p.n_tiles, wl, lane) - 1;
-    tile = a.tiles[rt];
-    pos = wl - a.tile_cum[rt];
-    end = min(tile.ntiles, pos + (w1 - w));
-    ri = warp_count_le(&a.runs[tile.run0].slot0, tile.nruns, pos * kSlots, lane,
-                       sizeof(PagedRun) / sizeof(int)) - 1;
-    run = a.runs[tile.run0 + ri];
+  // Up to `left` tiles from tile `pos` of row tile `rt` on; a full warp calls
+  // it. The row tile and its first runs, a lane each, come in one round trip.
+  // `cap` runs are held for each row tile.
+  __device__ __forceinline__ void load(const PagedTile* tiles, const PagedRun* all_runs, int cap,
+                                       int left, int lane) {
+    runs = all_runs + static_cast<int64_t>(rt) * cap;
+    run = runs[min(lane, cap - 1)];
+    tile = tiles[rt];
+    end = min(tile.ntiles, pos + left);
+    if (tile.nruns <= 32) {
+      ri = __popc(__ballot_sync(0xffffffffu, lane < tile.nruns && run.slot0 <= pos * kSlots)) - 1;
+      run.slot0 = __shfl_sync(0xffffffffu, run.slot0, ri);
+      run.n = __shfl_sync(0xffffffffu, run.n, ri);
+      run.key0 = __shfl_sync(0xffffffffu, run.key0, ri);
+      run.kend = __shfl_sync(0xffffffffu, run.kend, ri);
+      run.rows = __shfl_sync(0xffffffffu, run.rows, ri);
+      run.i0 = __shfl_sync(0xffffffffu, run.i0, ri);
+      run.owner = __shfl_sync(0xffffffffu, run.owner, ri);
+    } else {
+      ri = warp_count_le(&runs[0].slot0, tile.nruns, pos * kSlots, lane,
+                         sizeof(PagedRun) / sizeof(int)) - 1;
+      run = runs[ri];
+    }
     slot = pos * kSlots + (lane & (kSlots - 1));
-    settle(a);
+    settle();
   }
-  __device__ __forceinline__ void settle(const PagedAttnArgs& a) {
+  // On to the next row tile, or the first of the next KV head.
+  __device__ __forceinline__ void leave(int n_tiles) {
+    pos = 0;
+    if (++rt == n_tiles) {
+      rt = 0;
+      ++kv;
+    }
+  }
+  __device__ __forceinline__ void settle() {
     while (slot >= run.slot0 + run.n) {
       if (++ri >= tile.nruns) {
         run.rows = 0;
@@ -363,13 +346,13 @@ struct Share {
         run.slot0 = 0;
         break;
       }
-      run = a.runs[tile.run0 + ri];
+      run = runs[ri];
     }
   }
-  __device__ __forceinline__ void next(const PagedAttnArgs& a) {
+  __device__ __forceinline__ void next() {
     ++pos;
     slot += kSlots;
-    settle(a);
+    settle();
   }
   __device__ __forceinline__ int key() const { return run.key0 + (slot - run.slot0) * kSlot; }
 };
@@ -378,15 +361,6 @@ __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
-}
-
-// Bits [a, b) of a 64-bit set, clipped to it.
-__device__ __forceinline__ uint64_t bits_between(int a, int b) {
-  a = min(max(a, 0), 64);
-  b = min(max(b, 0), 64);
-  if (a >= b) return 0;
-  const uint64_t hi = b >= 64 ? ~0ull : (1ull << b) - 1;
-  return hi & ~((1ull << a) - 1);
 }
 
 // Every lane waits: a warp that is not split needs no broadcast.
@@ -425,7 +399,7 @@ enum { B_Q = 0, B_QFREE, B_S0, B_S1, B_P0, B_P1, B_O0, B_O1, B_CLEAN, B_DRAIN, B
 constexpr long long kDrainClocks = 1ll << 28;
 
 template <int HD, class T>
-__global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
+__global__ void __launch_bounds__(kThreads, Shape<HD>::kCtasPerSm)
     paged_attention_kernel(const __grid_constant__ PagedMaps maps, PagedAttnArgs a) {
   using Sh = Shape<HD>;
   constexpr int VD = Sh::kV, NST = Sh::kStages, CH = Sh::kChunks;
@@ -444,6 +418,10 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
   // [tile & 3][2]: a tile's keys with infinities or NaN in V. Four sets: a
   // warp can be two tiles ahead of the one that clears a set.
   uint32_t* bad_keys = tmem_slot + 2;
+  // one_tile: the plan.
+  PagedTile* my_tile = reinterpret_cast<PagedTile*>(reinterpret_cast<uint8_t*>(bars) + 320);
+  PagedRun* my_runs = reinterpret_cast<PagedRun*>(my_tile + 1);
+  static_assert((B_RING + 3 * NST) * 8 + 4 * (2 + 8) <= 320, "barriers");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int vhalf = blockIdx.y;  // this CTA's dims of V (head_dim 512)
@@ -464,12 +442,43 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
   const uint32_t tmem = *tmem_slot;
   griddep_wait();
   griddep_launch();
-
-  const PagedPlan plan = *a.plan;
+  PagedPlan plan;
+  PagedStart start;
+  const PagedRun* runs = a.runs;
+  const PagedTile* tiles = a.tiles;
+  const int run_cap = a.one_tile ? one_tile_runs(HD) : a.tpt + 1;
+  if (a.one_tile) {
+    // A single row tile: warp 2 of every CTA plans it here, in about the time
+    // of three loads; the first CTA leaves it to the merge.
+    if (warp == 2) {
+      const int s0 = a.b.n_groups > 0 ? min(max(a.b.group_start[0], 0), a.b.n_seqs) : 0;
+      const int s1 = a.b.n_groups > 0 ? min(max(a.b.group_start[1], s0), a.b.n_seqs) : a.b.n_seqs;
+      const int plen = a.b.n_groups > 0 ? max(a.b.prefix_lens[0], 0) : 0;
+      const int t0 = min(max(a.b.q_start[s0], 0), a.b.tokens);
+      const int t1 = min(max(a.b.q_start[s1], t0), a.b.tokens);
+      if (t1 > t0) plan_tile(a, a.b.q_start, a.b.lens, 0, 0, plen, t0, t1, s0, s1, my_runs, my_tile);
+      if (t1 == t0 && lane == 0) my_tile->ntiles = 0;
+      if (blockIdx.x == 0 && blockIdx.y == 0 && lane == 0) {
+        *a.plan = PagedPlan{1, my_tile->ntiles, tiles_per_cta(a, my_tile->ntiles), 0};
+        *a.tiles = *my_tile;
+      }
+    }
+    __syncthreads();
+    runs = my_runs;
+    tiles = my_tile;
+    const int line = my_tile->ntiles;
+    plan = PagedPlan{1, line, tiles_per_cta(a, line), 0};
+    const int w = blockIdx.x * plan.per;
+    start.kv = line ? w / line : 0;
+    start.rt = 0;
+    start.pos = line ? w - start.kv * line : 0;
+  } else {
+    plan = *a.plan;
+    start = a.starts[blockIdx.x];
+  }
   const int total = plan.line * a.c.kv_heads;
-  const int per = max((total + a.ctas - 1) / a.ctas, a.min_tiles);
-  const int w0 = min(static_cast<int>(blockIdx.x) * per, total);
-  const int w1 = min(w0 + per, total);
+  const int w0 = min(static_cast<int>(blockIdx.x) * plan.per, total);
+  const int w1 = min(w0 + plan.per, total);
   constexpr int KST = Sh::kHalves;  // ring stages of a K tile (V: one)
 
   if (w0 >= w1) {
@@ -509,22 +518,32 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
         ++issued_k;
       }
     };
-    // First cache row of this lane's slot; a page outside the pool lies past
-    // the map's end, where TMA fills zeros.
-    auto slot_row = [&](const Share& u) -> int {
-      const int key = u.key();
-      if (u.run.rows == 0 || key >= u.run.kend) return -1;
+    // The page of this lane's slot and the slot's first key (-1: no such
+    // keys), asked for a tile ahead; and the cache row they make. A page
+    // outside the pool lies past the map's end, where TMA fills zeros.
+    auto slot_page = [&](const Share& u, int* key) -> int {
+      *key = u.key();
+      if (u.run.rows == 0 || *key >= u.run.kend) {
+        *key = -1;
+        return 0;
+      }
       const int* table =
           u.run.owner < 0
               ? a.b.prefix_pages + static_cast<int64_t>(~u.run.owner) * a.b.max_prefix_pages
               : a.b.pages + static_cast<int64_t>(u.run.owner) * a.b.max_pages;
-      int page = table[key >> lg];
+      return table[*key >> lg];
+    };
+    auto row_of = [&](int page, int key) -> int {
+      if (key < 0) return -1;
       if (page < 0 || page >= a.c.n_pages) page = static_cast<int>(a.c.n_pages);
       return (page << lg) + (key & ((1 << lg) - 1));
     };
-    for (int w = w0; w < w1 && ok;) {
-      Share u;
-      u.enter(a, plan, w, w1, lane);
+    Share u;
+    u.rt = start.rt;
+    u.pos = start.pos;
+    u.kv = start.kv;
+    for (int w = w0; w < w1 && ok; u.leave(plan.n_tiles)) {
+      u.load(tiles, runs, run_cap, w1 - w, lane);
       const int n = u.end - u.pos;
       const int kx = u.kv * HD, vx = (a.c.kv_heads + u.kv) * HD + vhalf * VD;
       if (!first_q) {
@@ -539,13 +558,12 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
           tma_load_4d(qs + c * kQChunk, &maps.q, &bars[B_Q], c * 64, 0, u.kv, u.tile.tok0);
       }
       __syncwarp();
-      int row = slot_row(u), before = -1;
+      int key, page = slot_page(u, &key), before = -1;
       for (int t = 0; t < n && ok; ++t) {
-        // The next tile's pages are looked up before this one's waits.
-        int ahead = -1;
+        const int row = row_of(page, key);
         if (t + 1 < n) {
-          u.next(a);
-          ahead = slot_row(u);
+          u.next();
+          page = slot_page(u, &key);
         }
         __syncwarp();
 #pragma unroll
@@ -557,7 +575,6 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
           if (t > 0 && ok) load_stage(before, vx, true);
           before = row;
         }
-        row = ahead;
       }
       if (KST == 2 && ok) load_stage(before, vx, true);
       w += n;
@@ -630,9 +647,12 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
       vr.next();
       return true;
     };
-    for (int w = w0; w < w1 && ok;) {
-      Share u;
-      u.enter(a, plan, w, w1, lane);
+    Share u;
+    u.rt = start.rt;
+    u.pos = start.pos;
+    u.kv = start.kv;
+    for (int w = w0; w < w1 && ok; u.leave(plan.n_tiles)) {
+      u.load(tiles, runs, run_cap, w1 - w, lane);
       const int n = u.end - u.pos;
       if (!warp_wait(&bars[B_Q], qphase, abort_flag)) {
         ok = false;
@@ -644,7 +664,7 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
         int rows[kSlots];
 #pragma unroll
         for (int i = 0; i < kSlots; ++i) rows[i] = __shfl_sync(0xffffffffu, u.run.rows, i);
-        if (t + 1 < n) u.next(a);
+        if (t + 1 < n) u.next();
         __syncwarp();
         const int b = g & 1;
         // The score buffer's last reader finished before the P of two tiles
@@ -714,9 +734,12 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
       clean_phase ^= 1;
       return met;
     };
-    for (int w = w0; w < w1;) {
-      Share u;
-      u.enter(a, plan, w, w1, lane);
+    Share u;
+    u.rt = start.rt;
+    u.pos = start.pos;
+    u.kv = start.kv;
+    for (int w = w0; w < w1; u.leave(plan.n_tiles)) {
+      u.load(tiles, runs, run_cap, w1 - w, lane);
       const PagedTile tile = u.tile;
       const int kv = u.kv, n = u.end - u.pos;
       const bool first = w == w0, whole = n == tile.ntiles;
@@ -729,7 +752,7 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
       for (int c = 0; c < tile.nruns; c += 32) {
         int start = kRows + 1, stop = 0, i0 = 0;
         if (c + lane < tile.nruns) {
-          const PagedRun w = a.runs[tile.run0 + c + lane];
+          const PagedRun w = u.runs[c + lane];
           start = w.owner < 0 ? -1 : w.rows & 0xffff;
           stop = w.owner < 0 ? 0 : w.rows >> 16;
           i0 = w.i0;
@@ -1000,7 +1023,7 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
         ++g;
         vslot = ring_add<NST>(vslot, 2);
         vr.next();
-        if (done + 1 < n) u.next(a);
+        if (done + 1 < n) u.next();
         __syncwarp();
       }
       it += n * (KST + 1);
@@ -1107,9 +1130,10 @@ __global__ void __launch_bounds__(192, Shape<HD>::kCtasPerSm)
 // ---- merge ----------------------------------------------------------------------
 
 // A block takes the row tile that the boundary between CTA i - 1 and i cuts
-// first (later boundaries of the same tile leave), and of it the rows of its
-// row group. A warp per row and 128 dims (64 at head_dim 64).
+// first (later boundaries of the same tile leave), and of it every
+// kMergeSplit-th row. A warp per row and 128 dims (64 at head_dim 64).
 constexpr int kMergeWarps = 8;
+constexpr int kMergeSplit = 8;
 
 template <int HD, class T>
 __global__ void __launch_bounds__(32 * kMergeWarps) paged_merge_kernel(PagedAttnArgs a) {
@@ -1121,20 +1145,22 @@ __global__ void __launch_bounds__(32 * kMergeWarps) paged_merge_kernel(PagedAttn
   griddep_launch();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const PagedPlan plan = *a.plan;
-  const int total = plan.line * a.c.kv_heads;
-  const int per = max((total + a.ctas - 1) / a.ctas, a.min_tiles);
   const int i = blockIdx.x + 1;
-  const int w = i * per;
-  if (w >= total) return;
-  const int kv = w / plan.line, wl = w - kv * plan.line;
-  const int rt = warp_count_le(a.tile_cum, plan.n_tiles, wl, lane) - 1;
-  const PagedTile t = a.tiles[rt];
-  const int e0 = kv * plan.line + a.tile_cum[rt];
+  const int per = plan.per, w = i * per;
+  PagedStart st = a.one_tile ? PagedStart{} : a.starts[i];
+  if (w >= plan.line * a.c.kv_heads) return;
+  if (a.one_tile) {
+    st.kv = w / plan.line;
+    st.pos = w - st.kv * plan.line;
+  }
+  const int kv = st.kv, e0 = w - st.pos;
   if (e0 == w || (i - 1) * per > e0) return;
+  const PagedTile t = a.tiles[st.rt];
   const int c0 = i - 1, c1 = (e0 + t.ntiles - 1) / per;
-  const int r = blockIdx.y * kRowsHere + warp / kRowWarps;
-  if (r >= t.ntok * a.hpg) return;
   const int d0 = (warp % kRowWarps) * kPer + lane * kLane;
+  const int nrows = t.ntok * a.hpg;
+  for (int r = blockIdx.y + kMergeSplit * (warp / kRowWarps); r < nrows;
+       r += kMergeSplit * kRowsHere) {
   auto slot_row = [&](int c) {
     return (2 * static_cast<size_t>(c) + (c * per >= e0 ? 0 : 1)) * kRows + r;
   };
@@ -1188,7 +1214,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) paged_merge_kernel(PagedAttn
     }
   }
   const float inv = lsum > 0.f ? 1.0f / lsum : lsum != lsum ? lsum : 0.f;
-  const int tok = r / a.hpg;
+  const int tok = r * a.hpg_recip >> 16;
   T* o = static_cast<T*>(a.out) + (t.tok0 + tok) * a.out_stride +
          (kv * a.hpg + r - tok * a.hpg) * HD + d0;
   uint32_t h[kLane / 2];
@@ -1198,21 +1224,19 @@ __global__ void __launch_bounds__(32 * kMergeWarps) paged_merge_kernel(PagedAttn
     *reinterpret_cast<uint2*>(o) = make_uint2(h[0], h[1]);
   else
     *reinterpret_cast<uint32_t*>(o) = h[0];
+  }
 }
 
 template <int HD, class T>
 void launch(const PagedAttnArgs& a, const PagedMaps& m, cudaStream_t s) {
-  const int groups = std::max(a.b.n_groups, 1);
-  launch_pdl(paged_plan_kernel, dim3(1), dim3(kPlanThreads),
-             plan_smem_ints(groups, a.max_tiles, a.max_segs) * 4, s, a);
-  launch_pdl(paged_attention_kernel<HD, T>, dim3(a.ctas, Shape<HD>::kHalves), dim3(192),
+  if (!a.one_tile)
+    launch_pdl(paged_plan_kernel, dim3(1), dim3(kPlanThreads),
+               plan_smem_ints(a.b.n_seqs, std::max(a.b.n_groups, 1), a.max_tiles) * 4, s, a);
+  launch_pdl(paged_attention_kernel<HD, T>, dim3(a.ctas, Shape<HD>::kHalves), dim3(kThreads),
              Shape<HD>::kSmem, s, m, a);
-  if (a.ctas > 1) {
-    const int rows = std::min<int64_t>(kRows, static_cast<int64_t>(a.b.tokens) * a.hpg);
-    constexpr int kRowsHere = kMergeWarps / (HD < 128 ? 1 : HD / 128);
-    launch_pdl(paged_merge_kernel<HD, T>, dim3(a.ctas - 1, (rows + kRowsHere - 1) / kRowsHere),
-               dim3(32 * kMergeWarps), 0, s, a);
-  }
+  if (a.ctas > 1)
+    launch_pdl(paged_merge_kernel<HD, T>, dim3(a.ctas - 1, kMergeSplit), dim3(32 * kMergeWarps), 0,
+               s, a);
 }
 
 template <int HD>
@@ -1246,17 +1270,18 @@ size_t paged_attention_layout(PagedAttnArgs* a, int num_sms) {
   a->hpg_recip = (65536 + a->hpg - 1) / a->hpg;
   const int64_t tiles = (static_cast<int64_t>(a->b.tokens) + a->tpt - 1) / a->tpt +
                         std::min<int64_t>(groups, a->b.tokens);
-  const int64_t segs = tiles + a->b.n_seqs, runs = segs + tiles;
-  if (plan_smem_ints(groups, tiles, segs) * 4 > kPlanSmemMax) return 0;
-  a->max_runs = static_cast<int>(runs);
+  if (plan_smem_ints(a->b.n_seqs, groups, tiles) * 4 > kPlanSmemMax) return 0;
   a->max_tiles = static_cast<int>(tiles);
-  a->max_segs = static_cast<int>(segs);
+  // One row tile of few runs (a batch of branches of one state, a token each):
+  // planned by every CTA for itself, which spares a launch.
+  a->one_tile = a->b.n_groups <= 1 && a->b.tokens <= a->tpt &&
+                std::min(a->b.n_seqs, a->tpt) < one_tile_runs(a->c.hd);
   const int per_sm = a->c.hd <= 128 ? 2 : 1;
   a->ctas = std::max(num_sms * per_sm / (a->c.hd == 512 ? 2 : 1), 1);
   a->min_tiles = 2;
   const size_t slots = 2 * static_cast<size_t>(a->ctas) * kRows;
-  return align_up(sizeof(PagedPlan)) + align_up((tiles + 1) * 4) +
-         align_up((runs + 1) * sizeof(PagedRun)) +
+  return align_up(sizeof(PagedPlan)) + align_up(a->ctas * sizeof(PagedStart)) +
+         align_up(tiles * (a->tpt + 1) * sizeof(PagedRun)) +
          align_up(tiles * sizeof(PagedTile)) + align_up(slots * 8) + slots * a->c.hd * 4;
 }
 
@@ -1269,9 +1294,9 @@ void paged_attention_workspace(PagedAttnArgs* a, void* ws) {
   };
   const size_t slots = 2 * static_cast<size_t>(a->ctas) * kRows;
   a->plan = static_cast<PagedPlan*>(take(sizeof(PagedPlan)));
-  const size_t runs = static_cast<size_t>(a->max_runs) + 1;
-  a->tile_cum = static_cast<int*>(take((static_cast<size_t>(a->max_tiles) + 1) * 4));
-  a->runs = static_cast<PagedRun*>(take(runs * sizeof(PagedRun)));
+  a->starts = static_cast<PagedStart*>(take(a->ctas * sizeof(PagedStart)));
+  a->runs = static_cast<PagedRun*>(
+      take(static_cast<size_t>(a->max_tiles) * (a->tpt + 1) * sizeof(PagedRun)));
   a->tiles = static_cast<PagedTile*>(take(static_cast<size_t>(a->max_tiles) * sizeof(PagedTile)));
   a->part_ml = static_cast<float2*>(take(slots * 8));
   a->part_o = static_cast<float*>(take(slots * a->c.hd * 4));

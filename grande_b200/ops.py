@@ -246,8 +246,7 @@ def paged_attention(q: torch.Tensor, cache: torch.Tensor, batch: PagedBatch, *,
     n, heads, _ = shape = q.shape
     out = _out(op, out, shape, q)
     if workspace is None:
-        workspace = torch.empty(_workspace(index, c, batch, n, heads), dtype=torch.uint8,
-                                device=cache.device)
+        workspace = cache.new_empty(_workspace(index, c, batch, n, heads), dtype=torch.uint8)
     elif workspace.get_device() != index or workspace.dtype is not torch.uint8 or (
             not workspace.is_contiguous()):
         _fail(f"{op}: the workspace must be contiguous uint8 on cuda:{index}")
