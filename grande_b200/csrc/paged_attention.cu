@@ -113,35 +113,56 @@ __device__ __forceinline__ int last_le(const int* a, int n, int v) {
   return lo - 1;
 }
 
-// Row tile `rt`, tokens [t0, t1) of group g: its record and its runs. A full
-// warp calls it, a lane per sequence; `s` is the first sequence that may have
-// tokens there, `s_end` the group's end.
-__device__ void plan_tile(const PagedAttnArgs& a, const int* q, const int* lens, int rt, int g,
-                          int plen, int t0, int t1, int s, int s_end, PagedRun* runs,
-                          PagedTile* out) {
+// Row tile `rt`, tokens [t0, t1) of group g: its record and its runs; returns
+// its key tiles. A full warp calls it, a lane per sequence; `first` is the
+// first sequence that may have tokens there, `s_end` the group's end.
+__device__ int plan_tile(const PagedAttnArgs& a, const int* q, const int* lens, int rt, int g,
+                         int plen, int t0, int t1, int first, int s_end, PagedRun* runs,
+                         PagedTile* out) {
   const int lane = threadIdx.x & 31;
   const int own_cap = a.b.max_pages << a.c.page_log2;
   const int pre_cap = a.b.n_groups > 0 ? a.b.max_prefix_pages << a.c.page_log2 : 0;
-  // The own runs, placed as if no prefix came before them.
-  int imin = INT_MAX, imax = INT_MIN, slots = 0, n_runs = 0;
-  for (; s < s_end; s += 32) {
-    const int me = s + lane;
-    int n = 0, ta = 0, tb = 0, key0 = 0, kend = 0, i0 = 0, q0 = t1;
-    if (me < s_end) {
-      q0 = q[me];
-      const int q1 = q[me + 1];
-      ta = max(q0, t0);
-      tb = min(q1, t1);
-      if (ta < tb) {
-        i0 = lens[me] - (q1 - ta);
-        const int i1 = i0 + (tb - ta) - 1;
-        imin = min(imin, i0);
-        imax = max(imax, i1);
-        kend = min(i1 + 1, own_cap);
-        const int lo = a.window > 0 ? max(0, i0 - a.window + 1) : 0;
-        key0 = lo / kSlot * kSlot;
-        n = kend > lo ? (kend - key0 + kSlot - 1) / kSlot : 0;
-      }
+  // Sequence `s`'s tokens [ta, tb) of the tile; i0: own index of the first.
+  auto part = [&](int s, int* ta, int* tb, int* i0) -> bool {
+    *ta = *tb = 0;
+    *i0 = 0;
+    if (s >= s_end) return false;
+    const int q0 = q[s], q1 = q[s + 1], len = lens[s];
+    *ta = max(q0, t0);
+    *tb = min(q1, t1);
+    *i0 = len - (q1 - *ta);
+    return q0 >= t1;  // the sequences from here on are past the tile
+  };
+  int imin = INT_MAX, imax = INT_MIN;
+  int ta, tb, i0;
+  int chunks = 0;
+  for (int s = first; s < s_end; s += 32) {
+    const bool past = part(s + lane, &ta, &tb, &i0);
+    if (ta < tb) {
+      imin = min(imin, i0);
+      imax = max(imax, i0 + (tb - ta) - 1);
+    }
+    ++chunks;
+    if (__any_sync(0xffffffffu, past)) break;
+  }
+  imin = __reduce_min_sync(0xffffffffu, imin);
+  imax = __reduce_max_sync(0xffffffffu, imax);
+  // The prefix's slots, then the own runs.
+  const int end = min(plen, pre_cap);
+  const int lo = a.window > 0 && imin != INT_MAX ? max(0, plen + imin - a.window + 1) : 0;
+  int key0 = lo / kSlot * kSlot, kend = end;
+  int pre = lo < end ? (end - key0 + kSlot - 1) / kSlot : 0;
+  const int held = pre;
+  int slots = 0, n_runs = 0;
+  for (int c = 0; c < chunks; ++c) {
+    const int me = first + 32 * c + lane;
+    if (chunks > 1) part(me, &ta, &tb, &i0);  // one chunk: still at hand
+    int n = 0, k0 = 0, ke = 0;
+    if (ta < tb) {
+      ke = min(i0 + (tb - ta), own_cap);
+      const int l = a.window > 0 ? max(0, i0 - a.window + 1) : 0;
+      k0 = l / kSlot * kSlot;
+      n = ke > l ? (ke - k0 + kSlot - 1) / kSlot : 0;
     }
     int upto = n;
 #pragma unroll
@@ -153,40 +174,34 @@ __device__ void plan_tile(const PagedAttnArgs& a, const int* q, const int* lens,
     const int at = n_runs + __popc(have & ((1u << lane) - 1));
     // (No more runs than tokens in a tile, but for tables out of order.)
     if (n > 0 && at < a.tpt)
-      runs[1 + at] = PagedRun{rt,   slots + upto - n,
-                              n,    key0,
-                              kend, ((ta - t0) * a.hpg) | (((tb - t0) * a.hpg) << 16),
-                              i0,   me};
+      runs[1 + at] = PagedRun{rt, held + slots + upto - n,
+                              n,  k0,
+                              ke, ((ta - t0) * a.hpg) | (((tb - t0) * a.hpg) << 16),
+                              i0, me};
     n_runs = min(n_runs + __popc(have), a.tpt);
     slots += __shfl_sync(0xffffffffu, upto, 31);
-    if (__any_sync(0xffffffffu, me < s_end && q0 >= t1)) break;
   }
-  imin = __reduce_min_sync(0xffffffffu, imin);
-  imax = __reduce_max_sync(0xffffffffu, imax);
-  // The prefix's slots. Rows that see nothing at all still get their zeros:
-  // one slot, all of it masked.
-  const int end = min(plen, pre_cap);
-  const int lo = a.window > 0 && imin != INT_MAX ? max(0, plen + imin - a.window + 1) : 0;
-  int key0 = lo / kSlot * kSlot, kend = end, pre = lo < end ? (end - key0 + kSlot - 1) / kSlot : 0;
+  // Rows that see nothing at all still get their zeros: one slot, all of it
+  // masked. (A prefix run of no slots stays, before the own runs.)
   if (pre + slots == 0) {
     pre = 1;
     key0 = kend = 0;
   }
-  __syncwarp();
-  for (int i = lane; i < n_runs; i += 32) runs[1 + i].slot0 += pre;
+  const int ntiles = (pre + slots + kSlots - 1) / kSlots;
   if (lane == 0) {
     runs[0] = PagedRun{rt, 0, pre, key0, kend, ((t1 - t0) * a.hpg) << 16, 0, ~g};
     PagedTile t{};
     t.tok0 = t0;
     t.ntok = t1 - t0;
     t.prefix_len = plen;
-    t.ntiles = (pre + slots + kSlots - 1) / kSlots;
+    t.ntiles = ntiles;
     t.nruns = 1 + n_runs;
     t.imin = imin;
     t.imax = imax;
     *out = t;
   }
   __syncwarp();
+  return ntiles;
 }
 
 __device__ __forceinline__ int tiles_per_cta(const PagedAttnArgs& a, int line) {
@@ -244,9 +259,9 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedAttnArgs 
     const int t1 = min(t0 + a.tpt, q[gs[g + 1]]);
     // The last sequence that starts at or before the first token.
     const int s = max(gs[g], warp_count_le(q + gs[g], gs[g + 1] - gs[g], t0, lane) - 1 + gs[g]);
-    plan_tile(a, q, len, rt, g, plen[g], t0, t1, s, gs[g + 1],
-              a.runs + static_cast<int64_t>(rt) * (a.tpt + 1), a.tiles + rt);
-    if (lane == 0) cum[rt] = a.tiles[rt].ntiles;
+    const int n = plan_tile(a, q, len, rt, g, plen[g], t0, t1, s, gs[g + 1],
+                            a.runs + static_cast<int64_t>(rt) * (a.tpt + 1), a.tiles + rt);
+    if (lane == 0) cum[rt] = n;
   }
   __syncthreads();
   int line = 0;
@@ -1032,6 +1047,7 @@ __global__ void __launch_bounds__(kThreads, Shape<HD>::kCtasPerSm)
       tc_fence_after();
       const size_t slot = 2 * static_cast<size_t>(blockIdx.x) + (first ? 0 : 1);
       float keep = 0.f;
+      const bool zero = l == 0.f && ok;  // O may hold anything
       if (whole) {
         keep = l > 0.f ? 1.0f / l : 0.f;
         if (l != l) keep = l;
@@ -1048,24 +1064,29 @@ __global__ void __launch_bounds__(kThreads, Shape<HD>::kCtasPerSm)
         // 128 bytes of each row at a time, then whole rows of it to memory.
         if (whole) {
           constexpr int kPass = 64;  // 16-bit values of 128 bytes
+          uint32_t o[2][32];
+          tmem_ld32_nowait(trow + Sh::kTmemO, o[0]);
+          tmem_ld32_nowait(trow + Sh::kTmemO + 32, o[1]);
 #pragma unroll 1
           for (int c = 0; c < VD / kPass; ++c) {
             uint8_t* st = my_stage[c & 1];
+            tmem_ld_wait();
+            if (Sh::kPSlots == 1) __syncwarp();
 #pragma unroll
-            for (int hh = 0; hh < 2; ++hh) {
-              float o[32];
-              tmem_ld32(trow + Sh::kTmemO + c * kPass + hh * 32, o);
+            for (int e = 0; e < 8; ++e) {
+              uint32_t h[4];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                uint32_t h[4];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                  const float x = o[8 * e + 2 * q], y = o[8 * e + 2 * q + 1];
-                  h[q] = pack2<T>(l == 0.f && ok ? 0.f : x * keep, l == 0.f && ok ? 0.f : y * keep);
-                }
-                *reinterpret_cast<uint4*>(st + lane * 128 + (((4 * hh + e) ^ (lane & 7)) << 4)) =
-                    make_uint4(h[0], h[1], h[2], h[3]);
+              for (int q = 0; q < 4; ++q) {
+                const float x = __uint_as_float(o[e >> 2][8 * (e & 3) + 2 * q]),
+                            y = __uint_as_float(o[e >> 2][8 * (e & 3) + 2 * q + 1]);
+                h[q] = zero ? 0u : pack2<T>(x * keep, y * keep);
               }
+              *reinterpret_cast<uint4*>(st + lane * 128 + ((e ^ (lane & 7)) << 4)) =
+                  make_uint4(h[0], h[1], h[2], h[3]);
+            }
+            if (c + 1 < VD / kPass) {
+              tmem_ld32_nowait(trow + Sh::kTmemO + (c + 1) * kPass, o[0]);
+              tmem_ld32_nowait(trow + Sh::kTmemO + (c + 1) * kPass + 32, o[1]);
             }
             __syncwarp();
             uint4 v[8];
@@ -1082,21 +1103,22 @@ __global__ void __launch_bounds__(kThreads, Shape<HD>::kCtasPerSm)
                      (kv * a.hpg + row - tok * a.hpg) * HD + vhalf * VD + c * kPass;
               if (i < rows_here) reinterpret_cast<uint4*>(o)[lane & 7] = v[e];
             }
-            __syncwarp();
           }
         } else {
           const uint32_t live = __ballot_sync(0xffffffffu, used);
           float* po = a.part_o + slot * kRows * HD + vhalf * VD;
+          uint32_t o[32];
+          tmem_ld32_nowait(trow + Sh::kTmemO, o);
 #pragma unroll 1
           for (int c = 0; c < VD / 32; ++c) {
             uint8_t* st = my_stage[c & 1];
-            float o[32];
-            tmem_ld32(trow + Sh::kTmemO + c * 32, o);
+            tmem_ld_wait();
+            if (Sh::kPSlots == 1) __syncwarp();
 #pragma unroll
             for (int e = 0; e < 8; ++e)
               *reinterpret_cast<uint4*>(st + lane * 128 + ((e ^ (lane & 7)) << 4)) =
-                  make_uint4(__float_as_uint(o[4 * e]), __float_as_uint(o[4 * e + 1]),
-                             __float_as_uint(o[4 * e + 2]), __float_as_uint(o[4 * e + 3]));
+                  make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            if (c + 1 < VD / 32) tmem_ld32_nowait(trow + Sh::kTmemO + (c + 1) * 32, o);
             __syncwarp();
             uint4 v[8];
 #pragma unroll
@@ -1111,9 +1133,9 @@ __global__ void __launch_bounds__(kThreads, Shape<HD>::kCtasPerSm)
                 reinterpret_cast<uint4*>(po + static_cast<size_t>(32 * q4 + i) * HD +
                                          c * 32)[lane & 7] = v[e];
             }
-            __syncwarp();
           }
         }
+        __syncwarp();
       }
       tc_fence_before();
       w += n;
@@ -1131,9 +1153,15 @@ __global__ void __launch_bounds__(kThreads, Shape<HD>::kCtasPerSm)
 
 // A block takes the row tile that the boundary between CTA i - 1 and i cuts
 // first (later boundaries of the same tile leave), and of it every
-// kMergeSplit-th row. A warp per row and 128 dims (64 at head_dim 64).
+// gridDim.y-th row. A warp per row and 128 dims (64 at head_dim 64).
 constexpr int kMergeWarps = 8;
-constexpr int kMergeSplit = 8;
+
+// Blocks that share a cut row tile's rows. Few row tiles are cut by many CTAs
+// each: many blocks, each with long sums. Many row tiles are cut once or
+// twice: every boundary has work, and more blocks than fit at once wait.
+// (One state, 12 branches: 8 blocks 22.4 us a call, 16 blocks 20.4; 64
+// states: 8 blocks 90 us, 16 blocks 95.6.)
+constexpr int merge_split(int64_t entries) { return entries < 64 ? 16 : 8; }
 
 template <int HD, class T>
 __global__ void __launch_bounds__(32 * kMergeWarps) paged_merge_kernel(PagedAttnArgs a) {
@@ -1141,26 +1169,39 @@ __global__ void __launch_bounds__(32 * kMergeWarps) paged_merge_kernel(PagedAttn
   constexpr int kRowWarps = HD / kPer;            // warps per row
   constexpr int kRowsHere = kMergeWarps / kRowWarps;
   constexpr int kLane = kPer / 32;                // dims per lane
+  constexpr int kMany = 4;                        // ranges summed at a time
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int i = blockIdx.x + 1;
+  PagedPlan plan;
+  PagedStart st;
+  PagedTile t;
+  auto read = [&]() {
+    plan = *a.plan;
+    if (a.one_tile) {
+      const int w = i * plan.per;
+      st.rt = 0;
+      st.kv = plan.line ? w / plan.line : 0;
+      st.pos = w - st.kv * plan.line;
+    } else {
+      st = a.starts[i];
+    }
+    t = a.tiles[st.rt];
+  };
+  // A plan of the plan kernel is there before the attention kernel lets this
+  // one start; one that the attention kernel made comes with its end.
+  if (!a.one_tile) read();
   griddep_wait();
   griddep_launch();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const PagedPlan plan = *a.plan;
-  const int i = blockIdx.x + 1;
+  if (a.one_tile) read();
   const int per = plan.per, w = i * per;
-  PagedStart st = a.one_tile ? PagedStart{} : a.starts[i];
   if (w >= plan.line * a.c.kv_heads) return;
-  if (a.one_tile) {
-    st.kv = w / plan.line;
-    st.pos = w - st.kv * plan.line;
-  }
   const int kv = st.kv, e0 = w - st.pos;
   if (e0 == w || (i - 1) * per > e0) return;
-  const PagedTile t = a.tiles[st.rt];
   const int c0 = i - 1, c1 = (e0 + t.ntiles - 1) / per;
   const int d0 = (warp % kRowWarps) * kPer + lane * kLane;
   const int nrows = t.ntok * a.hpg;
-  for (int r = blockIdx.y + kMergeSplit * (warp / kRowWarps); r < nrows;
-       r += kMergeSplit * kRowsHere) {
+  for (int r = blockIdx.y + gridDim.y * (warp / kRowWarps); r < nrows;
+       r += gridDim.y * kRowsHere) {
   auto slot_row = [&](int c) {
     return (2 * static_cast<size_t>(c) + (c * per >= e0 ? 0 : 1)) * kRows + r;
   };
@@ -1181,11 +1222,11 @@ __global__ void __launch_bounds__(32 * kMergeWarps) paged_merge_kernel(PagedAttn
     const float wt = ml.x == mmax || ml.x == -INFINITY ? 1.0f : exp2_fast(ml.x - mmax);
     uint32_t todo = __ballot_sync(0xffffffffu, live);
     while (todo) {
-      // Four ranges' loads in flight.
-      float v[4][kLane], wv[4], lv[4];
+      // Several ranges' loads in flight.
+      float v[kMany][kLane], wv[kMany], lv[kMany];
       int n = 0;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < kMany; ++k) {
         const int src = todo ? __ffs(todo) - 1 : 0;
         const bool on = todo != 0;
         if (on) ++n;
@@ -1204,7 +1245,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) paged_merge_kernel(PagedAttn
         }
       }
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < kMany; ++k) {
         if (k < n) {
 #pragma unroll
           for (int e = 0; e < kLane; ++e) acc[e] = fmaf(wv[k], v[k][e], acc[e]);
@@ -1235,7 +1276,7 @@ void launch(const PagedAttnArgs& a, const PagedMaps& m, cudaStream_t s) {
   launch_pdl(paged_attention_kernel<HD, T>, dim3(a.ctas, Shape<HD>::kHalves), dim3(kThreads),
              Shape<HD>::kSmem, s, m, a);
   if (a.ctas > 1)
-    launch_pdl(paged_merge_kernel<HD, T>, dim3(a.ctas - 1, kMergeSplit), dim3(32 * kMergeWarps), 0,
+    launch_pdl(paged_merge_kernel<HD, T>, dim3(a.ctas - 1, merge_split(static_cast<int64_t>(a.max_tiles) * a.c.kv_heads)), dim3(32 * kMergeWarps), 0,
                s, a);
 }
 
