@@ -26,6 +26,7 @@ namespace omg {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kMaxTokens = kThreads / 32;  // tokens of a block: a warp each
 
 template <class T>
 __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
@@ -66,138 +67,153 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
   *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// A head takes HD / 16 threads, each 8 dims of its lower half and the 8 they
-// are paired with; the block sweeps the heads of a token, all of them sharing
-// the token's rotation in shared memory.
+// A block takes `tb` tokens: a warp looks up each token's sequence, cache row
+// and position, the block computes their rotations into shared memory, then
+// sweeps their heads. A head takes HD / 16 threads, each 8 dims of its lower
+// half and the 8 they are paired with.
 template <int HD, class TI, class TO>
-__global__ void __launch_bounds__(kThreads) paged_append_kernel(PagedAppendArgs a) {
+__global__ void __launch_bounds__(kThreads) paged_append_kernel(PagedAppendArgs a, int tb) {
   constexpr int L = HD / 16;
   constexpr int kUnits = kThreads / L;
   constexpr int HALF = HD / 2;
-  __shared__ float2 rot[HALF];
-  __shared__ long long s_row;  // cache row of the token, -1: none
-  __shared__ int s_pos;        // its position
-  __shared__ int s_live;
-  griddep_wait();
-  griddep_launch();
-  const int tid = threadIdx.x, lane = tid & 31;
+  __shared__ float2 rot[kMaxTokens][HALF];
+  __shared__ long long s_row[kMaxTokens];  // cache row of the token, -1: none
+  __shared__ int s_pos[kMaxTokens];        // its position
+  __shared__ int s_live[kMaxTokens];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int l = tid % L, u_in = tid / L;
   const int kvh = a.c.kv_heads;
   const int nh = a.heads + (a.has_kv ? 2 * kvh : 0);
-  const TI* qkv = static_cast<const TI*>(a.qkv);
-  TO* q_out = static_cast<TO*>(a.q_out);
+  const int t0 = blockIdx.x * tb, nt = min(tb, a.b.tokens - t0);
+  const TI* qkv = static_cast<const TI*>(a.qkv) + t0 * a.qkv_stride;
+  TO* q_out = static_cast<TO*>(a.q_out) + t0 * a.q_stride;
   TO* cache = static_cast<TO*>(a.c.rows);
-  for (int t = blockIdx.x; t < a.b.tokens; t += gridDim.x) {
-    const TI* row = qkv + t * a.qkv_stride;
-    if (tid < 32) {
-      const int s = warp_count_le(a.b.q_start, a.b.n_seqs + 1, t, lane) - 1;
-      const bool live = s >= 0 && s < a.b.n_seqs;
-      int pos = 0;
-      long long crow = -1;
-      if (live) {
-        const int own = a.b.lens[s] - (a.b.q_start[s + 1] - t);
-        int prefix = 0;
-        if (a.b.n_groups > 0) {
-          const int g = warp_count_le(a.b.group_start, a.b.n_groups + 1, s, lane) - 1;
-          if (g >= 0 && g < a.b.n_groups) prefix = a.b.prefix_lens[g];
-        }
-        pos = prefix + own;
-        // A token without a place (a length below its query rows, a page
-        // outside the table or the pool) leaves the cache as it was.
-        const int pi = own >> a.c.page_log2;
-        if (own >= 0 && pi < a.b.max_pages) {
-          const int page = a.b.pages[static_cast<int64_t>(s) * a.b.max_pages + pi];
-          if (page >= 0 && page < a.c.n_pages)
-            crow = (static_cast<long long>(page) << a.c.page_log2) +
-                   (own & ((1 << a.c.page_log2) - 1));
-        }
-      }
-      if (lane == 0) {
-        s_row = crow;
-        s_pos = pos;
-        s_live = live;
-      }
+  griddep_wait();
+  griddep_launch();
+  // The first heads' values are on their way while the tokens are looked up.
+  float x[8], y[8];
+  int u = u_in, tok = u / nh, h = u - tok * nh;
+  auto fetch = [&]() {
+    if (tok < nt) {
+      const TI* row = qkv + tok * a.qkv_stride + h * HD + 8 * l;
+      load8(row, x);
+      load8(row + HALF, y);
     }
-    __syncthreads();
-    const bool live = s_live;
-    const long long crow = s_row;
+  };
+  fetch();
+  if (warp < nt) {
+    const int t = t0 + warp;
+    const int s = warp_count_le(a.b.q_start, a.b.n_seqs + 1, t, lane) - 1;
+    const bool live = s >= 0 && s < a.b.n_seqs;
+    int pos = 0;
+    long long crow = -1;
     if (live) {
-      for (int d = tid; d < a.n_freq; d += kThreads) {
-        const double turns = static_cast<double>(s_pos) * (a.inv_freq[d] * 0.15915494309189535);
-        float sn, cs;
-        sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &sn, &cs);
-        rot[d] = make_float2(cs, sn);
+      const int own = a.b.lens[s] - (a.b.q_start[s + 1] - t);
+      int prefix = 0;
+      if (a.b.n_groups > 0) {
+        const int g = warp_count_le(a.b.group_start, a.b.n_groups + 1, s, lane) - 1;
+        if (g >= 0 && g < a.b.n_groups) prefix = a.b.prefix_lens[g];
+      }
+      pos = prefix + own;
+      // A token without a place (a length below its query rows, a page
+      // outside the table or the pool) leaves the cache as it was.
+      const int pi = own >> a.c.page_log2;
+      if (own >= 0 && pi < a.b.max_pages) {
+        const int page = a.b.pages[static_cast<int64_t>(s) * a.b.max_pages + pi];
+        if (page >= 0 && page < a.c.n_pages)
+          crow = (static_cast<long long>(page) << a.c.page_log2) +
+                 (own & ((1 << a.c.page_log2) - 1));
       }
     }
-    __syncthreads();
-    for (int u0 = 0; live && u0 < nh; u0 += kUnits) {
-      const int h = u0 + u_in;
-      const bool on = h < nh;
-      float x[8], y[8];
-      if (on) {
-        load8(row + h * HD + 8 * l, x);
-        load8(row + h * HD + HALF + 8 * l, y);
-      }
-      const bool is_q = h < a.heads, is_v = h >= a.heads + kvh;
-      const float* w = is_q ? a.q_norm : is_v ? nullptr : a.k_norm;
-      float ss = 0.f;
+    if (lane == 0) {
+      s_row[warp] = crow;
+      s_pos[warp] = pos;
+      s_live[warp] = live;
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < nt * a.n_freq; i += kThreads) {
+    const int k = i / a.n_freq, d = i - k * a.n_freq;
+    const double turns = static_cast<double>(s_pos[k]) * (a.inv_freq[d] * 0.15915494309189535);
+    float sn, cs;
+    sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &sn, &cs);
+    rot[k][d] = make_float2(cs, sn);
+  }
+  __syncthreads();
+  for (int u0 = 0; u0 < nt * nh; u0 += kUnits) {
+    const int ht = h, tt = tok;
+    const bool on = tt < nt && s_live[min(tt, kMaxTokens - 1)];
+    const bool is_q = ht < a.heads, is_v = ht >= a.heads + kvh;
+    const float* w = is_q ? a.q_norm : is_v ? nullptr : a.k_norm;
+    float v[8], z[8];
+    float ss = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss += x[e] * x[e] + y[e] * y[e];
+    for (int e = 0; e < 8; ++e) {
+      v[e] = x[e];
+      z[e] = y[e];
+      ss += v[e] * v[e] + z[e] * z[e];
+    }
+    // The next heads' values.
+    u += kUnits;
+    tok = u / nh;
+    h = u - tok * nh;
+    fetch();
 #pragma unroll
-      for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      if (!on) continue;
-      if (is_v ? a.v_norm : w != nullptr) {
-        const float inv = rsqrtf(ss * (1.0f / HD) + a.eps);
+    for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if (!on) continue;
+    if (is_v ? a.v_norm : w != nullptr) {
+      const float inv = rsqrtf(ss * (1.0f / HD) + a.eps);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          x[e] *= inv;
-          y[e] *= inv;
-        }
-      }
-      if (!is_v) {
-        if (w) {
-          float wx[8], wy[8];
-          load8(w + 8 * l, wx);
-          load8(w + HALF + 8 * l, wy);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            x[e] *= a.norm_offset + wx[e];
-            y[e] *= a.norm_offset + wy[e];
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (8 * l + e < a.n_freq) {
-            const float2 r = rot[8 * l + e];
-            const float p = x[e] * r.x - y[e] * r.y;
-            y[e] = y[e] * r.x + x[e] * r.y;
-            x[e] = p;
-          }
-        }
-      }
-      if (is_q) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          x[e] *= a.q_scale;
-          y[e] *= a.q_scale;
-        }
-        TO* o = q_out + t * a.q_stride + h * HD + 8 * l;
-        store8(o, x);
-        store8(o + HALF, y);
-      } else if (crow >= 0) {
-        TO* o = cache + crow * (2 * kvh * HD) + (h - a.heads) * HD + 8 * l;
-        store8(o, x);
-        store8(o + HALF, y);
+      for (int e = 0; e < 8; ++e) {
+        v[e] *= inv;
+        z[e] *= inv;
       }
     }
-    __syncthreads();
+    if (!is_v) {
+      if (w) {
+        float wv[8], wz[8];
+        load8(w + 8 * l, wv);
+        load8(w + HALF + 8 * l, wz);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          v[e] *= a.norm_offset + wv[e];
+          z[e] *= a.norm_offset + wz[e];
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (8 * l + e < a.n_freq) {
+          const float2 r = rot[tt][8 * l + e];
+          const float p = v[e] * r.x - z[e] * r.y;
+          z[e] = z[e] * r.x + v[e] * r.y;
+          v[e] = p;
+        }
+      }
+    }
+    if (is_q) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        v[e] *= a.q_scale;
+        z[e] *= a.q_scale;
+      }
+      TO* o = q_out + tt * a.q_stride + ht * HD + 8 * l;
+      store8(o, v);
+      store8(o + HALF, z);
+    } else if (s_row[tt] >= 0) {
+      TO* o = cache + s_row[tt] * (2 * kvh * HD) + (ht - a.heads) * HD + 8 * l;
+      store8(o, v);
+      store8(o + HALF, z);
+    }
   }
 }
 
 template <int HD, class TI, class TO>
 void launch(const PagedAppendArgs& a, int num_sms, cudaStream_t s) {
-  const int grid = std::min(a.b.tokens, num_sms * 8);
-  launch_pdl(paged_append_kernel<HD, TI, TO>, dim3(grid), dim3(kThreads), 0, s, a);
+  // A token per block while that does not fill the GPU (5 blocks fit an SM),
+  // then 8: the lookups and the barriers are paid once for all of them.
+  const int tb = a.b.tokens <= num_sms * 5 ? 1 : kMaxTokens;
+  launch_pdl(paged_append_kernel<HD, TI, TO>, dim3((a.b.tokens + tb - 1) / tb), dim3(kThreads), 0, s,
+             a, tb);
 }
 
 template <int HD>
