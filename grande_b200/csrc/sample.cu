@@ -49,7 +49,8 @@ constexpr int kScale = 44;       // weights in units of 2^-44
 constexpr int kMaxCluster = 16;
 constexpr int kSliceBytes = 160 * 1024;     // of a row in a CTA's shared memory
 constexpr int kEach = kList / kThreads;     // list entries per thread
-constexpr int kRankSort = 512;              // lists up to this are sorted by counting
+constexpr int kRankSort = 256;              // lists up to this are sorted by counting
+constexpr u64 kDropped = 1ull << 63;        // list entries that a filter took out
 constexpr int kSubBits = 11;     // refinement: up to 2^11 bins of the (value, index) order
 
 // The crossing bin of a search: what lies before it, what it holds, and the
@@ -127,6 +128,10 @@ struct Weigher {
     return m >= kLast ? bin_of_mark(m) : -1;
   }
   __device__ __forceinline__ u64 weight(float x, unsigned bin) const {
+    return weight(x, bin, table[bin]);
+  }
+  // `b`: 2^(44 - bin / 64), the table's entry.
+  __device__ __forceinline__ u64 weight(float x, unsigned bin, double b) const {
     // The bin as a double, through the low bits of 2^52.
     const double db = __hiloint2double(0x43300000, bin) - 4503599627370496.0;
     const double r = fma(static_cast<double>(x) - bestd, c64d, db);
@@ -134,7 +139,6 @@ struct Weigher {
     double p = fma(r, l * l * l * l / 24, l * l * l / 6);
     p = fma(p, r, l * l / 2);
     p = fma(p, r, l);
-    const double b = table[bin];
     const double w = fma(b * r, p, b) + 4503599627370496.0;
     return (static_cast<u64>(__double2hiint(w) - 0x43300000) << 32) |
            static_cast<unsigned>(__double2loint(w));
@@ -210,22 +214,28 @@ __device__ __forceinline__ u64 floor_part(float u, u64 m) {
   return __umul64hi(__double2ull_rz(static_cast<double>(u) * 18446744073709551616.0), m);
 }
 
-// Sort sh.l.comp[0 .. n) ascending; n <= kList. Short lists by counting the
-// smaller entries (all are distinct but for the padding ~0, which may land
-// anywhere behind), longer ones bitonically, padded to a power of two.
+// Sort sh.l.comp[0 .. n) ascending, all distinct; n <= kList. Short lists by
+// counting the smaller entries (n^2 / 128 times 5 instructions: 256 entries
+// 2,600 clocks, the bitonic sort of as many 36 barriers), longer ones
+// bitonically, padded to a power of two.
 __device__ void sort_list(Shared& sh, int n) {
   const int tid = threadIdx.x;
   __syncthreads();
   if (n <= kRankSort) {
     static_assert(kRankSort <= kThreads, "an entry per thread");
-    const u64 mine = tid < n ? sh.l.comp[tid] : ~0ull;
+    // Threads side by side share an entry's count: as many as there are.
+    int share = 32;
+    while (share * n > kThreads) share >>= 1;
+    const int entry = tid / share, part = tid & (share - 1);
+    const u64 mine = entry < n ? sh.l.comp[entry] : ~0ull;
     int at = 0;
-    if (tid < n) {
-#pragma unroll 8
-      for (int i = 0; i < n; ++i) at += sh.l.comp[i] < mine || (sh.l.comp[i] == mine && i < tid);
+    if (entry < n) {
+#pragma unroll 4
+      for (int i = part; i < n; i += share) at += sh.l.comp[i] < mine;
     }
+    for (int o = share >> 1; o > 0; o >>= 1) at += __shfl_xor_sync(0xffffffffu, at, o);
     __syncthreads();
-    if (tid < n) sh.l.comp[at] = mine;
+    if (entry < n && part == 0) sh.l.comp[at] = mine;
     __syncthreads();
     return;
   }
@@ -280,7 +290,19 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
       u.e[q] = at + q >= 0 && at + q < n ? src[at + q] : static_cast<T>(-INFINITY);
     return u.v;
   };
-  for (int i = tid; i < kBins; i += kThreads) sh.table[i] = exp2(kScale - i / 64.0);
+  // The row's settings come while the row does.
+  const float temp = a.temperature ? a.temperature[row] : a.temperature1;
+  int k = a.top_k ? a.top_k[row] : a.top_k1;
+  float top_p = a.top_p ? a.top_p[row] : a.top_p1;
+  float min_p = a.min_p ? a.min_p[row] : a.min_p1;
+  const float u = fminf(fmaxf(a.u[row], 0.0f), 0.99999994f);
+  // A row of one CTA needs no barrier but the block's.
+  auto sync = [&]() INLINE {
+    if (C == 1)
+      __syncthreads();
+    else
+      cluster.sync();
+  };
   if (tid == 0) {
     sh.list_n = 0;
     sh.threshold = ~0ull;
@@ -326,15 +348,10 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
     top = warp_max(sh.redf[lane]);
     if (lane == 0) sh.top = top;
   }
-  cluster.sync();
+  sync();
   top = warp_max(lane < C ? peer(lane).top : -INFINITY);
 
-  const float temp = a.temperature ? a.temperature[row] : a.temperature1;
-  int k = a.top_k ? a.top_k[row] : a.top_k1;
-  float top_p = a.top_p ? a.top_p[row] : a.top_p1;
-  float min_p = a.min_p ? a.min_p[row] : a.min_p1;
   min_p = min_p > 0.0f ? fminf(min_p, 1.0f) : 0.0f;
-  const float u = fminf(fmaxf(a.u[row], 0.0f), 0.99999994f);
   if (k <= 0 || k >= a.vocab) k = INT_MAX;
   if (!(top_p < 1.0f)) top_p = 1.0f;
   const bool dead = top == -INFINITY;
@@ -408,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
       at = __reduce_min_sync(0xffffffffu, sh.redc[lane]);
       if (lane == 0) sh.part_cnt = at;
     }
-    cluster.sync();
+    sync();
     if (rank == 0 && warp == 0) {
       at = __reduce_min_sync(0xffffffffu, lane < C ? peer(lane).part_cnt : UINT_MAX);
       if (lane == 0) {
@@ -416,7 +433,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
         if (a.probs) a.probs[row] = dead ? 0.0f : 1.0f;
       }
     }
-    cluster.sync();  // no CTA leaves while another may read its memory
+    sync();  // no CTA leaves while another may read its memory
     return;
   }
   Weigher wt;
@@ -455,7 +472,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
   // The first bin at which the running sum (of counts or masses) reaches
   // `target`; 0: top_p of the mass.
   auto find = [&](bool mass, u64 target) INLINE -> Found {
-    cluster.sync();
+    sync();
     const int share = kBins / C;  // C divides it
     const int each = (share + kThreads - 1) / kThreads;
     constexpr int kMost = (kBins + kThreads - 1) / kThreads;
@@ -502,7 +519,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
     u64 mx = mt, mtot;
     block_scan(sh, none, mx, &ntot, &mtot);
     if (tid == 0) sh.part_mass = mtot;
-    cluster.sync();
+    sync();
     const u64 part = lane < C ? peer(lane).part_mass : 0;
     const u64 all = warp_sum64(part);
     mx += warp_sum64(lane < rank ? part : 0);
@@ -520,7 +537,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
       }
       mx += m[e];
     }
-    cluster.sync();
+    sync();
     const Found f = sh.found;
     __syncthreads();  // read by all before the next sweep clears it
     return f;
@@ -555,7 +572,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
           ++at;
         }
     });
-    cluster.sync();
+    sync();
     int count = 0;
     if (rank == 0) {
       count = min(static_cast<int>(sh.list_n), kList);
@@ -567,7 +584,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
   auto list_weight = [&](u64 comp) INLINE -> u64 {
     const float v = value_of(comp);
     const int b = bin_of(v);
-    return b < 0 ? 0 : weight_of(v, b);
+    return b < 0 ? 0 : wt.weight(v, b, exp2(kScale - b / 64.0));
   };
 
   // Finds the last element that top-k (mass false, `count`) or top-p keeps
@@ -653,7 +670,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
           atomicMin(&sh.lo, mn);
           atomicMin(&sh.hi, mx);
         }
-        cluster.sync();
+        sync();
         lo = warp_min64(lane < C ? peer(lane).lo : ~0ull);
         hi = ~warp_min64(lane < C ? peer(lane).hi : ~0ull);
         first = false;
@@ -699,9 +716,9 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
         at += w[e];
       }
     }
-    cluster.sync();
+    sync();
     const u64 th = peer(0).threshold;
-    cluster.sync();
+    sync();
     return th;
   };
   auto finish = [&](int token, u64 w, u64 total) INLINE {
@@ -729,7 +746,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
       if (i < kept) {
         const bool stays = at < target && static_cast<double>(w[e]) >= min_w;
         const u64 idx = sh.l.comp[i] & 0xffffffffu;
-        sh.l.comp[i] = stays ? (idx << 32) | i : ~0ull;
+        sh.l.comp[i] = (stays ? idx << 32 : kDropped) | i;
         sh.l.w[i] = w[e];
       }
       at += w[e];
@@ -741,7 +758,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
     for (int e = 0; e < kEach; ++e) {
       const int i = kEach * tid + e;
       c[e] = i < kept ? sh.l.comp[i] : ~0ull;
-      w[e] = c[e] != ~0ull ? sh.l.w[c[e] & 0xffffffffu] : 0;
+      w[e] = c[e] < kDropped ? sh.l.w[c[e] & 0xffffffffu] : 0;
       at += w[e];
     }
     none = 0;
@@ -753,13 +770,16 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
     }
   };
 
+  // (Lists compute the few entries they need.)
+  if (k > kList)
+    for (int i = tid; i < kBins; i += kThreads) sh.table[i] = exp2(kScale - i / 64.0);
   u64 limit = ~0ull, goal = 0;
   int listed = -1;
   if (k != INT_MAX) {
     limit = search(false, k, limit, &listed, &goal);
     if (listed >= 0) {
       if (rank == 0) finish_list(min(listed, k), 0);
-      cluster.sync();
+      sync();
       return;
     }
   }
@@ -767,7 +787,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
     limit = search(true, UINT_MAX, limit, &listed, &goal);
     if (listed >= 0) {
       if (rank == 0) finish_list(listed, goal);
-      cluster.sync();
+      sync();
       return;
     }
   }
@@ -819,7 +839,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
   const u64 of_warp = sh.red[lane];
   u64 total = warp_sum64(of_warp);
   if (tid == 0) sh.part_mass = total;
-  cluster.sync();
+  sync();
   const u64 part = lane < C ? peer(lane).part_mass : 0;
   u64 before = warp_sum64(lane < rank ? part : 0);
   const u64 here = total;
@@ -871,16 +891,20 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
       });
     }
   }
-  cluster.sync();
+  sync();
 }
 
 constexpr int kShared = (sizeof(Shared) + 15) / 16 * 16;
 
 template <class T>
 void launch(const SampleArgs& a, int num_sms, cudaStream_t s) {
-  // CTAs per row: more than one only while there are SMs without a row.
+  // CTAs per row: more while there are SMs without a row and 8 elements per
+  // thread; below that the cluster's barriers cost more than the sweeps gain.
+  // (5 rows of 25,000: 20.1, 18.5, 16.4, 16.4, 20.5 us with 1, 2, 4, 8, 16.)
   int c = 1;
-  while (c < kMaxCluster && static_cast<int64_t>(a.rows) * c * 2 <= num_sms) c *= 2;
+  while (c < kMaxCluster && static_cast<int64_t>(a.rows) * c * 2 <= num_sms &&
+         a.vocab > c * 8 * kThreads)
+    c *= 2;
   const int slice = (a.vocab + c - 1) / c * static_cast<int>(sizeof(T)) + 16;
   const bool staged = slice <= kSliceBytes;
   cudaLaunchAttribute attr[1];
