@@ -102,6 +102,15 @@ class AttentionArgsC(C.Structure):
     ]
 
 
+class RowSamplingC(C.Structure):
+    # omg_row_sampling
+    _fields_ = [
+        ("u", C.c_void_p), ("temperature", C.c_void_p), ("top_k", C.c_void_p),
+        ("top_p", C.c_void_p), ("min_p", C.c_void_p), ("temperature_all", C.c_float),
+        ("top_k_all", C.c_int32), ("top_p_all", C.c_float), ("min_p_all", C.c_float),
+    ]
+
+
 class SampleArgsC(C.Structure):
     # omg_sample_args
     _fields_ = [
@@ -138,6 +147,8 @@ PROTOTYPES: dict[str, tuple] = {
     "omg_builder_finish": (C.c_int, [vp, sz, sz, pp]),
     "omg_builder_free": (None, [vp]),
     "omg_engine_evaluate_groups": (C.c_int, [vp, GroupP, sz, C.c_int, f32p, sz, i32p]),
+    "omg_engine_sample_groups": (C.c_int, [vp, GroupP, sz, C.POINTER(RowSamplingC), vp, vp, sz,
+                                           i32p]),
     "omg_engine_evaluate": (C.c_int, [vp, u32p, sz, BranchP, sz, C.c_int, f32p, sz]),
     "omg_engine_evaluate_rows": (C.c_int, [vp, u32p, sz, BranchP, sz, C.c_int, vp, sz, f32p, sz]),
     "omg_engine_warmup": (C.c_int, [vp]),

@@ -178,6 +178,23 @@ int omg_engine_evaluate_groups(omg_engine* e, const omg_group* groups, size_t n_
   });
 }
 
+int omg_engine_sample_groups(omg_engine* e, const omg_group* groups, size_t n_groups,
+                             const omg_row_sampling* p, int32_t* tokens, float* probs,
+                             size_t capacity, int32_t* prefix_sources) {
+  return guarded([&] {
+    auto gs = to_groups(groups, n_groups);
+    size_t rows = 0;
+    for (const GroupIn& g : gs) rows += g.rows();
+    if (!p || (rows && !p->u)) fail("sampling settings are null");
+    if (rows && !tokens) fail("tokens is null");
+    const RowSampling s{p->u,           p->temperature,     p->top_k,     p->top_p,
+                        p->min_p,       p->temperature_all, p->top_k_all, p->top_p_all,
+                        p->min_p_all,   tokens,             probs,        capacity};
+    eng(e).sample_groups(gs.data(), gs.size(), s, prefix_sources);
+    return 0;
+  });
+}
+
 int omg_engine_evaluate(omg_engine* e, const uint32_t* prefix, size_t n_prefix,
                         const omg_branch* branches, size_t n_branches, int want, float* out,
                         size_t out_floats) {

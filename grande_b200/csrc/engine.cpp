@@ -16,6 +16,7 @@
 
 #include "attention.cuh"
 #include "capi_util.h"
+#include "sample.cuh"
 
 namespace omg {
 
@@ -463,6 +464,7 @@ Engine::Engine(EngineBuilder&& b, size_t capacity_, size_t max_rows_)
   gemm_setup_device();
   attention_setup_device();
   logits_setup_device(config.d);
+  sample_setup_device();
 
   const Config& c = config;
   const int d = c.d, L = c.layers, P = c.per_layer_dim;
@@ -1236,22 +1238,8 @@ void Engine::check_status() {
     fail("a kernel gave up waiting (device status %u); the pass was abandoned", st);
 }
 
-void Engine::run(const GroupIn* groups, size_t n, size_t first,
-                 std::optional<PrefixSource> source, Want want, const uint8_t* per_layer_rows,
-                 size_t rows_bytes, float* out, size_t out_floats, int32_t* sources) {
-  CUDA_TRY(cudaSetDevice(device_));
-  Packing p = pack(groups, n, first, source.has_value());
+void Engine::read_rows(const Packing& p, Want want, float* out) {
   const size_t width = want == Want::Hidden ? config.d : config.vocab;
-  size_t total_rows = 0;
-  for (size_t i = 0; i < n; ++i) total_rows += groups[i].rows();
-  if (out_floats < total_rows * width)
-    fail("output buffer holds %zu floats, the request returns %zu", out_floats,
-         total_rows * width);
-  upload(p, per_layer_rows, rows_bytes);
-  if (stall_clocks_)
-    launch_forward(p, want);  // a test pass that must fail: never captured
-  else
-    run_forward(p, want);
   const float* src = want == Want::Logits ? logits_.as<float>() : rows_.as<float>();
   // A page-locked output buffer (omg_host_alloc) takes the rows straight from
   // the device, one copy per run of consecutive rows; any other buffer gets
@@ -1283,6 +1271,80 @@ void Engine::run(const GroupIn* groups, size_t n, size_t first,
     for (size_t i = 0; i + 1 < p.out_index.size(); i += 2)
       std::memcpy(out + p.out_index[i + 1] * width, h + p.out_index[i] * width, width * 4);
   }
+}
+
+void Engine::read_samples(const Packing& p, const RowSampling& s) {
+  // Device rows are in pass order, the caller's in (group, branch, want)
+  // order: settings go in and results come out through out_index.
+  const size_t rows = p.nwanted;
+  if (!sample_.p) {
+    sample_.alloc(std::max<size_t>(max_rows, 1) * 7 * 4, false);
+    h_sample_.alloc(std::max<size_t>(max_rows, 1) * 7 * 4);
+  }
+  float* h = h_sample_.as<float>();
+  int32_t* hk = h_sample_.as<int32_t>() + 2 * rows;
+  for (size_t i = 0; i + 1 < p.out_index.size(); i += 2) {
+    const size_t d = p.out_index[i], c = p.out_index[i + 1];
+    h[d] = s.u[c];
+    h[rows + d] = s.temperature ? s.temperature[c] : s.temperature1;
+    hk[d] = s.top_k ? s.top_k[c] : s.top_k1;
+    h[3 * rows + d] = s.top_p ? s.top_p[c] : s.top_p1;
+    h[4 * rows + d] = s.min_p ? s.min_p[c] : s.min_p1;
+  }
+  float* dv = sample_.as<float>();
+  if (rows) {
+    CUDA_TRY(cudaMemcpyAsync(dv, h, rows * 5 * 4, cudaMemcpyHostToDevice, stream_));
+    SampleArgs a{};
+    a.logits = logits_.p;
+    a.stride = config.vocab;
+    a.rows = static_cast<int>(rows);
+    a.vocab = config.vocab;
+    a.dtype = kOpF32;
+    a.u = dv;
+    a.temperature = dv + rows;
+    a.top_k = reinterpret_cast<const int*>(dv + 2 * rows);
+    a.top_p = dv + 3 * rows;
+    a.min_p = dv + 4 * rows;
+    a.tokens = reinterpret_cast<int*>(dv + 5 * rows);
+    a.probs = dv + 6 * rows;
+    launch_sample(a, num_sms_, stream_);
+    CUDA_TRY(cudaGetLastError());
+    CUDA_TRY(cudaMemcpyAsync(h + 5 * rows, dv + 5 * rows, rows * 2 * 4, cudaMemcpyDeviceToHost,
+                             stream_));
+  }
+  CUDA_TRY(cudaMemcpyAsync(h_status_.p, status_.p, 4, cudaMemcpyDeviceToHost, stream_));
+  CUDA_TRY(cudaStreamSynchronize(stream_));
+  check_status();
+  const int32_t* tok = h_sample_.as<int32_t>() + 5 * rows;
+  for (size_t i = 0; i + 1 < p.out_index.size(); i += 2) {
+    s.tokens[p.out_index[i + 1]] = tok[p.out_index[i]];
+    if (s.probs) s.probs[p.out_index[i + 1]] = h[6 * rows + p.out_index[i]];
+  }
+}
+
+void Engine::run(const GroupIn* groups, size_t n, size_t first,
+                 std::optional<PrefixSource> source, Want want, const uint8_t* per_layer_rows,
+                 size_t rows_bytes, float* out, size_t out_floats, int32_t* sources,
+                 const RowSampling* sampling) {
+  CUDA_TRY(cudaSetDevice(device_));
+  Packing p = pack(groups, n, first, source.has_value());
+  const size_t width = want == Want::Hidden ? config.d : config.vocab;
+  size_t total_rows = 0;
+  for (size_t i = 0; i < n; ++i) total_rows += groups[i].rows();
+  if (sampling && sampling->capacity < total_rows)
+    fail("output buffer holds %zu tokens, the request returns %zu", sampling->capacity, total_rows);
+  if (!sampling && out_floats < total_rows * width)
+    fail("output buffer holds %zu floats, the request returns %zu", out_floats,
+         total_rows * width);
+  upload(p, per_layer_rows, rows_bytes);
+  if (stall_clocks_)
+    launch_forward(p, want);  // a test pass that must fail: never captured
+  else
+    run_forward(p, want);
+  if (sampling)
+    read_samples(p, *sampling);
+  else
+    read_rows(p, want, out);
   {
     std::lock_guard<std::mutex> g(mu_);
     resident_ = std::vector<uint32_t>(groups[first].prefix,
@@ -1300,6 +1362,18 @@ void Engine::run(const GroupIn* groups, size_t n, size_t first,
 
 void Engine::evaluate_groups(const GroupIn* groups, size_t n, Want want, float* out,
                              size_t out_floats, int32_t* sources) {
+  evaluate(groups, n, want, out, out_floats, sources, nullptr);
+}
+
+void Engine::sample_groups(const GroupIn* groups, size_t n, const RowSampling& s,
+                           int32_t* sources) {
+  if (config.vocab > sample_max_vocab(kOpF32))
+    fail("sampling from a vocabulary of %d (at most %d)", config.vocab, sample_max_vocab(kOpF32));
+  evaluate(groups, n, Want::Logits, nullptr, 0, sources, &s);
+}
+
+void Engine::evaluate(const GroupIn* groups, size_t n, Want want, float* out, size_t out_floats,
+                      int32_t* sources, const RowSampling* sampling) {
   if (n == 0) fail("empty request");
   auto [first, source] = admit(groups, n);
   std::vector<uint8_t> rows;
@@ -1321,7 +1395,7 @@ void Engine::evaluate_groups(const GroupIn* groups, size_t n, Want want, float* 
     rows = gather_per_layer(ids.data(), ids.size());
   }
   run(groups, n, first, source, want, rows.empty() ? nullptr : rows.data(), rows.size(), out,
-      out_floats, sources);
+      out_floats, sources, sampling);
 }
 
 void Engine::evaluate_rows(const GroupIn& g, Want want, const uint8_t* per_layer_rows,

@@ -141,6 +141,22 @@ struct PinnedBuffer {
   template <class T> T* as() const { return static_cast<T*>(p); }
 };
 
+// Settings of a sampled request (sample.cuh), host memory in the rows' output
+// order: per-row arrays, or null and one value for all; and where the tokens
+// and their probabilities go (probs may be null).
+struct RowSampling {
+  const float* u;
+  const float* temperature;
+  const int32_t* top_k;
+  const float *top_p, *min_p;
+  float temperature1;
+  int32_t top_k1;
+  float top_p1, min_p1;
+  int32_t* tokens;
+  float* probs;
+  size_t capacity;  // rows that tokens and probs hold
+};
+
 class Engine;
 
 // engine.rs:805-1334 EngineBuilder: receives the weights one tensor at a
@@ -198,6 +214,9 @@ class Engine {
   // `sources[g]` the PrefixSource of each group (-1 none).
   void evaluate_groups(const GroupIn* groups, size_t n, Want want, float* out, size_t out_floats,
                        int32_t* sources);
+  // The same pass, a token sampled on the device from each wanted logits row:
+  // only the tokens and their probabilities leave it.
+  void sample_groups(const GroupIn* groups, size_t n, const RowSampling& s, int32_t* sources);
   // engine.rs:1449-1463: caller-gathered per-layer rows (f16 LE).
   void evaluate_rows(const GroupIn& g, Want want, const uint8_t* per_layer_rows,
                      size_t rows_bytes, float* out, size_t out_floats);
@@ -324,7 +343,13 @@ class Engine {
   int launch_forward(const Packing& p, Want want);
   void run(const GroupIn* groups, size_t n, size_t first, std::optional<PrefixSource> source,
            Want want, const uint8_t* per_layer_rows, size_t rows_bytes, float* out,
-           size_t out_floats, int32_t* sources);
+           size_t out_floats, int32_t* sources, const RowSampling* sampling = nullptr);
+  void evaluate(const GroupIn* groups, size_t n, Want want, float* out, size_t out_floats,
+                int32_t* sources, const RowSampling* sampling);
+  // The wanted rows to the caller's buffer, or (sampling) their tokens; waits
+  // for the pass and checks its status.
+  void read_rows(const Packing& p, Want want, float* out);
+  void read_samples(const Packing& p, const RowSampling& s);
   void check_status();
   void prof_mark(const char* name);
   bool profiling_ = false;
@@ -363,6 +388,9 @@ class Engine {
   std::vector<DevBuffer> kv_;  // per layer that owns K/V: [cap_rows, 2 * kv_heads * hd] f16
   size_t cap_rows_ = 0;
   PinnedBuffer h_ids_, h_meta_, h_row_map_, h_out_, h_status_;
+  // sample_groups: settings and results, five and two words per row.
+  DevBuffer sample_;
+  PinnedBuffer h_sample_;
   DevBuffer rope_tab_[2];  // [cap_rows][128] (cos, sin): local theta, global theta
   GemmPlan pl_model_proj_;
   DevBuffer w_pl_model_proj_;

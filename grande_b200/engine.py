@@ -93,6 +93,14 @@ class GroupOutput:
 
 
 @dataclass
+class SampleOutput:
+    """One branch's sampled answer rows in ``want`` order: token ids and their
+    probabilities in what the filters left."""
+    tokens: np.ndarray
+    probs: np.ndarray
+
+
+@dataclass
 class QTensor:
     """model.rs:376-384: raw little-endian payload plus f16 block scales."""
     dtype: Dtype
@@ -382,6 +390,54 @@ class Engine:
         if not groups:
             raise OmgError("empty request")
         return self._run(groups, want)
+
+    def sample(self, prefix, branches, uniforms, **settings) -> list:
+        """:meth:`sample_groups` of one group: a SampleOutput per branch."""
+        return self.sample_groups([Group(prefix, branches)], uniforms, **settings)[0].branches
+
+    def sample_groups(self, groups: Sequence[Group], uniforms, *, temperature=1.0, top_k=0,
+                      top_p=1.0, min_p=0.0) -> list:
+        """:meth:`evaluate_groups` with a token sampled on the device from each
+        wanted logits row: a GroupOutput of SampleOutputs per group, and no
+        logits row leaves the GPU. ``uniforms`` holds a number in [0, 1) per
+        wanted row in (group, branch, want) order; the settings
+        (:func:`grande_b200.ops.sample`) are a number for all rows or a
+        sequence with one per row."""
+        if not groups:
+            raise OmgError("empty request")
+        req = _Branches(groups)
+        nrows = sum(g.rows() for g in groups)
+        keep, fields = [], []
+
+        def per_row(name, v, dtype):
+            if v is not None and np.ndim(v) == 0:
+                return None, v
+            a = np.ascontiguousarray(v, dtype=dtype)
+            if a.shape != (nrows,):
+                raise OmgError(f"{name}: {list(a.shape)} values for {nrows} rows")
+            keep.append(a)
+            return a.ctypes.data if nrows else None, 0
+
+        if np.ndim(uniforms) != 1:
+            raise OmgError(f"uniforms: a sequence of {nrows} numbers, one per row")
+        u, _ = per_row("uniforms", uniforms, np.float32)
+        for name, v, dtype in (("temperature", temperature, np.float32), ("top_k", top_k, np.int32),
+                               ("top_p", top_p, np.float32), ("min_p", min_p, np.float32)):
+            fields.append(per_row(name, v, dtype))
+        s = _lib.RowSamplingC(u, *(f[0] for f in fields), *(f[1] for f in fields))
+        tokens = np.empty(nrows, dtype=np.int32)
+        probs = np.empty(nrows, dtype=np.float32)
+        srcs = (C.c_int32 * len(groups))()
+        check(lib().omg_engine_sample_groups(self._h, req.groups, len(groups), C.byref(s),
+                                             tokens.ctypes.data, probs.ctypes.data, nrows, srcs))
+        outs, r = [], 0
+        for gi, grp in enumerate(groups):
+            brs = []
+            for b in grp.branches:
+                brs.append(SampleOutput(tokens[r:r + len(b.want)], probs[r:r + len(b.want)]))
+                r += len(b.want)
+            outs.append(GroupOutput(brs, _source(srcs[gi])))
+        return outs
 
     def evaluate_rows(self, prefix, branches, want: Want, per_layer_rows: Optional[bytes]):
         """engine.rs:1449-1463."""

@@ -154,6 +154,28 @@ void omg_builder_free(omg_builder* b);
 int omg_engine_evaluate_groups(omg_engine* e, const omg_group* groups, size_t n_groups, int want,
                                float* out, size_t out_floats, int32_t* prefix_sources);
 
+/* Settings of a sampled request, host memory, a value per returned row in
+ * (group, branch, want) order, or NULL and the one value for all (omg_sample
+ * says what each does). */
+typedef struct {
+  const float* u;          /* [rows] uniform numbers in [0, 1) */
+  const float* temperature;
+  const int32_t* top_k;
+  const float *top_p, *min_p;
+  float temperature_all;
+  int32_t top_k_all;
+  float top_p_all, min_p_all;
+} omg_row_sampling;
+
+/* omg_engine_evaluate_groups with OMG_WANT_LOGITS, each row sampled on the
+ * device instead of read back (no reference counterpart; its readouts take
+ * whole rows, crates/omg-core/src/readout.rs:124-147): `tokens` and `probs`
+ * (may be NULL), `capacity` values each, get every wanted row's token and its
+ * probability in (group, branch, want) order. */
+int omg_engine_sample_groups(omg_engine* e, const omg_group* groups, size_t n_groups,
+                             const omg_row_sampling* sampling, int32_t* tokens, float* probs,
+                             size_t capacity, int32_t* prefix_sources);
+
 /* Engine::evaluate (engine.rs:1386-1398): one group. */
 int omg_engine_evaluate(omg_engine* e, const uint32_t* prefix, size_t n_prefix,
                         const omg_branch* branches, size_t n_branches, int want, float* out,
