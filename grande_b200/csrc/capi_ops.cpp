@@ -215,6 +215,8 @@ int omg_paged_attention(int device, const omg_paged_cache* cache, const omg_page
     if (p->tokens == 0 || batch->n_seqs == 0) return 0;
     check_aligned(op, "q", p->q, 16);
     check_aligned(op, "out", p->out, 16);
+    // (At head_dim 512 two CTAs read a row's q, and one may be done first.)
+    if (p->q == p->out) fail("%s: out is q", op);
     check_aligned(op, "workspace", workspace, 256);
     if (workspace_bytes < need)
       fail("%s: workspace of %zu bytes, %zu needed", op, workspace_bytes, need);

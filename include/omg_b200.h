@@ -575,7 +575,8 @@ size_t omg_paged_attention_workspace(int device, const omg_paged_cache* cache,
  * pages): a prefix is read once for all the sequences of its group. A row
  * that sees no key gets zeros. Keys and values a row does not see never
  * reach it, whatever they hold; a page id outside the pool reads as zeros.
- * A row whose kernel gave up waiting (a bounded device wait) is NaN. */
+ * A row whose kernel gave up waiting (a bounded device wait) is NaN. `out`
+ * must not overlap q. */
 int omg_paged_attention(int device, const omg_paged_cache* cache, const omg_paged_batch* batch,
                         const omg_attention_args* args, void* workspace, size_t workspace_bytes,
                         void* stream);

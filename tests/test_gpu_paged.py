@@ -263,3 +263,99 @@ def test_empty_calls_launch_nothing(device, torch, ops):
     out = torch.full_like(q, 7.0)
     ops.paged_attention(q, cache, none, out=out)
     assert (out == 7).all()
+
+
+def test_rows_past_32_bits_of_the_pool(device, torch, ops):
+    """A pool of 6 GB: rows whose byte and element offsets pass 2^32 and 2^31."""
+    dev = torch.device("cuda", device)
+    g = torch.Generator(device=dev).manual_seed(8)
+    b = Batch([(30, [(50, 1), (3, 2)])], 16, np.random.default_rng(8))
+    n_pages = 100000  # x 16 rows x 2,048 values x 2 bytes
+    cache = torch.empty((n_pages, 16, 2, 4, 256), dtype=torch.float16, device=dev)
+    up = n_pages - b.n_pages
+    cache[up:] = make_cache(torch, dev, b, 4, 256, torch.float16, g)
+    dev_b = b.device(ops, torch, dev, pages=b.pages + up, prefix_pages=b.prefix_pages + up)
+    qkv = torch.randn((b.tokens, 16 * 256), generator=g, device=dev)
+    before = cache[up:].clone()
+    q = ops.paged_append(qkv, cache, dev_b, heads=8)
+    _, exp_c = append(host(qkv), host(before), b, 8, None, None, 0.0, 0.0, False, np.zeros(0), 1.0)
+    used = b.used_rows()
+    got_c = host(cache[up:]).reshape(-1, 2048)[used]
+    assert np.abs(got_c - exp_c.reshape(-1, 2048)[used]).max() < 4e-3
+    out = ops.paged_attention(q, cache, dev_b, scale=0.05)
+    check_attention(out, q, cache[up:], b, np.float32(0.05), 0, "f16")
+
+
+def test_two_graphs_and_two_streams_with_workspaces_of_their_own(device, torch, ops):
+    dev = torch.device("cuda", device)
+    g = torch.Generator(device=dev).manual_seed(12)
+    b = Batch([(700, [(30, 1)] * 7), (90, [(200, 4)] * 3)], 32, np.random.default_rng(12))
+    cache = make_cache(torch, dev, b, 2, 128, torch.float16, g, fill=0.0)
+    dev_b = b.device(ops, torch, dev)
+    qs = [torch.randn((b.tokens, 8, 128), generator=g, device=dev).half() for _ in range(2)]
+    want = [ops.paged_attention(q, cache, dev_b, scale=0.1) for q in qs]
+    check_attention(want[0], qs[0], cache, b, np.float32(0.1), 0, "f16")
+    graphs, outs = [], []
+    for q in qs:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(ops.paged_attention(q, cache, dev_b, scale=0.1))
+    streams = [torch.cuda.Stream(dev) for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream(dev))
+    for _ in range(20):
+        for s, graph in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize(dev)
+    # The work is cut the same way each time, so the bits are the same.
+    assert all(torch.equal(o, w) for o, w in zip(outs, want))
+
+
+def test_a_first_call_under_capture(device, tmp_path):
+    """A process whose first call of each operator is captured."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = f"""
+import torch
+from grande_b200 import ops
+dev = torch.device("cuda", {device})
+torch.cuda.set_device(dev)
+i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)
+b = ops.PagedBatch(i32([0, 1, 2]), i32([3, 20]), i32([[0, 1], [2, 3]]))
+cache = torch.zeros((4, 16, 2, 1, 256), device=dev).half()
+qkv = torch.ones((2, 4 * 256), device=dev)
+u = torch.full((2,), 0.5, device=dev)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    q = ops.paged_append(qkv, cache, b, heads=2)
+    out = ops.paged_attention(q, cache, b)
+    tok, prob = ops.sample(out.view(2, 512), u)
+graph.replay()
+torch.cuda.synchronize()
+# The last key of each sequence is the row just appended, the others zeros.
+assert out[0].min() > 0.9 and tok.min() >= 0
+"""
+    root = Path(__file__).resolve().parent.parent
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True,
+                       timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
+def test_an_output_in_place_is_refused(device, torch, ops):
+    dev = torch.device("cuda", device)
+    b = Batch([(0, [(3, 1)])], 16, np.random.default_rng(1))
+    cache = torch.zeros((b.n_pages, 16, 2, 1, 64), device=dev).half()
+    q = torch.zeros((1, 1, 64), device=dev).half()
+    with pytest.raises(ops.OmgError, match="out is q"):
+        ops.paged_attention(q, cache, b.device(ops, torch, dev), out=q)
+    with pytest.raises(ops.OmgError, match="workspace of 256 bytes"):
+        ops.paged_attention(q, cache, b.device(ops, torch, dev),
+                            workspace=torch.empty(256, dtype=torch.uint8, device=dev))
+    with pytest.raises(ops.OmgError, match="out must be"):
+        ops.paged_attention(q, cache, b.device(ops, torch, dev), out=q[:, :, :32])
+    with pytest.raises(ops.OmgError, match="norm must be 64 contiguous"):
+        ops.paged_append(torch.zeros((1, 192), device=dev), cache, b.device(ops, torch, dev),
+                         heads=1, q_norm=torch.zeros(32, device=dev))
