@@ -126,8 +126,6 @@ vp = C.c_void_p
 pp = C.POINTER(C.c_void_p)
 cs = C.c_char_p
 sz = C.c_size_t
-CacheP = C.POINTER(PagedCacheC)
-BatchP = C.POINTER(PagedBatchC)
 GroupP = C.POINTER(GroupC)
 BranchP = C.POINTER(Branch)
 
@@ -223,11 +221,11 @@ PROTOTYPES: dict[str, tuple] = {
     "omg_laya_record_event": (C.c_int, [vp, C.c_int]),
     "omg_laya_elapsed_ms": (C.c_int, [vp, C.c_int, C.c_int, f32p]),
     "omg_laya_destroy": (None, [vp]),
-    "omg_paged_attention_workspace": (sz, [C.c_int, CacheP, BatchP, C.c_int, C.c_int]),
-    "omg_paged_attention": (C.c_int, [C.c_int, CacheP, BatchP, C.POINTER(AttentionArgsC), vp, sz,
-                                      vp]),
-    "omg_sample": (C.c_int, [C.c_int, C.POINTER(SampleArgsC), vp]),
-    "omg_paged_append": (C.c_int, [C.c_int, CacheP, BatchP, C.POINTER(AppendArgsC), vp]),
+    # (Their structs as plain pointers: packed bytes or references.)
+    "omg_paged_attention_workspace": (sz, [C.c_int, vp, vp, C.c_int, C.c_int]),
+    "omg_paged_attention": (C.c_int, [C.c_int, vp, vp, vp, vp, sz, vp]),
+    "omg_sample": (C.c_int, [C.c_int, vp, vp]),
+    "omg_paged_append": (C.c_int, [C.c_int, vp, vp, vp, vp]),
 }
 
 

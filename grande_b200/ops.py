@@ -21,6 +21,7 @@ A step of a batch of branches::
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from dataclasses import dataclass, field
 from typing import Optional
 
@@ -32,9 +33,26 @@ from ._lib import OmgError, check, lib
 
 _TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 
+# The argument structs of include/omg_b200.h, packed in one go: a call's host
+# time is a good part of a small batch's.
+_CACHE = struct.Struct("=Qqiiii")                  # omg_paged_cache
+_APPEND = struct.Struct("=QqiiiiQqQQifffQi4x")     # omg_append_args
+_ATTENTION = struct.Struct("=QqQqiiif")            # omg_attention_args
+_SAMPLE = struct.Struct("=Qqiii4xQQQQQfiffQQ")     # omg_sample_args
+assert (_CACHE.size, _APPEND.size, _ATTENTION.size, _SAMPLE.size) == tuple(
+    C.sizeof(t) for t in (_lib.PagedCacheC, _lib.AppendArgsC, _lib.AttentionArgsC,
+                          _lib.SampleArgsC))
+
 
 def _fail(msg: str):
     raise OmgError(msg)
+
+
+def _pack(op: str, s: struct.Struct, *values) -> bytes:
+    try:
+        return s.pack(*values)
+    except struct.error as e:
+        raise OmgError(f"{op}: an argument is not a number that fits ({e})") from None
 
 
 def _table(t, name: str, shape: tuple, device):
@@ -64,6 +82,8 @@ class PagedBatch:
     prefix_lens: Optional[torch.Tensor] = None
     prefix_pages: Optional[torch.Tensor] = None
     _c: object = field(init=False, repr=False, compare=False, default=None)
+    # Workspace bytes by shape: they follow from sizes alone.
+    _workspaces: dict = field(init=False, repr=False, compare=False, default_factory=dict)
 
     def __post_init__(self):
         dev = self.q_start.device
@@ -83,7 +103,8 @@ class PagedBatch:
             pp = self.prefix_pages.shape[1]
         ptr = [t.data_ptr() if t is not None and t.numel() else None
                for t in (self.q_start, self.lens, self.pages) + groups]
-        object.__setattr__(self, "_c", _lib.PagedBatchC(*ptr, n, g, self.pages.shape[1], pp))
+        c = _lib.PagedBatchC(*ptr, n, g, self.pages.shape[1], pp)
+        object.__setattr__(self, "_c", C.byref(c))
 
     def validate(self, cache: torch.Tensor, tokens: int):
         """Read the tables back (this waits for the device) and raise on the
@@ -138,7 +159,8 @@ def rope_frequencies(theta: float, head_dim: int, rope_dims: Optional[int] = Non
 # The checks below run before every launch: they read each property of a tensor
 # once and build their messages only when they refuse.
 
-def _cache(op: str, cache: torch.Tensor, batch: PagedBatch) -> "_lib.PagedCacheC":
+def _cache(op: str, cache: torch.Tensor, batch: PagedBatch):
+    """omg_paged_cache, device, kv_heads and head_dim of a pool for the batch."""
     code = _TYPES.get(cache.dtype, 2)
     if code == 2:
         _fail(f"{op}: cache dtype {cache.dtype} (float16 or bfloat16)")
@@ -150,12 +172,13 @@ def _cache(op: str, cache: torch.Tensor, batch: PagedBatch) -> "_lib.PagedCacheC
     if batch.q_start.get_device() != index:
         _fail(f"{op}: the batch is on {batch.q_start.device}, the cache on {cache.device}")
     pages, page, _, kv_heads, head_dim = cache.shape
-    return _lib.PagedCacheC(cache.data_ptr(), pages, page, kv_heads, head_dim, code)
+    return _pack(op, _CACHE, cache.data_ptr(), pages, page, kv_heads, head_dim,
+                 code), index, kv_heads, head_dim
 
 
 def _vector(op: str, t, name: str, n: int, dtype, index: int):
     if t is None:
-        return None
+        return 0
     if t.dtype is not dtype or t.get_device() != index or t.numel() != n or t.dim() != 1 or (
             not t.is_contiguous()):
         _fail(f"{op}: {name} must be {n} contiguous {dtype} values on cuda:{index}")
@@ -203,8 +226,7 @@ def paged_append(qkv: torch.Tensor, cache: torch.Tensor, batch: PagedBatch, *, h
     go to their cache rows, q times ``q_scale`` is returned
     [tokens, heads, head_dim]."""
     op = "paged_append"
-    c = _cache(op, cache, batch)
-    kvh, hd, index = c.kv_heads, c.head_dim, cache.get_device()
+    c, index, kvh, hd = _cache(op, cache, batch)
     if qkv.get_device() != index or (qkv.dtype is not torch.float32 and
                                      qkv.dtype is not cache.dtype):
         _fail(f"{op}: qkv must be float32 or {cache.dtype} on cuda:{index}")
@@ -215,14 +237,14 @@ def paged_append(qkv: torch.Tensor, cache: torch.Tensor, batch: PagedBatch, *, h
     n, have = qkv.shape
     out = _out(op, out, (n, heads, hd), cache)
     n_freq = 0 if inv_freq is None else inv_freq.numel()
-    args = _lib.AppendArgsC(
-        qkv.data_ptr(), qkv.stride(0) if n > 1 else have, _TYPES[qkv.dtype], n, heads,
+    f32 = torch.float32
+    args = _pack(
+        op, _APPEND, qkv.data_ptr(), qkv.stride(0) if n > 1 else have, _TYPES[qkv.dtype], n, heads,
         have > width, out.data_ptr(), _rows(op, out, "out"),
-        _vector(op, q_norm, "q_norm", hd, torch.float32, index),
-        _vector(op, k_norm, "k_norm", hd, torch.float32, index), v_norm, norm_offset, eps, q_scale,
+        _vector(op, q_norm, "q_norm", hd, f32, index),
+        _vector(op, k_norm, "k_norm", hd, f32, index), v_norm, norm_offset, eps, q_scale,
         _vector(op, inv_freq, "inv_freq", n_freq, torch.float64, index), n_freq)
-    if lib().omg_paged_append(index, C.byref(c), C.byref(batch._c), C.byref(args),
-                              _stream(index)) < 0:
+    if lib().omg_paged_append(index, c, batch._c, args, _stream(index)) < 0:
         check(-1)
     return out
 
@@ -237,30 +259,33 @@ def paged_attention(q: torch.Tensor, cache: torch.Tensor, batch: PagedBatch, *,
     are zero. ``workspace`` (uint8, :func:`paged_attention_workspace` bytes)
     is allocated from torch's pool when not given."""
     op = "paged_attention"
-    c = _cache(op, cache, batch)
-    index = cache.get_device()
-    if q.get_device() != index or q.dtype is not cache.dtype or q.dim() != 3 or (
-            q.size(2) != c.head_dim):
+    c, index, kvh, hd = _cache(op, cache, batch)
+    if q.get_device() != index or q.dtype is not cache.dtype or q.dim() != 3 or q.size(2) != hd:
         _fail(f"{op}: q is {list(q.shape)} {q.dtype} on {q.device}, expected [tokens, heads, "
-              f"{c.head_dim}] {cache.dtype} on cuda:{index}")
+              f"{hd}] {cache.dtype} on cuda:{index}")
     n, heads, _ = shape = q.shape
     out = _out(op, out, shape, q)
     if workspace is None:
-        workspace = cache.new_empty(_workspace(index, c, batch, n, heads), dtype=torch.uint8)
+        workspace = cache.new_empty(_workspace(c, batch, index, n, heads, kvh, hd),
+                                    dtype=torch.uint8)
     elif workspace.get_device() != index or workspace.dtype is not torch.uint8 or (
             not workspace.is_contiguous()):
         _fail(f"{op}: the workspace must be contiguous uint8 on cuda:{index}")
-    args = _lib.AttentionArgsC(q.data_ptr(), _rows(op, q, "q"), out.data_ptr(),
-                               _rows(op, out, "out"), n, heads, window, scale)
-    if lib().omg_paged_attention(index, C.byref(c), C.byref(batch._c), C.byref(args),
-                                 workspace.data_ptr(), workspace.numel(), _stream(index)) < 0:
+    args = _pack(op, _ATTENTION, q.data_ptr(), _rows(op, q, "q"), out.data_ptr(),
+                 _rows(op, out, "out"), n, heads, window, scale)
+    if lib().omg_paged_attention(index, c, batch._c, args, workspace.data_ptr(), workspace.numel(),
+                                 _stream(index)) < 0:
         check(-1)
     return out
 
 
-def _workspace(index: int, c, batch, tokens: int, heads: int) -> int:
-    n = lib().omg_paged_attention_workspace(index, C.byref(c), C.byref(batch._c), tokens, heads)
-    return n if n else check(-1)
+def _workspace(c: bytes, batch: PagedBatch, *shape) -> int:
+    n = batch._workspaces.get(shape)
+    if n is None:
+        index, tokens, heads = shape[:3]
+        n = lib().omg_paged_attention_workspace(index, c, batch._c, tokens, heads) or check(-1)
+        batch._workspaces[shape] = n
+    return n
 
 
 def paged_attention_workspace(cache: torch.Tensor, batch: PagedBatch, tokens: int,
@@ -268,17 +293,17 @@ def paged_attention_workspace(cache: torch.Tensor, batch: PagedBatch, tokens: in
     """Workspace bytes of a :func:`paged_attention` call with ``tokens`` query
     rows. Calls that may overlap (two streams, two captured graphs) need a
     workspace each."""
-    return _workspace(cache.get_device(), _cache("paged_attention_workspace", cache, batch), batch,
-                      tokens, heads)
+    c, index, kvh, hd = _cache("paged_attention_workspace", cache, batch)
+    return _workspace(c, batch, index, tokens, heads, kvh, hd)
 
 
 def _setting(op: str, v, name: str, n: int, dtype, index: int, off):
     """(pointer, value): a tensor of one value per row, or one for all."""
     if v is None:
-        return None, off
+        return 0, off
     if isinstance(v, torch.Tensor):
         return _vector(op, v, name, n, dtype, index), off
-    return None, v
+    return 0, v
 
 
 def sample(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature=None, top_k=None,
@@ -311,11 +336,11 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature=None, to
     k = _setting(op, top_k, "top_k", n, i32, index, 0)
     p = _setting(op, top_p, "top_p", n, f32, index, 1.0)
     m = _setting(op, min_p, "min_p", n, f32, index, 0.0)
-    args = _lib.SampleArgsC(
-        logits.data_ptr(), logits.stride(0) if n > 1 else vocab, code, n, vocab,
+    args = _pack(
+        op, _SAMPLE, logits.data_ptr(), logits.stride(0) if n > 1 else vocab, code, n, vocab,
         _vector(op, uniforms, "uniforms", n, f32, index), temp[0], k[0], p[0], m[0], temp[1], k[1],
         p[1], m[1], _vector(op, tokens, "tokens", n, i32, index),
         _vector(op, probs, "probs", n, f32, index))
-    if lib().omg_sample(index, C.byref(args), _stream(index)) < 0:
+    if lib().omg_sample(index, args, _stream(index)) < 0:
         check(-1)
     return tokens, probs
