@@ -123,11 +123,11 @@ struct PagedAttnArgs {
   float* part_o;        // [2 * ctas][128][hd]
   float2* part_ml;      // [2 * ctas][128]
   int max_tiles;
-  int ctas, min_tiles;  // grid of the attention kernel; least line tiles per CTA
+  int ctas;             // grid of the attention kernel
   bool one_tile;        // a single row tile, which every CTA plans for itself
 };
 
-// Sizes of a call: fills max_tiles, ctas, min_tiles, one_tile of `a` from its
+// Sizes of a call: fills max_tiles, ctas, one_tile of `a` from its
 // batch and shape and returns the workspace bytes (0: more sequences and row
 // tiles than the plan kernel holds).
 size_t paged_attention_layout(PagedAttnArgs* a, int num_sms);

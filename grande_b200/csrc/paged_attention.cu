@@ -205,7 +205,8 @@ __device__ int plan_tile(const PagedAttnArgs& a, const int* q, const int* lens, 
 }
 
 __device__ __forceinline__ int tiles_per_cta(const PagedAttnArgs& a, int line) {
-  return max((line * a.c.kv_heads + a.ctas - 1) / a.ctas, a.min_tiles);
+  // (At least 1, 2, 3, 4: one state with 12 branches 18.8, 20.4, 21.9, 24.1 us.)
+  return max((line * a.c.kv_heads + a.ctas - 1) / a.ctas, 1);
 }
 
 __host__ __device__ inline size_t plan_smem_ints(int64_t seqs, int64_t groups, int64_t max_tiles) {
@@ -1319,7 +1320,6 @@ size_t paged_attention_layout(PagedAttnArgs* a, int num_sms) {
                 std::min(a->b.n_seqs, a->tpt) < one_tile_runs(a->c.hd);
   const int per_sm = a->c.hd <= 128 ? 2 : 1;
   a->ctas = std::max(num_sms * per_sm / (a->c.hd == 512 ? 2 : 1), 1);
-  a->min_tiles = 2;
   const size_t slots = 2 * static_cast<size_t>(a->ctas) * kRows;
   return align_up(sizeof(PagedPlan)) + align_up(a->ctas * sizeof(PagedStart)) +
          align_up(tiles * (a->tpt + 1) * sizeof(PagedRun)) +
