@@ -8,8 +8,12 @@
 // crates/omg-wgpu/src/shaders/qk_prep.wgsl:1-80).
 //
 // Each value is read and written once and costs about ten operations, so HBM
-// bounds it; at a few tokens the chain of dependent loads does (sequence,
-// length, page).
+// bounds it: 12,000 tokens of 8 + 2 x 2 heads of 512 from f32 take 74.7 us,
+// 5.9 TB/s; 16,384 bf16 tokens of 16 + 2 x 4 heads of 128 take 49.5 us, 4.1
+// TB/s. At a few tokens the chain of dependent loads does (sequence, length,
+// page): 3.5 us for one. The heads' values are fetched before that chain, as
+// they lie in memory so that four blocks fit an SM (values widened at the load
+// hold twice the registers: 66 us for those 16,384 tokens).
 //
 // Numerics: everything in f32 and one rounding to the 16-bit outputs, except
 // the angle. position * inv_freq passes 2^17 radians in long contexts, where
@@ -26,20 +30,29 @@ namespace omg {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxTokens = kThreads / 32;  // tokens of a block: a warp each
+constexpr int kMaxTokens = 4;  // tokens of a block, at most
 
+// Eight values as they lie in memory, and as f32.
 template <class T>
-__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0];
-    const float4 b = reinterpret_cast<const float4*>(p)[1];
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  } else {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+struct Raw8 {
+  uint4 w[sizeof(T) / 2];
+};
+template <class T>
+__device__ __forceinline__ Raw8<T> load8(const T* p) {
+  Raw8<T> r;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) r.w[i] = reinterpret_cast<const uint4*>(p)[i];
+  return r;
+}
+template <class T>
+__device__ __forceinline__ void to_f32(const Raw8<T>& r, float (&v)[8]) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(r.w);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      v[2 * i] = __uint_as_float(w[2 * i]);
+      v[2 * i + 1] = __uint_as_float(w[2 * i + 1]);
+    } else {
       float2 f;
       if constexpr (std::is_same<T, __half>::value)
         f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
@@ -72,7 +85,7 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
 // sweeps their heads. A head takes HD / 16 threads, each 8 dims of its lower
 // half and the 8 they are paired with.
 template <int HD, class TI, class TO>
-__global__ void __launch_bounds__(kThreads) paged_append_kernel(PagedAppendArgs a, int tb) {
+__global__ void __launch_bounds__(kThreads, 4) paged_append_kernel(PagedAppendArgs a, int tb) {
   constexpr int L = HD / 16;
   constexpr int kUnits = kThreads / L;
   constexpr int HALF = HD / 2;
@@ -91,16 +104,17 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(PagedAppendArgs 
   griddep_wait();
   griddep_launch();
   // The first heads' values are on their way while the tokens are looked up.
-  float x[8], y[8];
+  Raw8<TI> x{}, y{};
   int u = u_in, tok = u / nh, h = u - tok * nh;
   auto fetch = [&]() {
     if (tok < nt) {
       const TI* row = qkv + tok * a.qkv_stride + h * HD + 8 * l;
-      load8(row, x);
-      load8(row + HALF, y);
+      x = load8(row);
+      y = load8(row + HALF);
     }
   };
   fetch();
+  const double freq0 = tid < nt * a.n_freq ? a.inv_freq[tid % a.n_freq] : 0.0;
   if (warp < nt) {
     const int t = t0 + warp;
     const int s = warp_count_le(a.b.q_start, a.b.n_seqs + 1, t, lane) - 1;
@@ -109,21 +123,20 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(PagedAppendArgs 
     long long crow = -1;
     if (live) {
       const int own = a.b.lens[s] - (a.b.q_start[s + 1] - t);
-      int prefix = 0;
+      // A token without a place (a length below its query rows, a page
+      // outside the table or the pool) leaves the cache as it was.
+      const int pi = own >> a.c.page_log2;
+      int page = -1, prefix = 0;
+      if (own >= 0 && pi < a.b.max_pages)
+        page = a.b.pages[static_cast<int64_t>(s) * a.b.max_pages + pi];
       if (a.b.n_groups > 0) {
         const int g = warp_count_le(a.b.group_start, a.b.n_groups + 1, s, lane) - 1;
         if (g >= 0 && g < a.b.n_groups) prefix = a.b.prefix_lens[g];
       }
       pos = prefix + own;
-      // A token without a place (a length below its query rows, a page
-      // outside the table or the pool) leaves the cache as it was.
-      const int pi = own >> a.c.page_log2;
-      if (own >= 0 && pi < a.b.max_pages) {
-        const int page = a.b.pages[static_cast<int64_t>(s) * a.b.max_pages + pi];
-        if (page >= 0 && page < a.c.n_pages)
-          crow = (static_cast<long long>(page) << a.c.page_log2) +
-                 (own & ((1 << a.c.page_log2) - 1));
-      }
+      if (page >= 0 && page < a.c.n_pages)
+        crow = (static_cast<long long>(page) << a.c.page_log2) +
+               (own & ((1 << a.c.page_log2) - 1));
     }
     if (lane == 0) {
       s_row[warp] = crow;
@@ -134,7 +147,7 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(PagedAppendArgs 
   __syncthreads();
   for (int i = tid; i < nt * a.n_freq; i += kThreads) {
     const int k = i / a.n_freq, d = i - k * a.n_freq;
-    const double turns = static_cast<double>(s_pos[k]) * (a.inv_freq[d] * 0.15915494309189535);
+    const double turns = static_cast<double>(s_pos[k]) * ((i == tid ? freq0 : a.inv_freq[d]) * 0.15915494309189535);
     float sn, cs;
     sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &sn, &cs);
     rot[k][d] = make_float2(cs, sn);
@@ -147,12 +160,10 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(PagedAppendArgs 
     const float* w = is_q ? a.q_norm : is_v ? nullptr : a.k_norm;
     float v[8], z[8];
     float ss = 0.f;
+    to_f32(x, v);
+    to_f32(y, z);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      v[e] = x[e];
-      z[e] = y[e];
-      ss += v[e] * v[e] + z[e] * z[e];
-    }
+    for (int e = 0; e < 8; ++e) ss += v[e] * v[e] + z[e] * z[e];
     // The next heads' values.
     u += kUnits;
     tok = u / nh;
@@ -172,8 +183,8 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(PagedAppendArgs 
     if (!is_v) {
       if (w) {
         float wv[8], wz[8];
-        load8(w + 8 * l, wv);
-        load8(w + HALF + 8 * l, wz);
+        to_f32(load8(w + 8 * l), wv);
+        to_f32(load8(w + HALF + 8 * l), wz);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           v[e] *= a.norm_offset + wv[e];
@@ -209,9 +220,12 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(PagedAppendArgs 
 
 template <int HD, class TI, class TO>
 void launch(const PagedAppendArgs& a, int num_sms, cudaStream_t s) {
-  // A token per block while that does not fill the GPU (5 blocks fit an SM),
-  // then 8: the lookups and the barriers are paid once for all of them.
-  const int tb = a.b.tokens <= num_sms * 5 ? 1 : kMaxTokens;
+  // Tokens per block: the lookups and barriers are paid once for all of them,
+  // but few blocks leave SMs idle. us with 1, 2, 4, 8 tokens, 8 + 2 x 2 heads
+  // of 512 from f32: 60 tokens 4.4, 5.2, 7.4, 11.9; 720 tokens 10.5, 9.3, 9.8,
+  // 12.3; 12,000 tokens 92, 80, 75, 76. 16 + 2 x 4 bf16 heads of 128: 1,024
+  // tokens 7.8, 6.6, 6.4, 7.6; 16,384 tokens 76, 62, 50, 47.
+  const int tb = a.b.tokens <= num_sms ? 1 : a.b.tokens <= 5 * num_sms ? 2 : kMaxTokens;
   launch_pdl(paged_append_kernel<HD, TI, TO>, dim3((a.b.tokens + tb - 1) / tb), dim3(kThreads), 0, s,
              a, tb);
 }
