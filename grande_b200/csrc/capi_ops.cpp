@@ -118,10 +118,10 @@ PagedAttnArgs attention_shape(const char* op, int device, const omg_paged_cache*
   if (heads < 1 || heads % a.c.kv_heads || heads / a.c.kv_heads > kPagedTileRows)
     fail("%s: %d query heads over %d KV heads", op, heads, a.c.kv_heads);
   a.heads = heads;
-  *bytes = paged_attention_layout(&a, device_info(device).sms);
-  if (!*bytes)
+  if (!paged_attention_shape(&a))
     fail("%s: %d query rows of %d sequences in one call (split the batch)", op, tokens,
          batch->n_seqs);
+  *bytes = paged_attention_layout(&a, device_info(device).sms);
   return a;
 }
 

@@ -96,14 +96,15 @@ struct alignas(16) PagedTile {
 
 struct alignas(16) PagedPlan {
   int n_tiles;    // row tiles
-  int line;       // key tiles of one KV head
-  int per;        // key tiles per CTA
+  int line;       // units of one KV head
+  int per;        // units per CTA
   int pad;
 };
 
-// Where a CTA's range of the line begins: tile `pos` of row tile `rt`.
+// Where a CTA's range of the line begins: tile `pos` of row tile `rt`, after
+// `toll` more units of its toll.
 struct alignas(16) PagedStart {
-  int rt, pos, kv, pad;
+  int rt, pos, kv, toll;
 };
 
 struct PagedAttnArgs {
@@ -127,9 +128,11 @@ struct PagedAttnArgs {
   bool one_tile;        // a single row tile, which every CTA plans for itself
 };
 
-// Sizes of a call: fills max_tiles, ctas, one_tile of `a` from its
-// batch and shape and returns the workspace bytes (0: more sequences and row
-// tiles than the plan kernel holds).
+// Row tiles of a call: fills hpg, tpt, max_tiles, one_tile of `a` from its batch
+// and shape. False: more sequences and row tiles than the plan kernel holds, or
+// a line of more than 2^29 key tiles.
+bool paged_attention_shape(PagedAttnArgs* a);
+// Then its grid, `ctas`; returns the workspace bytes.
 size_t paged_attention_layout(PagedAttnArgs* a, int num_sms);
 // Point the workspace members of `a` into `ws`.
 void paged_attention_workspace(PagedAttnArgs* a, void* ws);

@@ -2,9 +2,9 @@
 // prefix (see paged.cuh): out = softmax(scale q K^T) V over the prefix keys
 // and the sequence's own keys up to the query's position, inside the window.
 //
-// Three launches. The plan kernel (one CTA) cuts the query tokens into row
-// tiles and lays their key tiles on one line (paged.cuh). The attention
-// kernel gives every CTA an equal range of the line, whatever it crosses; a
+// Three launches, two for a single row tile, which the attention kernel plans
+// itself. The plan kernel (one CTA) cuts the query tokens into row tiles and
+// lays their key tiles on one line (paged.cuh). The attention kernel gives every CTA an equal range of the line, whatever it crosses; a
 // row tile inside one CTA's range is finished there, one that several CTAs
 // cross leaves per CTA an unnormalised O and each row's (max, sum), which the
 // merge kernel joins.
@@ -18,8 +18,19 @@
 // by infinities or NaN among another sequence's values.
 //
 // Roles (192 threads): warp 0 loads Q and the K / V ring through TMA, a box
-// per page; warp 1 issues S = Q K^T one tile ahead and O += P V; warps 2-5
+// per 16-key slot and 64 dims (boxes of whole pages took the same time within
+// 2%, and a slot never straddles a page); warp 1 issues S = Q K^T one tile ahead and O += P V; warps 2-5
 // own one query row per thread: mask, online softmax, P, the rescale of O.
+//
+// What bounds it. Prefixes of few rows: HBM; a 64-key tile of head_dim 256
+// (64 KB) takes an SM 3,100 clocks, 90% of the copy rate, but slots hold more
+// keys than a short branch has, and two partial O per CTA go out and back: 64
+// states of up to 2,000 + 20 branches x 31 keys take 90 us, 2.8 TB/s. Long
+// sequences of a few rows each: 123 us for 64 of up to 8,192 keys, 4.4 TB/s.
+// Prompts: the softmax warps, 780 TFLOP/s at head_dim 128 over 8,000 keys and
+// more, 620 for a prompt of 8,192 tokens alone. One state's next token:
+// latency; 13 to 20 us are two launches, the tables' chain of loads, a key tile
+// per CTA and the merge.
 //
 // Numerics: scores, max, exponentials and sums f32, O accumulated in f32; P
 // enters the second product in the cache's 16-bit type (its rounding is of
@@ -48,8 +59,14 @@ constexpr int kKvChunk = kKeys * 128;  // [64 keys][64 dims]
 constexpr int kPBytes = kRows * kKeys * 2;
 constexpr float kTau = 8.0f;           // slack of the reference max, in log2 units x ln 2
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kPlanThreads = 1024;
+constexpr int kPlanThreads = 1024;  // 32 warps (block_scan)
 constexpr int kThreads = 192;
+// What a row tile costs on the line beside its key tiles, in key tiles: its Q,
+// the first tile's latency, the epilogue. Without it the CTA that the first,
+// short row tiles of a prompt fall to holds up the rest. (us with 0, 2, 3, 4, 8:
+// a prompt of 4,096 tokens, 8 heads of 128: 121, 98, 89, 86, 90; of 512: 378,
+// 333, 333, 339, 351; 64 states' next tokens: 89.4, 88.7, 89.5, 90.5, 94.9.)
+constexpr int kToll = 3;
 // Runs (the prefix's included) that a CTA plans for itself in shared memory.
 constexpr int one_tile_runs(int hd) { return hd == 128 ? 21 : 33; }
 
@@ -60,7 +77,13 @@ struct Shape {
   static constexpr int kChunks = kV / 64;           // 64-dim chunks of a ring stage
   static constexpr int kStage = kChunks * kKvChunk; // 64 keys x kV dims
   static constexpr int kQ = HD / 64 * kQChunk;
-  static constexpr int kPSlots = HD == 128 ? 1 : 2;  // one: a ring of two whole tiles instead
+  // Two CTAs of an SM hide each other's waits where both fit; at head_dim 128
+  // one P slot each leaves room for rings of two whole tiles. (64 sequences of
+  // up to 8,192 keys, head_dim 128: one CTA with 8 stages and 2 P slots 148 us,
+  // two with 3 stages and 2 P slots 146, two with 4 stages and 1 P slot 118. At
+  // head_dim 512 five stages of half the size and one P slot: 51 -> 57 us for
+  // 288 tokens over 2,000 keys.)
+  static constexpr int kPSlots = HD == 128 ? 1 : 2;
   static constexpr int kCtasPerSm = HD <= 128 ? 2 : 1;
   static constexpr int kStages = HD == 512 ? 2 : HD == 64 ? 6 : 4;
   static constexpr int kTmemO = 128;                // S buffers at columns 0 and 64
@@ -71,31 +94,28 @@ struct Shape {
 
 // ---- plan -------------------------------------------------------------------
 
-// Exclusive scan of v over a block of THREADS; returns its total. (Scratch of
-// 64 ints, 8-byte aligned: static shared memory would cost the second CTA of
-// an SM.)
-template <int THREADS, class N>
-__device__ __forceinline__ N block_scan(N v, N* excl, int* scratch) {
-  N* ws = reinterpret_cast<N*>(scratch);
+// Exclusive scan of v over the plan's block; returns its total. `ws`: 32 ints
+// of shared memory.
+__device__ __forceinline__ int block_scan(int v, int* excl, int* ws) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  N x = v;
+  int x = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const N y = __shfl_up_sync(0xffffffffu, x, o);
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
     if (lane >= o) x += y;
   }
   if (lane == 31) ws[warp] = x;
   __syncthreads();
   // Every warp scans the warps' sums for itself.
-  N w = lane < THREADS / 32 ? ws[lane] : 0;
+  int w = ws[lane];
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const N y = __shfl_up_sync(0xffffffffu, w, o);
+    const int y = __shfl_up_sync(0xffffffffu, w, o);
     if (lane >= o) w += y;
   }
-  const N before = __shfl_sync(0xffffffffu, w, max(warp - 1, 0));
+  const int before = __shfl_sync(0xffffffffu, w, max(warp - 1, 0));
   *excl = x - v + (warp ? before : 0);
-  const N total = __shfl_sync(0xffffffffu, w, 31);
+  const int total = __shfl_sync(0xffffffffu, w, 31);
   __syncthreads();
   return total;
 }
@@ -204,13 +224,20 @@ __device__ int plan_tile(const PagedAttnArgs& a, const int* q, const int* lens, 
   return ntiles;
 }
 
+// The place on the line that unit `w` of one KV head's `line` units is, in row
+// tile `rt` that begins at unit `at` of it: the toll comes before the tiles.
+__device__ __forceinline__ PagedStart place(int kv, int rt, int at, int w) {
+  const int pos = w - at - kToll;
+  return PagedStart{rt, max(pos, 0), kv, max(-pos, 0)};
+}
+
 __device__ __forceinline__ int tiles_per_cta(const PagedAttnArgs& a, int line) {
   // (At least 1, 2, 3, 4: one state with 12 branches 18.8, 20.4, 21.9, 24.1 us.)
   return max((line * a.c.kv_heads + a.ctas - 1) / a.ctas, 1);
 }
 
 __host__ __device__ inline size_t plan_smem_ints(int64_t seqs, int64_t groups, int64_t max_tiles) {
-  return 64 + 2 * (seqs + 1) + 4 * (groups + 1) + max_tiles + 1;
+  return 32 + 2 * (seqs + 1) + 4 * (groups + 1) + max_tiles + 1;
 }
 
 // One block: groups to row tiles, a warp per row tile, and the CTAs' places on
@@ -218,7 +245,7 @@ __host__ __device__ inline size_t plan_smem_ints(int64_t seqs, int64_t groups, i
 __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedAttnArgs a) {
   extern __shared__ __align__(16) int sm[];
   const int groups = max(a.b.n_groups, 1), S = a.b.n_seqs, T = a.b.tokens;
-  int* q = sm + 64;            // [S + 1]
+  int* q = sm + 32;            // [S + 1]
   int* len = q + S + 1;        // [S + 1]
   int* gs = len + S + 1;       // [groups + 1] first sequence, token, row tile; prefix length
   int* gtok = gs + groups + 1;
@@ -248,7 +275,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedAttnArgs 
       n = (max(t1 - t0, 0) + a.tpt - 1) / a.tpt;
     }
     int at;
-    const int total = block_scan<kPlanThreads>(n, &at, sm);
+    const int total = block_scan(n, &at, sm);
     if (g < groups) gtile[g] = n_tiles + at;
     n_tiles += total;
   }
@@ -262,14 +289,14 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedAttnArgs 
     const int s = max(gs[g], warp_count_le(q + gs[g], gs[g + 1] - gs[g], t0, lane) - 1 + gs[g]);
     const int n = plan_tile(a, q, len, rt, g, plen[g], t0, t1, s, gs[g + 1],
                             a.runs + static_cast<int64_t>(rt) * (a.tpt + 1), a.tiles + rt);
-    if (lane == 0) cum[rt] = n;
+    if (lane == 0) cum[rt] = n + kToll;
   }
   __syncthreads();
   int line = 0;
   for (int rt0 = 0; rt0 < n_tiles; rt0 += kPlanThreads) {
     const int rt = rt0 + tid;
     int at;
-    const int total = block_scan<kPlanThreads>(rt < n_tiles ? cum[rt] : 0, &at, sm);
+    const int total = block_scan(rt < n_tiles ? cum[rt] : 0, &at, sm);
     if (rt < n_tiles) cum[rt] = line + at;
     line += total;
   }
@@ -279,10 +306,8 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(PagedAttnArgs 
     const int w = i * per;
     PagedStart st{0, 0, 0, 0};
     if (w < line * a.c.kv_heads) {
-      st.kv = w / line;
-      const int wl = w - st.kv * line;
-      st.rt = last_le(cum, n_tiles, wl);
-      st.pos = wl - cum[st.rt];
+      const int kv = w / line, wl = w - kv * line, rt = last_le(cum, n_tiles, wl);
+      st = place(kv, rt, cum[rt], wl);
     }
     a.starts[i] = st;
   }
@@ -473,21 +498,20 @@ __global__ void __launch_bounds__(kThreads, Shape<HD>::kCtasPerSm)
       const int t0 = min(max(a.b.q_start[s0], 0), a.b.tokens);
       const int t1 = min(max(a.b.q_start[s1], t0), a.b.tokens);
       if (t1 > t0) plan_tile(a, a.b.q_start, a.b.lens, 0, 0, plen, t0, t1, s0, s1, my_runs, my_tile);
-      if (t1 == t0 && lane == 0) my_tile->ntiles = 0;
+      if (t1 == t0 && lane == 0) my_tile->ntiles = -kToll;  // an empty line
       if (blockIdx.x == 0 && blockIdx.y == 0 && lane == 0) {
-        *a.plan = PagedPlan{1, my_tile->ntiles, tiles_per_cta(a, my_tile->ntiles), 0};
+        const int line = my_tile->ntiles + kToll;
+        *a.plan = PagedPlan{1, line, tiles_per_cta(a, line), 0};
         *a.tiles = *my_tile;
       }
     }
     __syncthreads();
     runs = my_runs;
     tiles = my_tile;
-    const int line = my_tile->ntiles;
+    const int line = my_tile->ntiles + kToll;
     plan = PagedPlan{1, line, tiles_per_cta(a, line), 0};
-    const int w = blockIdx.x * plan.per;
-    start.kv = line ? w / line : 0;
-    start.rt = 0;
-    start.pos = line ? w - start.kv * line : 0;
+    const int w = blockIdx.x * plan.per, kv = line ? w / line : 0;
+    start = place(kv, 0, 0, w - kv * line);
   } else {
     plan = *a.plan;
     start = a.starts[blockIdx.x];
@@ -558,7 +582,7 @@ __global__ void __launch_bounds__(kThreads, Shape<HD>::kCtasPerSm)
     u.rt = start.rt;
     u.pos = start.pos;
     u.kv = start.kv;
-    for (int w = w0; w < w1 && ok; u.leave(plan.n_tiles)) {
+    for (int w = w0 + start.toll; w < w1 && ok; u.leave(plan.n_tiles), w += kToll) {
       u.load(tiles, runs, run_cap, w1 - w, lane);
       const int n = u.end - u.pos;
       const int kx = u.kv * HD, vx = (a.c.kv_heads + u.kv) * HD + vhalf * VD;
@@ -667,7 +691,7 @@ __global__ void __launch_bounds__(kThreads, Shape<HD>::kCtasPerSm)
     u.rt = start.rt;
     u.pos = start.pos;
     u.kv = start.kv;
-    for (int w = w0; w < w1 && ok; u.leave(plan.n_tiles)) {
+    for (int w = w0 + start.toll; w < w1 && ok; u.leave(plan.n_tiles), w += kToll) {
       u.load(tiles, runs, run_cap, w1 - w, lane);
       const int n = u.end - u.pos;
       if (!warp_wait(&bars[B_Q], qphase, abort_flag)) {
@@ -754,11 +778,12 @@ __global__ void __launch_bounds__(kThreads, Shape<HD>::kCtasPerSm)
     u.rt = start.rt;
     u.pos = start.pos;
     u.kv = start.kv;
-    for (int w = w0; w < w1; u.leave(plan.n_tiles)) {
+    bool first = true;
+    for (int w = w0 + start.toll; w < w1; u.leave(plan.n_tiles), w += kToll) {
       u.load(tiles, runs, run_cap, w1 - w, lane);
       const PagedTile tile = u.tile;
       const int kv = u.kv, n = u.end - u.pos;
-      const bool first = w == w0, whole = n == tile.ntiles;
+      const bool whole = n == tile.ntiles;
       const int nrows = tile.ntok * a.hpg;
       const bool valid = r < nrows;
       // The row's own index, from its sequence's run: a lane per run, and a
@@ -899,143 +924,143 @@ __global__ void __launch_bounds__(kThreads, Shape<HD>::kCtasPerSm)
           }
         }
         const bool my_warp = __any_sync(0xffffffffu, mine);
-          uint8_t* pj = ps + (b & (Sh::kPSlots - 1)) * kPBytes;
-          if (my_warp) {
-            tc_fence_after();
-            float s[kKeys];
-            {
-              uint32_t raw0[32], raw1[32];
-              tmem_ld32_nowait(trow + b * kKeys, raw0);
-              tmem_ld32_nowait(trow + b * kKeys + 32, raw1);
-              tmem_ld_wait();
+        uint8_t* pj = ps + (b & (Sh::kPSlots - 1)) * kPBytes;
+        if (my_warp) {
+          tc_fence_after();
+          float s[kKeys];
+          {
+            uint32_t raw0[32], raw1[32];
+            tmem_ld32_nowait(trow + b * kKeys, raw0);
+            tmem_ld32_nowait(trow + b * kKeys + 32, raw1);
+            tmem_ld_wait();
 #pragma unroll
-              for (int c = 0; c < 32; ++c) {
-                s[c] = __uint_as_float(raw0[c]);
-                s[32 + c] = __uint_as_float(raw1[c]);
-              }
+            for (int c = 0; c < 32; ++c) {
+              s[c] = __uint_as_float(raw0[c]);
+              s[32 + c] = __uint_as_float(raw1[c]);
             }
-            // Rows without a slot here see nothing: their lanes are off in the
-            // product, so only their (max, sum) must not move and their
-            // scores need no mask.
-            if (__any_sync(0xffffffffu, vis != ~0ull && mine)) {
-              const uint32_t vlo = static_cast<uint32_t>(vis), vhi = static_cast<uint32_t>(vis >> 32);
-#pragma unroll
-              for (int c = 0; c < kKeys; ++c) {
-                const uint32_t m = c < 32 ? vlo : vhi;
-                s[c] = ((m >> (c & 31)) & 1u) ? s[c] : -INFINITY;
-              }
-            }
-            float mx[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) mx[e] = s[e];
-#pragma unroll
-            for (int c = 8; c < kKeys; ++c) mx[c & 7] = fmaxf(mx[c & 7], s[c]);
-            const float mt = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])),
-                                   fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7]))) *
-                             a.scale_log2;
-            float alpha = 1.f;
-            bool rescale = false;
-            if (mine && mt > m_ref + kTau * kLog2e) {
-              rescale = m_ref != -INFINITY;
-              alpha = rescale ? exp2_fast(m_ref - mt) : 0.f;
-              m_ref = mt;
-            }
-            // A row that has seen nothing yet has no reference: its scores are
-            // all -infinity, or NaN, which counts (fmaxf drops it).
-            const float ref = m_ref == -INFINITY ? 0.f : m_ref;
-            float psum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+          }
+          // Rows without a slot here see nothing: their lanes are off in the
+          // product, so only their (max, sum) must not move and their
+          // scores need no mask.
+          if (__any_sync(0xffffffffu, vis != ~0ull && mine)) {
+            const uint32_t vlo = static_cast<uint32_t>(vis), vhi = static_cast<uint32_t>(vis >> 32);
 #pragma unroll
             for (int c = 0; c < kKeys; ++c) {
-              s[c] = exp2_fast(fmaf(s[c], a.scale_log2, -ref));
-              psum[c & 7] += s[c];
+              const uint32_t m = c < 32 ? vlo : vhi;
+              s[c] = ((m >> (c & 31)) & 1u) ? s[c] : -INFINITY;
             }
-            const float sum = ((psum[0] + psum[1]) + (psum[2] + psum[3])) +
-                              ((psum[4] + psum[5]) + (psum[6] + psum[7]));
-            if (mine) l = l * alpha + sum;
-            const bool any_rescale = __any_sync(0xffffffffu, rescale);
-            // Rescaling O needs the P V before this one done; slot b was read
-            // by the one before that.
-            if (done > 0 && (any_rescale || Sh::kPSlots == 1)) {
-              if (!warp_wait(&bars[B_O0 + ((g - 1) & 1)], ((g - 1) >> 1) & 1, abort_flag)) {
-                ok = false;
-                break;
-              }
+          }
+          float mx[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) mx[e] = s[e];
+#pragma unroll
+          for (int c = 8; c < kKeys; ++c) mx[c & 7] = fmaxf(mx[c & 7], s[c]);
+          const float mt = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])),
+                                 fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7]))) *
+                           a.scale_log2;
+          float alpha = 1.f;
+          bool rescale = false;
+          if (mine && mt > m_ref + kTau * kLog2e) {
+            rescale = m_ref != -INFINITY;
+            alpha = rescale ? exp2_fast(m_ref - mt) : 0.f;
+            m_ref = mt;
+          }
+          // A row that has seen nothing yet has no reference: its scores are
+          // all -infinity, or NaN, which counts (fmaxf drops it).
+          const float ref = m_ref == -INFINITY ? 0.f : m_ref;
+          float psum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < kKeys; ++c) {
+            s[c] = exp2_fast(fmaf(s[c], a.scale_log2, -ref));
+            psum[c & 7] += s[c];
+          }
+          const float sum = ((psum[0] + psum[1]) + (psum[2] + psum[3])) +
+                            ((psum[4] + psum[5]) + (psum[6] + psum[7]));
+          if (mine) l = l * alpha + sum;
+          const bool any_rescale = __any_sync(0xffffffffu, rescale);
+          // Rescaling O needs the P V before this one done; slot b was read
+          // by the one before that.
+          if (done > 0 && (any_rescale || Sh::kPSlots == 1)) {
+            if (!warp_wait(&bars[B_O0 + ((g - 1) & 1)], ((g - 1) >> 1) & 1, abort_flag)) {
+              ok = false;
+              break;
             }
-            if (Sh::kPSlots == 2 && done > 1) {
-              if (!warp_wait(&bars[B_O0 + b], ((g - 2) >> 1) & 1, abort_flag)) {
-                ok = false;
-                break;
-              }
+          }
+          if (Sh::kPSlots == 2 && done > 1) {
+            if (!warp_wait(&bars[B_O0 + b], ((g - 2) >> 1) & 1, abort_flag)) {
+              ok = false;
+              break;
             }
-            if (any_rescale) {
-              tc_fence_after();
-              const float f = rescale ? alpha : 1.0f;
+          }
+          if (any_rescale) {
+            tc_fence_after();
+            const float f = rescale ? alpha : 1.0f;
+#pragma unroll 1
+            for (int c = 0; c < VD / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld32_nowait(trow + Sh::kTmemO + c * 32, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_st32(trow + Sh::kTmemO + c * 32, o);
+            }
+            tmem_st_wait();
+          }
+#pragma unroll
+          for (int pw = 0; pw < kKeys / 8; ++pw) {
+            uint32_t h[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) h[e] = pack2<T>(s[pw * 8 + 2 * e], s[pw * 8 + 2 * e + 1]);
+            *reinterpret_cast<uint4*>(pj + r * 128 + ((pw ^ (r & 7)) << 4)) =
+                make_uint4(h[0], h[1], h[2], h[3]);
+          }
+        }
+        if (my_warp || edge) fence_proxy_async();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars[B_P0 + b]);
+        if (bad) {
+          // The taken-out keys, for the rows that see them.
+          if (!warp_wait(&bars[B_O0 + b], (g >> 1) & 1, abort_flag)) {
+            ok = false;
+            break;
+          }
+          if (__any_sync(0xffffffffu, (vis & bad) != 0)) {
+            tc_fence_after();
+            for (uint64_t todo = bad; todo; todo &= todo - 1) {
+              const int key = __ffsll(static_cast<long long>(todo)) - 1;
+              // (All lanes take part: `todo` is the same in all of them.)
+              const int from = __shfl_sync(0xffffffffu, owner, key / kSlot);
+              const int at = __shfl_sync(0xffffffffu, key0, key / kSlot) + key % kSlot;
+              const int pi = at >> a.c.page_log2;
+              int page = from < 0 ? a.b.prefix_pages[static_cast<int64_t>(~from) *
+                                                         a.b.max_prefix_pages + pi]
+                                  : a.b.pages[static_cast<int64_t>(from) * a.b.max_pages + pi];
+              const int64_t row = (static_cast<int64_t>(page) << a.c.page_log2) +
+                                  (at & ((1 << a.c.page_log2) - 1));
+              const uint16_t* vrow = static_cast<const uint16_t*>(a.c.rows) +
+                                     (row * 2 * a.c.kv_heads + a.c.kv_heads + kv) * HD +
+                                     vhalf * VD;
+              const bool add = (vis >> key) & 1;
+              const float p = to_float<T>(*reinterpret_cast<const uint16_t*>(
+                  pj + r * 128 + (((key >> 3) ^ (r & 7)) << 4) + (key & 7) * 2));
 #pragma unroll 1
               for (int c = 0; c < VD / 32; ++c) {
                 uint32_t o[32];
                 tmem_ld32_nowait(trow + Sh::kTmemO + c * 32, o);
                 tmem_ld_wait();
 #pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                for (int e = 0; e < 32; ++e)
+                  if (add)
+                    o[e] = __float_as_uint(
+                        fmaf(p, to_float<T>(vrow[c * 32 + e]), __uint_as_float(o[e])));
                 tmem_st32(trow + Sh::kTmemO + c * 32, o);
               }
               tmem_st_wait();
             }
-#pragma unroll
-            for (int pw = 0; pw < kKeys / 8; ++pw) {
-              uint32_t h[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) h[e] = pack2<T>(s[pw * 8 + 2 * e], s[pw * 8 + 2 * e + 1]);
-              *reinterpret_cast<uint4*>(pj + r * 128 + ((pw ^ (r & 7)) << 4)) =
-                  make_uint4(h[0], h[1], h[2], h[3]);
-            }
+            tc_fence_before();
           }
-          if (my_warp || edge) fence_proxy_async();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bars[B_P0 + b]);
-          if (bad) {
-            // The taken-out keys, for the rows that see them.
-            if (!warp_wait(&bars[B_O0 + b], (g >> 1) & 1, abort_flag)) {
-              ok = false;
-              break;
-            }
-            if (__any_sync(0xffffffffu, (vis & bad) != 0)) {
-              tc_fence_after();
-              for (uint64_t todo = bad; todo; todo &= todo - 1) {
-                const int key = __ffsll(static_cast<long long>(todo)) - 1;
-                // (All lanes take part: `todo` is the same in all of them.)
-                const int from = __shfl_sync(0xffffffffu, owner, key / kSlot);
-                const int at = __shfl_sync(0xffffffffu, key0, key / kSlot) + key % kSlot;
-                const int pi = at >> a.c.page_log2;
-                int page = from < 0 ? a.b.prefix_pages[static_cast<int64_t>(~from) *
-                                                           a.b.max_prefix_pages + pi]
-                                    : a.b.pages[static_cast<int64_t>(from) * a.b.max_pages + pi];
-                const int64_t row = (static_cast<int64_t>(page) << a.c.page_log2) +
-                                    (at & ((1 << a.c.page_log2) - 1));
-                const uint16_t* vrow = static_cast<const uint16_t*>(a.c.rows) +
-                                       (row * 2 * a.c.kv_heads + a.c.kv_heads + kv) * HD +
-                                       vhalf * VD;
-                const bool add = (vis >> key) & 1;
-                const float p = to_float<T>(*reinterpret_cast<const uint16_t*>(
-                    pj + r * 128 + (((key >> 3) ^ (r & 7)) << 4) + (key & 7) * 2));
-#pragma unroll 1
-                for (int c = 0; c < VD / 32; ++c) {
-                  uint32_t o[32];
-                  tmem_ld32_nowait(trow + Sh::kTmemO + c * 32, o);
-                  tmem_ld_wait();
-#pragma unroll
-                  for (int e = 0; e < 32; ++e)
-                    if (add)
-                      o[e] = __float_as_uint(
-                          fmaf(p, to_float<T>(vrow[c * 32 + e]), __uint_as_float(o[e])));
-                  tmem_st32(trow + Sh::kTmemO + c * 32, o);
-                }
-                tmem_st_wait();
-              }
-              tc_fence_before();
-            }
-          }
+        }
         ++g;
         vslot = ring_add<NST>(vslot, 2);
         vr.next();
@@ -1139,6 +1164,7 @@ __global__ void __launch_bounds__(kThreads, Shape<HD>::kCtasPerSm)
         __syncwarp();
       }
       tc_fence_before();
+      first = false;
       w += n;
     }
   }
@@ -1179,10 +1205,8 @@ __global__ void __launch_bounds__(32 * kMergeWarps) paged_merge_kernel(PagedAttn
   auto read = [&]() {
     plan = *a.plan;
     if (a.one_tile) {
-      const int w = i * plan.per;
-      st.rt = 0;
-      st.kv = plan.line ? w / plan.line : 0;
-      st.pos = w - st.kv * plan.line;
+      const int w = i * plan.per, kv = plan.line ? w / plan.line : 0;
+      st = place(kv, 0, 0, w - kv * plan.line);
     } else {
       st = a.starts[i];
     }
@@ -1196,76 +1220,76 @@ __global__ void __launch_bounds__(32 * kMergeWarps) paged_merge_kernel(PagedAttn
   if (a.one_tile) read();
   const int per = plan.per, w = i * per;
   if (w >= plan.line * a.c.kv_heads) return;
-  const int kv = st.kv, e0 = w - st.pos;
-  if (e0 == w || (i - 1) * per > e0) return;
+  const int kv = st.kv, e0 = w - st.pos;  // the row tile's first key tile
+  if (st.pos == 0 || (i - 1) * per > e0) return;
   const int c0 = i - 1, c1 = (e0 + t.ntiles - 1) / per;
   const int d0 = (warp % kRowWarps) * kPer + lane * kLane;
   const int nrows = t.ntok * a.hpg;
   for (int r = blockIdx.y + gridDim.y * (warp / kRowWarps); r < nrows;
        r += gridDim.y * kRowsHere) {
-  auto slot_row = [&](int c) {
-    return (2 * static_cast<size_t>(c) + (c * per >= e0 ? 0 : 1)) * kRows + r;
-  };
-  float mmax = -INFINITY;
-  for (int c = c0 + lane; c <= c1; c += 32) mmax = fmaxf(mmax, a.part_ml[slot_row(c)].x);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mmax = fmaxf(mmax, __shfl_xor_sync(0xffffffffu, mmax, o));
-  float acc[kLane], lsum = 0.f;
-#pragma unroll
-  for (int e = 0; e < kLane; ++e) acc[e] = 0.f;
-  for (int cb = c0; cb <= c1; cb += 32) {
-    const int c = cb + lane;
-    float2 ml = make_float2(-INFINITY, 0.f);
-    if (c <= c1) ml = a.part_ml[slot_row(c)];
-    // A range the row saw nothing of wrote no O. One whose scores were all
-    // NaN has no max but a sum.
-    const bool live = ml.y != 0.f;
-    const float wt = ml.x == mmax || ml.x == -INFINITY ? 1.0f : exp2_fast(ml.x - mmax);
-    uint32_t todo = __ballot_sync(0xffffffffu, live);
-    while (todo) {
-      // Several ranges' loads in flight.
-      float v[kMany][kLane], wv[kMany], lv[kMany];
-      int n = 0;
-#pragma unroll
-      for (int k = 0; k < kMany; ++k) {
-        const int src = todo ? __ffs(todo) - 1 : 0;
-        const bool on = todo != 0;
-        if (on) ++n;
-        todo &= todo - 1;
-        wv[k] = __shfl_sync(0xffffffffu, wt, src);
-        lv[k] = __shfl_sync(0xffffffffu, ml.y, src);
-        const float* p = a.part_o + slot_row(cb + src) * HD + d0;
-        if (on) {
-          if constexpr (kLane == 4) {
-            const float4 f = *reinterpret_cast<const float4*>(p);
-            v[k][0] = f.x; v[k][1] = f.y; v[k][2] = f.z; v[k][3] = f.w;
-          } else {
-            const float2 f = *reinterpret_cast<const float2*>(p);
-            v[k][0] = f.x; v[k][1] = f.y;
+    auto slot_row = [&](int c) {
+      return (2 * static_cast<size_t>(c) + (c * per >= e0 - kToll ? 0 : 1)) * kRows + r;
+    };
+    float mmax = -INFINITY;
+    for (int c = c0 + lane; c <= c1; c += 32) mmax = fmaxf(mmax, a.part_ml[slot_row(c)].x);
+  #pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mmax = fmaxf(mmax, __shfl_xor_sync(0xffffffffu, mmax, o));
+    float acc[kLane], lsum = 0.f;
+  #pragma unroll
+    for (int e = 0; e < kLane; ++e) acc[e] = 0.f;
+    for (int cb = c0; cb <= c1; cb += 32) {
+      const int c = cb + lane;
+      float2 ml = make_float2(-INFINITY, 0.f);
+      if (c <= c1) ml = a.part_ml[slot_row(c)];
+      // A range the row saw nothing of wrote no O. One whose scores were all
+      // NaN has no max but a sum.
+      const bool live = ml.y != 0.f;
+      const float wt = ml.x == mmax || ml.x == -INFINITY ? 1.0f : exp2_fast(ml.x - mmax);
+      uint32_t todo = __ballot_sync(0xffffffffu, live);
+      while (todo) {
+        // Several ranges' loads in flight.
+        float v[kMany][kLane], wv[kMany], lv[kMany];
+        int n = 0;
+  #pragma unroll
+        for (int k = 0; k < kMany; ++k) {
+          const int src = todo ? __ffs(todo) - 1 : 0;
+          const bool on = todo != 0;
+          if (on) ++n;
+          todo &= todo - 1;
+          wv[k] = __shfl_sync(0xffffffffu, wt, src);
+          lv[k] = __shfl_sync(0xffffffffu, ml.y, src);
+          const float* p = a.part_o + slot_row(cb + src) * HD + d0;
+          if (on) {
+            if constexpr (kLane == 4) {
+              const float4 f = *reinterpret_cast<const float4*>(p);
+              v[k][0] = f.x; v[k][1] = f.y; v[k][2] = f.z; v[k][3] = f.w;
+            } else {
+              const float2 f = *reinterpret_cast<const float2*>(p);
+              v[k][0] = f.x; v[k][1] = f.y;
+            }
+          }
+        }
+  #pragma unroll
+        for (int k = 0; k < kMany; ++k) {
+          if (k < n) {
+  #pragma unroll
+            for (int e = 0; e < kLane; ++e) acc[e] = fmaf(wv[k], v[k][e], acc[e]);
+            lsum = fmaf(wv[k], lv[k], lsum);
           }
         }
       }
-#pragma unroll
-      for (int k = 0; k < kMany; ++k) {
-        if (k < n) {
-#pragma unroll
-          for (int e = 0; e < kLane; ++e) acc[e] = fmaf(wv[k], v[k][e], acc[e]);
-          lsum = fmaf(wv[k], lv[k], lsum);
-        }
-      }
     }
-  }
-  const float inv = lsum > 0.f ? 1.0f / lsum : lsum != lsum ? lsum : 0.f;
-  const int tok = r * a.hpg_recip >> 16;
-  T* o = static_cast<T*>(a.out) + (t.tok0 + tok) * a.out_stride +
-         (kv * a.hpg + r - tok * a.hpg) * HD + d0;
-  uint32_t h[kLane / 2];
-#pragma unroll
-  for (int e = 0; e < kLane / 2; ++e) h[e] = pack2<T>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
-  if constexpr (kLane == 4)
-    *reinterpret_cast<uint2*>(o) = make_uint2(h[0], h[1]);
-  else
-    *reinterpret_cast<uint32_t*>(o) = h[0];
+    const float inv = lsum > 0.f ? 1.0f / lsum : lsum != lsum ? lsum : 0.f;
+    const int tok = r * a.hpg_recip >> 16;
+    T* o = static_cast<T*>(a.out) + (t.tok0 + tok) * a.out_stride +
+           (kv * a.hpg + r - tok * a.hpg) * HD + d0;
+    uint32_t h[kLane / 2];
+  #pragma unroll
+    for (int e = 0; e < kLane / 2; ++e) h[e] = pack2<T>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+    if constexpr (kLane == 4)
+      *reinterpret_cast<uint2*>(o) = make_uint2(h[0], h[1]);
+    else
+      *reinterpret_cast<uint32_t*>(o) = h[0];
   }
 }
 
@@ -1277,8 +1301,9 @@ void launch(const PagedAttnArgs& a, const PagedMaps& m, cudaStream_t s) {
   launch_pdl(paged_attention_kernel<HD, T>, dim3(a.ctas, Shape<HD>::kHalves), dim3(kThreads),
              Shape<HD>::kSmem, s, m, a);
   if (a.ctas > 1)
-    launch_pdl(paged_merge_kernel<HD, T>, dim3(a.ctas - 1, merge_split(static_cast<int64_t>(a.max_tiles) * a.c.kv_heads)), dim3(32 * kMergeWarps), 0,
-               s, a);
+    launch_pdl(paged_merge_kernel<HD, T>,
+               dim3(a.ctas - 1, merge_split(static_cast<int64_t>(a.max_tiles) * a.c.kv_heads)),
+               dim3(32 * kMergeWarps), 0, s, a);
 }
 
 template <int HD>
@@ -1305,25 +1330,39 @@ void paged_attention_setup_device() {
                        static_cast<int>(kPlanSmemMax));
 }
 
-size_t paged_attention_layout(PagedAttnArgs* a, int num_sms) {
+bool paged_attention_shape(PagedAttnArgs* a) {
   const int groups = std::max(a->b.n_groups, 1);
   a->hpg = a->heads / a->c.kv_heads;
   a->tpt = kRows / a->hpg;
   a->hpg_recip = (65536 + a->hpg - 1) / a->hpg;
   const int64_t tiles = (static_cast<int64_t>(a->b.tokens) + a->tpt - 1) / a->tpt +
                         std::min<int64_t>(groups, a->b.tokens);
-  if (plan_smem_ints(a->b.n_seqs, groups, tiles) * 4 > kPlanSmemMax) return 0;
+  if (plan_smem_ints(a->b.n_seqs, groups, tiles) * 4 > kPlanSmemMax) return false;
   a->max_tiles = static_cast<int>(tiles);
+  // Units of the line are 32-bit numbers, so are the slots of a row tile: a
+  // bound on them from the tables' widths. A run is a pair of a sequence and a
+  // row tile that holds some of it.
+  auto key_tiles = [&](int64_t pages) { return (pages << a->c.page_log2) / kKeys + 2; };
+  const int64_t runs = a->b.n_seqs + tiles;
+  const int64_t line = runs * key_tiles(a->b.max_pages) +
+                       tiles * (kToll + (a->b.n_groups > 0 ? key_tiles(a->b.max_prefix_pages) : 0));
+  if (line > (int64_t(1) << 29) / a->c.kv_heads) return false;
   // One row tile of few runs (a batch of branches of one state, a token each):
-  // planned by every CTA for itself, which spares a launch.
+  // planned by every CTA for itself, which spares a launch. (One state with 12
+  // branches: 26.8 us with the plan kernel, 22.4 without. More than 32 runs
+  // take a second round of loads in every CTA: with up to 160, 7,400 clocks.)
   a->one_tile = a->b.n_groups <= 1 && a->b.tokens <= a->tpt &&
                 std::min(a->b.n_seqs, a->tpt) < one_tile_runs(a->c.hd);
+  return true;
+}
+
+size_t paged_attention_layout(PagedAttnArgs* a, int num_sms) {
   const int per_sm = a->c.hd <= 128 ? 2 : 1;
   a->ctas = std::max(num_sms * per_sm / (a->c.hd == 512 ? 2 : 1), 1);
   const size_t slots = 2 * static_cast<size_t>(a->ctas) * kRows;
+  const size_t tiles = a->max_tiles;
   return align_up(sizeof(PagedPlan)) + align_up(a->ctas * sizeof(PagedStart)) +
-         align_up(tiles * (a->tpt + 1) * sizeof(PagedRun)) +
-         align_up(tiles * sizeof(PagedTile)) + align_up(slots * 8) + slots * a->c.hd * 4;
+         align_up(tiles * (a->tpt + 1) * sizeof(PagedRun)) + align_up(tiles * sizeof(PagedTile)) + align_up(slots * 8) + slots * a->c.hd * 4;
 }
 
 void paged_attention_workspace(PagedAttnArgs* a, void* ws) {

@@ -113,6 +113,23 @@ def test_attentions_refused(kw, text):
     refused(rc, text)
 
 
+# 8 heads over 2 KV heads: 32 tokens to a row tile. The first two fill the plan
+# kernel's shared memory; the others' line of key tiles would pass 2^29.
+@pytest.mark.parametrize("b,tokens", [
+    (dict(n_seqs=30000), 5),
+    (dict(n_seqs=1), 1 << 21),
+    (dict(n_seqs=32, max_pages=1 << 26), 32),
+    (dict(n_seqs=1, max_pages=1 << 20), 1 << 16),
+    (dict(n_seqs=1, max_prefix_pages=1 << 20), 1 << 16),
+])
+def test_batches_past_the_plan_refused(b, tokens):
+    b = batch(**b)
+    rc = L.lib().omg_paged_attention(0, C.byref(cache()), C.byref(b),
+                                     C.byref(attention_args(tokens=tokens)), P, 1 << 40, None)
+    refused(rc, "split the batch")
+    assert L.lib().omg_paged_attention_workspace(0, C.byref(cache()), C.byref(b), tokens, 8) == 0
+
+
 def test_null_structs_and_devices_refused():
     lib = L.lib()
     refused(call_append(device=-1), "device -1")
