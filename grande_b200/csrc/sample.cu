@@ -17,14 +17,22 @@
 // The outcome is discrete, so sums have to be good to well under a border's
 // width: a border of the running sum lies within 2^-24 of u times the total
 // for about one row in 2^24 / vocab, far too often for f32. Weights are
-// 64-bit integers in units of 2^-44 of the largest, from a 64-bit exp2, so all
+// 64-bit integers in units of 2^-43 of the largest, from a 64-bit exp2, so all
 // sums are exact and the same in any order, atomics included.
 //
-// Bound: one read of the logits at HBM rate; above it stands the 64-bit
-// exponential of every element where no top-k cuts the row first.
+// Bound: one read of the logits at HBM rate is the floor; above it stand a
+// sweep per step and, where no top-k cuts the row first, the 64-bit
+// exponential of every element: 30 to 40 issue slots each, f64, integer and
+// compare instructions at half rate. 128 rows of 262,144 f32, top-p: 124 us,
+// 1.1 TB/s (a first read 14 us, counts 24, exponentials and sums 58, the rest
+// the searches between); 64 rows of 56,000 bf16, settings of all kinds: 39 us;
+// 5 rows of 25,000 with a top-k: 14 us, the steps' barriers. Slices up to
+// kSliceBytes stay in shared memory, longer ones are read again: 128 rows of
+// 56,000 bf16 41.0 us against 42.5, 5 rows of 262,144 34.9 against 36.9.
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <climits>
 #include <type_traits>
 
@@ -45,13 +53,15 @@ constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 2944;      // log2 w from 0 to -46 in steps of 1/64
 constexpr int kList = 2048;      // elements the first CTA sorts
-constexpr int kScale = 44;       // weights in units of 2^-44
+constexpr int kScale = 43;       // weights in units of 2^-43
 constexpr int kMaxCluster = 16;
 constexpr int kSliceBytes = 160 * 1024;     // of a row in a CTA's shared memory
 constexpr int kEach = kList / kThreads;     // list entries per thread
 constexpr int kRankSort = 256;              // lists up to this are sorted by counting
 constexpr u64 kDropped = 1ull << 63;        // list entries that a filter took out
-constexpr int kSubBits = 11;     // refinement: up to 2^11 bins of the (value, index) order
+constexpr int kSubBits = 11;  // refinement: up to 2^11 bins of the (value, index) order
+
+enum { kCount, kMass, kGuess };  // what a histogram's search sums
 
 // The crossing bin of a search: what lies before it, what it holds, and the
 // target (counts or masses).
@@ -75,9 +85,11 @@ struct Shared {
   u64 red[kWarps];
   unsigned redc[kWarps];
   float redf[kWarps];
+  u64 runs[kWarps], above[kWarps];
+  int window_lo, window_hi;
   // Read by the other CTAs of the cluster.
-  u64 best, part_mass, lo, hi;
-  float top;
+  u64 part_mass, part_above, lo, hi;
+  float top, part_sq;
   unsigned part_cnt, list_n;
   Found found;
   u64 threshold;
@@ -108,9 +120,11 @@ __device__ __forceinline__ float value_of(u64 comp) {
 
 // Bin and weight of a value. The bin is -64 log2 w rounded, in f32: monotone
 // in the value, which is all that the search needs of it. The weight is
-// 2^44 w rounded, from 64 bits: 2^(44 - bin / 64) from a table and
+// 2^43 w rounded, from 64 bits: 2^(43 - bin / 64) from a table and
 // 2^(r / 64), r what the bin's rounding left (|r| < 0.51), a polynomial of
-// degree 4 in (ln 2 / 64)^k / k! r^k, good to 2^-44.
+// degree 4 in (ln 2 / 64)^k / k! r^k, good to 2^-44 of the weight.
+__device__ __forceinline__ u64 whole_number(double x) { return __double2ull_rz(x); }
+
 struct Weigher {
   float best, c64;      // the row's largest; 64 log2(e) / T
   double bestd, c64d;
@@ -118,7 +132,9 @@ struct Weigher {
 
   static constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: units of 1
   // The bin as kMagic - bin; a weight below 2^-45.5 lies below kLast.
-  static constexpr float kLast = kMagic - 2912.0f;
+  static constexpr int kLastBin = 2912;
+  static constexpr float kLast = kMagic - kLastBin;
+  static constexpr float kFloor = kMagic - (kBins - 1);
   __device__ __forceinline__ float mark(float x) const { return fmaf(x - best, c64, kMagic); }
   static __device__ __forceinline__ int bin_of_mark(float m) {
     return 0x4B400000 - __float_as_int(m);
@@ -130,18 +146,31 @@ struct Weigher {
   __device__ __forceinline__ u64 weight(float x, unsigned bin) const {
     return weight(x, bin, table[bin]);
   }
-  // `b`: 2^(44 - bin / 64), the table's entry.
+  // The weight as a double, of a finite x and its mark, at least kFloor; the
+  // table is 0 past kLastBin. (Integer instructions run at half the rate of
+  // f32 ones, as f64 ones do: a sum of doubles below 2^53 costs half of a
+  // 64-bit integer's, a maximum less than the selects it spares.)
+  __device__ __forceinline__ double mass(float x, float m) const {
+    const int bits = __float_as_int(m);
+    const double db = 4503599627370496.0 + 0x4B400000 - __hiloint2double(0x43300000, bits);
+    return power(x, db, table[0x4B400000 - bits]) - 4503599627370496.0;
+  }
+  // `b`: 2^(43 - bin / 64), the table's entry.
   __device__ __forceinline__ u64 weight(float x, unsigned bin, double b) const {
     // The bin as a double, through the low bits of 2^52.
     const double db = __hiloint2double(0x43300000, bin) - 4503599627370496.0;
+    const double w = power(x, db, b);
+    return (static_cast<u64>(__double2hiint(w) - 0x43300000) << 32) |
+           static_cast<unsigned>(__double2loint(w));
+  }
+  // The weight + 2^52: rounded, its bits in the low word.
+  __device__ __forceinline__ double power(float x, double db, double b) const {
     const double r = fma(static_cast<double>(x) - bestd, c64d, db);
     constexpr double l = 1.0830424696249145e-2;  // ln 2 / 64
     double p = fma(r, l * l * l * l / 24, l * l * l / 6);
     p = fma(p, r, l * l / 2);
     p = fma(p, r, l);
-    const double w = fma(b * r, p, b) + 4503599627370496.0;
-    return (static_cast<u64>(__double2hiint(w) - 0x43300000) << 32) |
-           static_cast<unsigned>(__double2loint(w));
+    return fma(b * r, p, b) + 4503599627370496.0;
   }
 };
 
@@ -382,6 +411,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
       uint4 b[U];
 #pragma unroll
       for (int k = 0; k < U; ++k) b[k] = p[k * step];
+      p += U * step;
 #pragma unroll
       for (int k = 0; k < U; ++k) {
         float v[kVec];
@@ -389,7 +419,6 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
         f(i, v);
         i += step * kVec;
       }
-      p += U * step;
     }
     // What is cut or left over: blocks [first, lo) and [at, last).
     const int at = lo + rounds * U * step, count = (lo - first) + (last - at);
@@ -470,8 +499,10 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
     }
   };
   // The first bin at which the running sum (of counts or masses) reaches
-  // `target`; 0: top_p of the mass.
-  auto find = [&](bool mass, u64 target) INLINE -> Found {
+  // `target`; 0: top_p of the mass. kGuess: masses as counts times the bin's
+  // weight; *tol is about three deviations of what that misses.
+  auto find = [&](int of, u64 target, u64* tol) INLINE -> Found {
+    const bool mass = of == kMass;
     sync();
     const int share = kBins / C;  // C divides it
     const int each = (share + kThreads - 1) / kThreads;
@@ -515,13 +546,36 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
         mt += m[e];
       }
     }
+    if (of == kGuess) {
+      float sq = 0.0f;
+      mt = 0;
+#pragma unroll
+      for (int e = 0; e < kMost; ++e) {
+        const int b = tid * each + e;
+        if (e < each && b < share)
+          m[e] = static_cast<u64>(static_cast<double>(m[e]) * sh.table[rank * share + b]);
+        const float x = static_cast<float>(m[e]);
+        sq = fmaf(x, x, sq);
+        mt += m[e];
+      }
+      sq = warp_sum(sq);
+      if (lane == 0) sh.redf[warp] = sq;
+    }
     unsigned none = 0, ntot;
     u64 mx = mt, mtot;
     block_scan(sh, none, mx, &ntot, &mtot);
+    if (of == kGuess && warp == 0) {
+      const float sq = warp_sum(sh.redf[lane]);
+      if (lane == 0) sh.part_sq = sq;
+    }
     if (tid == 0) sh.part_mass = mtot;
     sync();
     const u64 part = lane < C ? peer(lane).part_mass : 0;
     const u64 all = warp_sum64(part);
+    if (of == kGuess) {
+      const float sq = warp_sum(lane < C ? peer(lane).part_sq : 0.0f);
+      *tol = static_cast<u64>(0.0094f * sqrtf(sq) + 5e-5f * static_cast<float>(all));
+    }
     mx += warp_sum64(lane < rank ? part : 0);
     if (target == 0) target = ceil_part(top_p, all);
 #pragma unroll
@@ -619,7 +673,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
       sweep(heavy, [&](int i, const float(&v)[kVec]) INLINE { tally(i, v, false); });
     else
       sweep(one, [&](int i, const float(&v)[kVec]) INLINE { tally(i, v, true); });
-    Found f = find(mass, mass ? 0 : count);
+    Found f = find(mass ? kMass : kCount, mass ? 0 : count, nullptr);
     const u64 target = f.target;
     *goal = target;
     const int bin = f.bin;
@@ -687,7 +741,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
             add(static_cast<int>((order_of(v[q], i + q) - lo) >> shift),
                 mass ? weight_of(v[q], bin) : 0, mass);
       });
-      f = find(mass, target - above);
+      f = find(mass ? kMass : kCount, target - above, nullptr);
       above += f.above;
       lo += static_cast<u64>(f.bin) << shift;
       hi = min(hi, lo + (1ull << shift) - 1);
@@ -772,9 +826,214 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
 
   // (Lists compute the few entries they need.)
   if (k > kList)
-    for (int i = tid; i < kBins; i += kThreads) sh.table[i] = exp2(kScale - i / 64.0);
+    for (int i = tid; i < kBins; i += kThreads)
+      sh.table[i] = i <= Weigher::kLastBin ? exp2(kScale - i / 64.0) : 0.0;
   u64 limit = ~0ull, goal = 0;
   int listed = -1;
+  bool summed = false;  // sh.runs holds the warps' kept mass
+  const int run = (blocks + kWarps - 1) / kWarps;
+  const int r0 = min(warp * run, blocks), r1 = min(r0 + run, blocks);
+
+  // top-p of a whole row. Counts times the bins' weights say within about a
+  // bin where the mass is reached; one sweep then sums all that is above that
+  // window, per warp as the draw wants it, and lists what is in it. One
+  // exponential per element instead of two, and no 64-bit atomics: 128 rows of
+  // 262,144 124 us, the histogram of masses below 157. False: the guess was
+  // wrong, or more elements are in the window than the list holds (many equal
+  // logits).
+  auto window_search = [&]() INLINE -> bool {
+    clear_hist(false);
+    sweep(light, [&](int, const float(&v)[kVec]) INLINE {
+#pragma unroll
+      for (int q = 0; q < kVec; ++q) {
+        const float m = wt.mark(v[q]);
+        if (m >= Weigher::kLast) atomicAdd(&sh.h.cnt[Weigher::bin_of_mark(m)], 1u);
+      }
+    });
+    u64 tol = 0;
+    const Found f = find(kGuess, 0, &tol);
+    if (!f.ok) return false;
+    if (warp == 0) {
+      // Bins on both sides, a lane each, until they hold `tol` beyond the
+      // target.
+      auto count_of = [&](int b) INLINE -> unsigned {
+        unsigned c = 0;
+        if (b >= 0 && b < kBins)
+          for (int r = 0; r < C; ++r) c += peer(r).h.cnt[b];
+        return c;
+      };
+      auto reach = [&](int dir, u64 held, unsigned* count) INLINE -> int {
+        const int b = f.bin + dir * (1 + lane);
+        unsigned c = count_of(b);
+        u64 m = c ? static_cast<u64>(c * sh.table[b]) : 0;
+        u64 before = m;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const u64 y = __shfl_up_sync(0xffffffffu, before, o);
+          if (lane >= o) before += y;
+        }
+        const bool in = held + before - m < tol;
+        *count += __reduce_add_sync(0xffffffffu, in ? c : 0u);
+        return __popc(__ballot_sync(0xffffffffu, in));
+      };
+      unsigned count = count_of(f.bin);
+      const int up = reach(-1, f.target - f.above, &count);
+      const int down = reach(1, f.above + f.here - f.target, &count);
+      if (lane == 0) {
+        sh.window_lo = f.bin - up;
+        sh.window_hi = count <= kList ? f.bin + down : -1;
+      }
+    }
+    sync();  // the list takes the histograms' place
+    if (sh.window_hi < 0) return false;
+    const float top_mark = Weigher::kMagic - static_cast<float>(sh.window_lo);
+    const float low_mark = fmaxf(Weigher::kMagic - static_cast<float>(sh.window_hi), Weigher::kLast);
+    Shared& head = peer(0);
+    double dall = 0, dabove = 0, dkept = 0;  // of at most 2^10 weights: below 2^53
+    sweep_run(r0, r1, 32, heavy, [&](int i, const float(&v)[kVec]) INLINE {
+#pragma unroll
+      for (int q0 = 0; q0 < kVec; q0 += 2) {
+        float m[2];
+        double w[2];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const float x = fmaxf(v[q0 + q], -FLT_MAX);
+          m[q] = fmaxf(wt.mark(x), Weigher::kFloor);
+          w[q] = wt.mass(x, m[q]);
+        }
+        bool any = false;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          dall += w[q];
+          if (m[q] > top_mark) dabove += w[q];
+          any |= m[q] <= top_mark && m[q] >= low_mark;
+        }
+        if (min_p > 0.0f) {
+#pragma unroll
+          for (int q = 0; q < 2; ++q)
+            if (m[q] > top_mark && w[q] >= min_w) dkept += w[q];
+        }
+        if (any) {
+#pragma unroll
+          for (int q = 0; q < 2; ++q)
+            if (m[q] <= top_mark && m[q] >= low_mark) {
+              const unsigned at = atomicAdd(&head.list_n, 1u);
+              if (at < kList) head.l.comp[at] = order_of(v[q0 + q], i + q0 + q);
+            }
+        }
+      }
+    });
+    u64 all = warp_sum64(whole_number(dall)), above = warp_sum64(whole_number(dabove));
+    const u64 kept = min_p > 0.0f ? warp_sum64(whole_number(dkept)) : above;
+    if (lane == 0) {
+      sh.red[warp] = all;
+      sh.above[warp] = above;
+      sh.runs[warp] = kept;
+    }
+    __syncthreads();
+    all = warp_sum64(sh.red[lane]);
+    above = warp_sum64(sh.above[lane]);
+    if (tid == 0) {
+      sh.part_mass = all;
+      sh.part_above = above;
+    }
+    sync();
+    if (rank == 0) {
+      const u64 target = ceil_part(top_p, warp_sum64(lane < C ? peer(lane).part_mass : 0));
+      u64 above_all = warp_sum64(lane < C ? peer(lane).part_above : 0);
+      const int got = min(static_cast<int>(sh.list_n), kList);
+      // Their masses by order, in kList steps of the orders' range, and the
+      // few of the crossing step sorted.
+      u64 c[kEach], w[kEach];
+      u64 mn = ~0ull, mx = ~0ull;  // mx: the complement's least
+      __syncthreads();
+      for (int e = 0; e < kEach; ++e) {
+        const int i = tid + e * kThreads;
+        c[e] = i < got ? sh.l.comp[i] : ~0ull;
+        w[e] = 0;
+        sh.l.w[i] = 0;
+        if (i < got) {
+          const float v = value_of(c[e]);
+          w[e] = weight_of(v, bin_of(v));
+          mn = min(mn, c[e]);
+          mx = min(mx, ~c[e]);
+        }
+      }
+      mn = warp_min64(mn);
+      mx = warp_min64(mx);
+      if (lane == 0) {
+        sh.red[warp] = mn;
+        sh.above[warp] = mx;
+      }
+      if (tid == 0) sh.list_n = 0;
+      __syncthreads();
+      mn = warp_min64(sh.red[lane]);
+      mx = ~warp_min64(sh.above[lane]);
+      const int shift = max(0, 64 - __clzll(static_cast<long long>(mx - mn)) - kSubBits);
+      static_assert(1 << kSubBits == kList, "a step per list entry");
+      for (int e = 0; e < kEach; ++e)
+        if (w[e]) atomicAdd(&sh.l.w[(c[e] - mn) >> shift], w[e]);
+      __syncthreads();
+      u64 m[kEach];
+      u64 at = 0, tot;
+      unsigned none = 0, nt;
+      for (int e = 0; e < kEach; ++e) {
+        m[e] = sh.l.w[kEach * tid + e];
+        at += m[e];
+      }
+      if (tid == 0) sh.found.ok = 0;
+      block_scan(sh, none, at, &nt, &tot);
+      at += above_all;
+      for (int e = 0; e < kEach; ++e) {
+        if (at < target && at + m[e] >= target) {
+          sh.found.ok = 1;
+          sh.found.bin = kEach * tid + e;
+          sh.found.above = at;
+        }
+        at += m[e];
+      }
+      __syncthreads();
+      if (sh.found.ok) {  // (else the guess was wrong)
+        for (int e = 0; e < kEach; ++e)
+          if (w[e] && static_cast<int>((c[e] - mn) >> shift) == sh.found.bin)
+            sh.l.comp[atomicAdd(&sh.list_n, 1u)] = c[e];
+        __syncthreads();
+        const int few = sh.list_n;
+        sort_list(sh, few);
+        at = 0;
+        for (int e = 0; e < kEach; ++e) {
+          const int i = kEach * tid + e;
+          m[e] = i < few ? list_weight(sh.l.comp[i]) : 0;
+          at += m[e];
+        }
+        none = 0;
+        block_scan(sh, none, at, &nt, &tot);
+        at += sh.found.above;
+        for (int e = 0; e < kEach; ++e) {
+          if (at < target && at + m[e] >= target) sh.threshold = sh.l.comp[kEach * tid + e];
+          at += m[e];
+        }
+        if (tid == 0) sh.list_n = 0;
+        __syncthreads();
+      }
+      // Those of the window that stay, to the runs that they lie in.
+      for (int e = 0; e < kEach; ++e) {
+        if (w[e] && c[e] <= sh.threshold && static_cast<double>(w[e]) >= min_w) {
+          const int idx = static_cast<int>(c[e] & 0xffffffffu);
+          const int r = idx / per, first = r * per;
+          const int cut = static_cast<int>(
+              (reinterpret_cast<uintptr_t>(src + first) & 15) / sizeof(T));
+          const int all_blocks = (cut + min(per, a.vocab - first) + kVec - 1) / kVec;
+          const int of_warp = (idx - first + cut) / kVec / ((all_blocks + kWarps - 1) / kWarps);
+          atomicAdd(&peer(r).runs[of_warp], w[e]);
+        }
+      }
+    }
+    sync();
+    limit = peer(0).threshold;
+    sync();
+    return limit != ~0ull;
+  };
   if (k != INT_MAX) {
     limit = search(false, k, limit, &listed, &goal);
     if (listed >= 0) {
@@ -783,7 +1042,8 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
       return;
     }
   }
-  if (top_p < 1.0f) {
+  if (top_p < 1.0f && k == INT_MAX) summed = window_search();
+  if (top_p < 1.0f && !summed) {
     limit = search(true, UINT_MAX, limit, &listed, &goal);
     if (listed >= 0) {
       if (rank == 0) finish_list(listed, goal);
@@ -807,8 +1067,6 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
     const u64 w = weight_of(v, bin_of(v));
     return static_cast<double>(w) >= min_w ? w : 0;
   };
-  const int run = (blocks + kWarps - 1) / kWarps;
-  const int r0 = min(warp * run, blocks), r1 = min(r0 + run, blocks);
   float* queue = sh.queue[warp][0];
   u64 mine = 0;
   int waiting = 0;
@@ -819,7 +1077,9 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
     waiting = 0;
   };
   __syncthreads();  // the queues take the histograms' place
-  if (limit == ~0ull)
+  if (summed)
+    ;
+  else if (limit == ~0ull)
     sweep_run(r0, r1, 32, heavy, [&](int i, const float(&v)[kVec]) INLINE {
 #pragma unroll
       for (int q = 0; q < kVec; ++q) mine += bin_of(v[q]) >= 0 ? weigh(v[q]) : 0;
@@ -833,7 +1093,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
       }
     });
   flush();
-  mine = warp_sum64(mine);
+  mine = summed ? sh.runs[warp] : warp_sum64(mine);
   if (lane == 0) sh.red[warp] = mine;
   __syncthreads();
   const u64 of_warp = sh.red[lane];
@@ -935,7 +1195,7 @@ void set_attributes() {
 
 }  // namespace
 
-int sample_max_vocab(int) { return 1 << 19; }  // sums of 2^19 weights of 2^44 fit 64 bits
+int sample_max_vocab(int) { return 1 << 19; }  // (sums by thread stay below 2^53)
 
 void sample_setup_device() {
   set_attributes<float, true>();

@@ -1,7 +1,7 @@
 """Sampling against a plain 64-bit form: tokens equal, probabilities to f32
-rounding (2^-24) and the 2^-44 units that weights are counted in (2^-44 of
-the largest weight over a probability's own: below 2^-22 relative for any
-token above 2^-22 of it, and 2^-43 absolute)."""
+rounding (2^-24) and the 2^-43 units that weights are counted in (half of one,
+2^-44 of the largest weight, over a probability's own: below 2^-22 relative for
+any token above 2^-22 of it, and 2^-43 absolute)."""
 import numpy as np
 import pytest
 
@@ -83,6 +83,30 @@ def test_largest_vocabularies(device, torch, ops, dtype, vocab):
             for r in range(0, 90, 29):
                 one = ops.sample(x[r:r + 1], u[r:r + 1], top_p=0.9)
                 assert one[0] == whole[0][r] and one[1] == whole[1][r]
+
+
+@pytest.mark.parametrize("rows,vocab,dtype", [
+    (1, 30000, "f32"), (3, 150001, "bf16"), (20, 60000, "f16"), (80, 45003, "f32"), (2, 70000, "f32")])
+@pytest.mark.parametrize("shape", ["flat", "even", "wide", "peak", "two", "steps", "holes"])
+def test_top_p_of_whole_rows(device, torch, ops, rows, vocab, dtype, shape):
+    """Where the mass is reached: among a few of thousands of logits of a kind,
+    beside one or two that hold most of it, among equal ones, between rows of
+    -infinity and NaN; alone and with min-p."""
+    x = logits(torch, rows, vocab, 5, device, "f32",
+               {"flat": 0.004, "even": 0.8, "peak": 0.8, "two": 1.5}.get(shape, 6.0), 0)
+    if shape == "peak":
+        x[:, 77] = np.log(vocab) + 1.0
+    elif shape == "two":
+        x[:, ::vocab - 1] = np.log(vocab) + 1.5
+    elif shape == "steps":
+        x = (x * 3).round() / 3
+    elif shape == "holes":
+        x[:, ::2] = -np.inf
+        x[:, 1::6] = np.nan
+    x = x.to(getattr(torch, TYPES[dtype]))
+    p = np.resize(np.array([0.9, 0.5, 0.05, 0.999, 0.99999, 0.7], np.float32), rows)
+    check(torch, ops, x, uniforms(rows, 3), top_p=p)
+    check(torch, ops, x, uniforms(rows, 4), top_p=p, min_p=0.02, temperature=0.7)
 
 
 @pytest.mark.parametrize("rows", [1, 3, 40, 75, 200])
