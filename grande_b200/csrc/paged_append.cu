@@ -8,12 +8,12 @@
 // crates/omg-wgpu/src/shaders/qk_prep.wgsl:1-80).
 //
 // Each value is read and written once and costs about ten operations, so HBM
-// bounds it: 12,000 tokens of 8 + 2 x 2 heads of 512 from f32 take 74.7 us,
-// 5.9 TB/s; 16,384 bf16 tokens of 16 + 2 x 4 heads of 128 take 49.5 us, 4.1
+// bounds it: 12,000 tokens of 8 + 2 x 2 heads of 512 from f32 take 70.6 us,
+// 6.3 TB/s; 16,384 bf16 tokens of 16 + 2 x 4 heads of 128 take 45.1 us, 4.5
 // TB/s. At a few tokens the chain of dependent loads does (sequence, length,
-// page): 3.5 us for one. The heads' values are fetched before that chain, as
+// page): 3.2 us for one. The heads' values are fetched before that chain, as
 // they lie in memory so that four blocks fit an SM (values widened at the load
-// hold twice the registers: 66 us for those 16,384 tokens).
+// hold twice the registers: 66 us for those 16,384 tokens, when it was 50).
 //
 // Numerics: everything in f32 and one rounding to the 16-bit outputs, except
 // the angle. position * inv_freq passes 2^17 radians in long contexts, where
@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(kThreads, 4) paged_append_kernel(PagedAppendAr
   constexpr int L = HD / 16;
   constexpr int kUnits = kThreads / L;
   constexpr int HALF = HD / 2;
-  __shared__ float2 rot[kMaxTokens][HALF];
+  __shared__ float2 rot[kMaxTokens][HALF];  // dim 8 l + e at e L + l: no bank conflicts
   __shared__ long long s_row[kMaxTokens];  // cache row of the token, -1: none
   __shared__ int s_pos[kMaxTokens];        // its position
   __shared__ int s_live[kMaxTokens];
@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(kThreads, 4) paged_append_kernel(PagedAppendAr
     const double turns = static_cast<double>(s_pos[k]) * ((i == tid ? freq0 : a.inv_freq[d]) * 0.15915494309189535);
     float sn, cs;
     sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &sn, &cs);
-    rot[k][d] = make_float2(cs, sn);
+    rot[k][(d & 7) * L + (d >> 3)] = make_float2(cs, sn);
   }
   __syncthreads();
   for (int u0 = 0; u0 < nt * nh; u0 += kUnits) {
@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(kThreads, 4) paged_append_kernel(PagedAppendAr
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         if (8 * l + e < a.n_freq) {
-          const float2 r = rot[tt][8 * l + e];
+          const float2 r = rot[tt][e * L + l];
           const float p = v[e] * r.x - z[e] * r.y;
           z[e] = z[e] * r.x + v[e] * r.y;
           v[e] = p;
@@ -221,7 +221,8 @@ __global__ void __launch_bounds__(kThreads, 4) paged_append_kernel(PagedAppendAr
 template <int HD, class TI, class TO>
 void launch(const PagedAppendArgs& a, int num_sms, cudaStream_t s) {
   // Tokens per block: the lookups and barriers are paid once for all of them,
-  // but few blocks leave SMs idle. us with 1, 2, 4, 8 tokens, 8 + 2 x 2 heads
+  // but few blocks leave SMs idle. us with 1, 2, 4, 8 tokens before the
+  // rotations' layout cost them no bank conflicts (5 to 15%), 8 + 2 x 2 heads
   // of 512 from f32: 60 tokens 4.4, 5.2, 7.4, 11.9; 720 tokens 10.5, 9.3, 9.8,
   // 12.3; 12,000 tokens 92, 80, 75, 76. 16 + 2 x 4 bf16 heads of 128: 1,024
   // tokens 7.8, 6.6, 6.4, 7.6; 16,384 tokens 76, 62, 50, 47.
