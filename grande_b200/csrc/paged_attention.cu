@@ -27,10 +27,11 @@
 // keys than a short branch has, and two partial O per CTA go out and back: 64
 // states of up to 2,000 + 20 branches x 31 keys take 90 us, 2.8 TB/s. Long
 // sequences of a few rows each: 123 us for 64 of up to 8,192 keys, 4.4 TB/s.
-// Prompts: the softmax warps, 780 TFLOP/s at head_dim 128 over 8,000 keys and
-// more, 620 for a prompt of 8,192 tokens alone. One state's next token:
-// latency; 13 to 20 us are two launches, the tables' chain of loads, a key tile
-// per CTA and the merge.
+// Prompts: a tile's chain of scores, softmax and product, of which the two CTAs
+// of an SM overlap two (head_dim 128: 1,570 clocks a tile, 512 of them the
+// tensor pipe's): 780 TFLOP/s over 8,000 keys and more, 610 for a prompt of
+// 8,192 tokens alone. One state's next token: latency; 13 to 20 us are two
+// launches, the tables' chain of loads, a key tile per CTA and the merge.
 //
 // Numerics: scores, max, exponentials and sums f32, O accumulated in f32; P
 // enters the second product in the cache's 16-bit type (its rounding is of

@@ -607,7 +607,7 @@ typedef struct {
  * probability that of the kept distribution. A temperature of 0 or less, or
  * NaN: the largest logit, lowest index first, with probability 1. NaN logits
  * count as -infinity; a row of nothing else gets token -1, probability 0.
- * Weights are counted in units of 2^-44 of the largest. */
+ * Weights are counted in units of 2^-43 of the largest. */
 int omg_sample(int device, const omg_sample_args* args, void* stream);
 
 #ifdef __cplusplus
