@@ -81,6 +81,23 @@ def test_attention(device, torch, ops, hd, heads, kvh, name, dtype, page, window
     check_attention(got, q, cache, b, np.float32(scale), window, dtype)
 
 
+@pytest.mark.parametrize("hd,heads,kvh", [(64, 8, 1), (128, 32, 4), (256, 6, 2), (512, 8, 2)])
+@pytest.mark.parametrize("groups", [
+    [(0, [(0, 900)])],                                         # a prompt: row tiles of 1 key tile on
+    [(5 * i, [(i % 4, 1 + i % 3)]) for i in range(400)],       # hundreds of short row tiles
+    [(700, [(0, 300), (3, 1), (90, 77)]), (0, [(1, 1)] * 30)]  # cut by several CTAs each
+], ids=["prompt", "many", "cut"])
+def test_lines_of_many_row_tiles(device, torch, ops, hd, heads, kvh, groups):
+    dev = torch.device("cuda", device)
+    g = torch.Generator(device=dev).manual_seed(hd)
+    b = Batch(groups, 32, np.random.default_rng(hd))
+    cache = make_cache(torch, dev, b, kvh, hd, torch.bfloat16, g)
+    q = torch.randn((b.tokens, heads, hd), generator=g, device=dev).to(cache.dtype)
+    scale = 1.5 / np.sqrt(hd)
+    got = ops.paged_attention(q, cache, b.device(ops, torch, dev), scale=scale)
+    check_attention(got, q, cache, b, np.float32(scale), 0, "bf16")
+
+
 def test_attention_without_groups_equals_one_group_without_prefix(device, torch, ops):
     dev = torch.device("cuda", device)
     g = torch.Generator(device=dev).manual_seed(5)
