@@ -1274,26 +1274,27 @@ void Engine::read_rows(const Packing& p, Want want, float* out) {
 }
 
 void Engine::read_samples(const Packing& p, const RowSampling& s) {
-  // Device rows are in pass order, the caller's in (group, branch, want)
-  // order: settings go in and results come out through out_index.
-  const size_t rows = p.nwanted;
+  // A sample per wanted slot: several may name one device row, each with its
+  // own number and settings.
+  const size_t rows = p.out_index.size() / 2;
   if (!sample_.p) {
-    sample_.alloc(std::max<size_t>(max_rows, 1) * 7 * 4, false);
-    h_sample_.alloc(std::max<size_t>(max_rows, 1) * 7 * 4);
+    sample_.alloc(std::max<size_t>(max_rows, 1) * 8 * 4, false);
+    h_sample_.alloc(std::max<size_t>(max_rows, 1) * 8 * 4);
   }
   float* h = h_sample_.as<float>();
   int32_t* hk = h_sample_.as<int32_t>() + 2 * rows;
-  for (size_t i = 0; i + 1 < p.out_index.size(); i += 2) {
-    const size_t d = p.out_index[i], c = p.out_index[i + 1];
-    h[d] = s.u[c];
-    h[rows + d] = s.temperature ? s.temperature[c] : s.temperature1;
-    hk[d] = s.top_k ? s.top_k[c] : s.top_k1;
-    h[3 * rows + d] = s.top_p ? s.top_p[c] : s.top_p1;
-    h[4 * rows + d] = s.min_p ? s.min_p[c] : s.min_p1;
+  for (size_t i = 0; i < rows; ++i) {
+    const size_t c = p.out_index[2 * i + 1];
+    h[i] = s.u[c];
+    h[rows + i] = s.temperature ? s.temperature[c] : s.temperature1;
+    hk[i] = s.top_k ? s.top_k[c] : s.top_k1;
+    h[3 * rows + i] = s.top_p ? s.top_p[c] : s.top_p1;
+    h[4 * rows + i] = s.min_p ? s.min_p[c] : s.min_p1;
+    hk[3 * rows + i] = static_cast<int32_t>(p.out_index[2 * i]);
   }
   float* dv = sample_.as<float>();
   if (rows) {
-    CUDA_TRY(cudaMemcpyAsync(dv, h, rows * 5 * 4, cudaMemcpyHostToDevice, stream_));
+    CUDA_TRY(cudaMemcpyAsync(dv, h, rows * 6 * 4, cudaMemcpyHostToDevice, stream_));
     SampleArgs a{};
     a.logits = logits_.p;
     a.stride = config.vocab;
@@ -1305,20 +1306,21 @@ void Engine::read_samples(const Packing& p, const RowSampling& s) {
     a.top_k = reinterpret_cast<const int*>(dv + 2 * rows);
     a.top_p = dv + 3 * rows;
     a.min_p = dv + 4 * rows;
-    a.tokens = reinterpret_cast<int*>(dv + 5 * rows);
-    a.probs = dv + 6 * rows;
+    a.row_of = reinterpret_cast<const int*>(dv + 5 * rows);
+    a.tokens = reinterpret_cast<int*>(dv + 6 * rows);
+    a.probs = dv + 7 * rows;
     launch_sample(a, num_sms_, stream_);
     CUDA_TRY(cudaGetLastError());
-    CUDA_TRY(cudaMemcpyAsync(h + 5 * rows, dv + 5 * rows, rows * 2 * 4, cudaMemcpyDeviceToHost,
+    CUDA_TRY(cudaMemcpyAsync(h + 6 * rows, dv + 6 * rows, rows * 2 * 4, cudaMemcpyDeviceToHost,
                              stream_));
   }
   CUDA_TRY(cudaMemcpyAsync(h_status_.p, status_.p, 4, cudaMemcpyDeviceToHost, stream_));
   CUDA_TRY(cudaStreamSynchronize(stream_));
   check_status();
-  const int32_t* tok = h_sample_.as<int32_t>() + 5 * rows;
-  for (size_t i = 0; i + 1 < p.out_index.size(); i += 2) {
-    s.tokens[p.out_index[i + 1]] = tok[p.out_index[i]];
-    if (s.probs) s.probs[p.out_index[i + 1]] = h[6 * rows + p.out_index[i]];
+  const int32_t* tok = h_sample_.as<int32_t>() + 6 * rows;
+  for (size_t i = 0; i < rows; ++i) {
+    s.tokens[p.out_index[2 * i + 1]] = tok[i];
+    if (s.probs) s.probs[p.out_index[2 * i + 1]] = h[7 * rows + i];
   }
 }
 

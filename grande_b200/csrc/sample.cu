@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
   // as -infinity, which nothing keeps.
   const int per = (a.vocab + C - 1) / C;
   const int i0 = min(rank * per, a.vocab), n = min(per, a.vocab - i0);
-  const T* src = static_cast<const T*>(a.logits) + row * a.stride + i0;
+  const T* src = static_cast<const T*>(a.logits) + (a.row_of ? a.row_of[row] : row) * a.stride + i0;
   constexpr int kVec = 16 / sizeof(T);
   const int lead = static_cast<int>((reinterpret_cast<uintptr_t>(src) & 15) / sizeof(T));
   const int blocks = (lead + n + kVec - 1) / kVec;

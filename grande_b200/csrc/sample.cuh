@@ -13,6 +13,7 @@ struct SampleArgs {
   const void* logits;  // [rows] rows of vocab values
   int64_t stride;      // elements between rows
   int rows, vocab;
+  const int* row_of;   // [rows] the logits row of each sampled row; null: in order
   int dtype;           // OpType
   const float* u;      // [rows] in [0, 1)
   // Per-row settings, or null and the one value for all rows.

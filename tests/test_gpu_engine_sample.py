@@ -63,6 +63,19 @@ def test_sampled_rows_equal_the_rows_sampled_on_the_host(device, config, per_row
     eng.close()
 
 
+def test_a_row_wanted_several_times_is_sampled_each_time(device):
+    eng = RefModel(*gemma3(), 37, O.Q8, O.Q8).engine(64, 16, device)
+    groups = [Group([2, 7, 11], [BranchTokens([5, 6, 9], [2, 0, 2, 2]), BranchTokens([3], [0, 0])])]
+    u = np.array([0.05, 0.5, 0.95, 0.4, 0.99, 0.01], np.float32)
+    temperature = np.array([99.0, 1.0, 99.0, 0.0, 50.0, 50.0], np.float32)  # nearly even rows
+    got = eng.sample_groups(groups, u, temperature=temperature)[0].branches
+    rows = [r for b in eng.evaluate_groups(groups, Want.LOGITS)[0].branches for r in b.rows]
+    exp = [sample(r, *x, 0, np.float32(1), np.float32(0)) for r, x in zip(rows, zip(u, temperature))]
+    assert [t for b in got for t in b.tokens] == [t for t, _ in exp]
+    assert exp[0][0] != exp[2][0] and exp[4][0] != exp[5][0]
+    eng.close()
+
+
 def test_a_decoding_loop(device):
     """Two states, three branches: prompts appended and attended, then tokens
     one at a time, the last output through a projection to logits and sampled;
