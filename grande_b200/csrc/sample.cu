@@ -897,8 +897,11 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
         double w[2];
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
+          // The mark of the logit as it is: -infinity and NaN get the floor's,
+          // and with it no weight, at every temperature. (The mark of a finite
+          // stand-in does not at great ones.) x only keeps the product finite.
           const float x = fmaxf(v[q0 + q], -FLT_MAX);
-          m[q] = fmaxf(wt.mark(x), Weigher::kFloor);
+          m[q] = fmaxf(wt.mark(v[q0 + q]), Weigher::kFloor);
           w[q] = wt.mass(x, m[q]);
         }
         bool any = false;
