@@ -126,7 +126,7 @@ __device__ __forceinline__ float value_of(u64 comp) {
 __device__ __forceinline__ u64 whole_number(double x) { return __double2ull_rz(x); }
 
 struct Weigher {
-  float best, c64;      // the row's largest; 64 log2(e) / T
+  float half, c128;     // half of the row's largest; 2 * 64 log2(e) / T
   double bestd, c64d;
   const double* table;
 
@@ -135,7 +135,10 @@ struct Weigher {
   static constexpr int kLastBin = 2912;
   static constexpr float kLast = kMagic - kLastBin;
   static constexpr float kFloor = kMagic - (kBins - 1);
-  __device__ __forceinline__ float mark(float x) const { return fmaf(x - best, c64, kMagic); }
+  // Differences of halves: those of f32's largest values are finite, too.
+  __device__ __forceinline__ float mark(float x) const {
+    return fmaf(fmaf(x, 0.5f, -half), c128, kMagic);
+  }
   static __device__ __forceinline__ int bin_of_mark(float m) {
     return 0x4B400000 - __float_as_int(m);
   }
@@ -466,11 +469,11 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(SampleArgs a) {
     return;
   }
   Weigher wt;
-  wt.best = top;
+  wt.half = 0.5f * top;
   wt.bestd = top;
   // Finite for the least temperatures, too: the largest itself is in bin 0.
   wt.c64d = fmin(64 * 1.4426950408889634 / static_cast<double>(temp), 1e38);
-  wt.c64 = static_cast<float>(wt.c64d);
+  wt.c128 = static_cast<float>(2 * wt.c64d);
   wt.table = sh.table;
   const double min_w = static_cast<double>(min_p) * static_cast<double>(1ull << kScale);
   auto bin_of = [&](float v) INLINE { return wt.bin(v); };

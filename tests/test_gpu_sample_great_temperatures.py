@@ -28,3 +28,21 @@ def test_masked_logits_have_no_weight(device, torch, ops, temperature, rows, voc
         assert tok[2] == -1
         live = torch.isfinite(x)[np.arange(rows), np.maximum(tok, 0)].cpu().numpy()
         assert live[np.arange(rows) != 2].all()
+
+
+@pytest.mark.parametrize("temperature", [3e37, 1e38, 3.4e38])
+@pytest.mark.parametrize("rows,vocab", [(4, 2), (4, 1500), (4, 30000), (90, 1999)])
+def test_logits_of_the_largest_magnitudes(device, torch, ops, temperature, rows, vocab):  # noqa: F811
+    """Finite logits whose differences are beyond f32's largest: their weights
+    are exp of a few at such temperatures. (The largest ones stand at both
+    ends: 6.8e38 / 3.4e38 = 2.)"""
+    x = logits(torch, rows, vocab, vocab, device, "f32", 1.0, hot=0).clamp(-3, 3) * 1e38
+    x[:, 0] = torch.finfo(torch.float32).min
+    x[:, -1] = torch.finfo(torch.float32).max
+    u = uniforms(rows, vocab)
+    u[0] = 0.0  # the first logit, the least of all, where nothing cuts it
+    for kw in (dict(), dict(top_p=0.9), dict(top_p=0.999, min_p=0.001), dict(top_k=9, top_p=0.6),
+               dict(top_k=3000, top_p=0.9)):
+        tok = check(torch, ops, x, u, temperature=temperature, **kw)
+        if not kw and temperature > 5e37:
+            assert tok[0] == 0
