@@ -401,8 +401,8 @@ class Engine:
         wanted logits row: a GroupOutput of SampleOutputs per group, and no
         logits row leaves the GPU. ``uniforms`` holds a number in [0, 1) per
         wanted row in (group, branch, want) order; the settings
-        (:func:`grande_b200.ops.sample`) are a number for all rows or a
-        sequence with one per row."""
+        (:func:`grande_b200.ops.sample`) are a number for all rows, a sequence
+        with one per row, or None (off)."""
         if not groups:
             raise OmgError("empty request")
         req = _Branches(groups)
@@ -410,7 +410,7 @@ class Engine:
         keep, fields = [], []
 
         def per_row(name, v, dtype):
-            if v is not None and np.ndim(v) == 0:
+            if np.ndim(v) == 0:
                 return None, v
             a = np.ascontiguousarray(v, dtype=dtype)
             if a.shape != (nrows,):
@@ -421,9 +421,10 @@ class Engine:
         if np.ndim(uniforms) != 1:
             raise OmgError(f"uniforms: a sequence of {nrows} numbers, one per row")
         u, _ = per_row("uniforms", uniforms, np.float32)
-        for name, v, dtype in (("temperature", temperature, np.float32), ("top_k", top_k, np.int32),
-                               ("top_p", top_p, np.float32), ("min_p", min_p, np.float32)):
-            fields.append(per_row(name, v, dtype))
+        for name, v, off, dtype in (
+                ("temperature", temperature, 1.0, np.float32), ("top_k", top_k, 0, np.int32),
+                ("top_p", top_p, 1.0, np.float32), ("min_p", min_p, 0.0, np.float32)):
+            fields.append((None, off) if v is None else per_row(name, v, dtype))
         s = _lib.RowSamplingC(u, *(f[0] for f in fields), *(f[1] for f in fields))
         tokens = np.empty(nrows, dtype=np.int32)
         probs = np.empty(nrows, dtype=np.float32)
