@@ -409,22 +409,35 @@ class Engine:
         nrows = sum(g.rows() for g in groups)
         keep, fields = [], []
 
+        def numbers(name, v, dtype):
+            a = np.asarray(v)
+            if a.dtype.kind not in "biuf":
+                raise OmgError(f"{name}: numbers expected")
+            if dtype is np.int32 and not ((a == np.trunc(a)) & (np.abs(a, dtype=np.float64) <
+                                                                2.0 ** 31)).all():
+                raise OmgError(f"{name}: whole numbers of 32 bits expected")
+            with np.errstate(over="ignore"):
+                return np.ascontiguousarray(a, dtype=dtype)
+
         def per_row(name, v, dtype):
-            if np.ndim(v) == 0:
-                return None, v
-            a = np.ascontiguousarray(v, dtype=dtype)
+            a = numbers(name, v, dtype)
             if a.shape != (nrows,):
                 raise OmgError(f"{name}: {list(a.shape)} values for {nrows} rows")
             keep.append(a)
-            return a.ctypes.data if nrows else None, 0
+            return a.ctypes.data if nrows else None
 
         if np.ndim(uniforms) != 1:
             raise OmgError(f"uniforms: a sequence of {nrows} numbers, one per row")
-        u, _ = per_row("uniforms", uniforms, np.float32)
+        u = per_row("uniforms", uniforms, np.float32)
         for name, v, off, dtype in (
                 ("temperature", temperature, 1.0, np.float32), ("top_k", top_k, 0, np.int32),
                 ("top_p", top_p, 1.0, np.float32), ("min_p", min_p, 0.0, np.float32)):
-            fields.append((None, off) if v is None else per_row(name, v, dtype))
+            if v is None:
+                fields.append((None, off))
+            elif np.ndim(v) == 0:
+                fields.append((None, numbers(name, v, dtype).item()))
+            else:
+                fields.append((per_row(name, v, dtype), off))
         s = _lib.RowSamplingC(u, *(f[0] for f in fields), *(f[1] for f in fields))
         tokens = np.empty(nrows, dtype=np.int32)
         probs = np.empty(nrows, dtype=np.float32)

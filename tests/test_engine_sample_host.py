@@ -43,3 +43,35 @@ def test_none_is_off(call):
     for groups, u in ((ONE, [0.25]), (THREE, [0.25, 0.5, 0.75])):
         f = call(groups, u, temperature=None, top_k=None, top_p=None, min_p=None)
         assert f.all == (1.0, 0, 1.0, 0.0) and f.rows == {"u": u}
+
+
+def test_numbers_of_any_kind(call):
+    f = call(ONE, np.array([0.25]), temperature=np.float64(0.5), top_k=np.int64(7),
+             top_p=np.float32(0.75), min_p=np.array(0.125))
+    assert f.all == (0.5, 7, 0.75, 0.125)
+    f = call(THREE, [0.25, 0.5, 0.75], temperature=(0, 1, 2), top_k=[3.0, 2.0, 0.0],
+             top_p=np.array([1, 0.5, 1], np.float16), min_p=[0, 0.5, 0])
+    assert f.rows == {"u": [0.25, 0.5, 0.75], "temperature": [0, 1, 2], "top_k": [3, 2, 0],
+                      "top_p": [1, 0.5, 1], "min_p": [0, 0.5, 0]}
+    assert call(ONE, [0.5], temperature=1e300).all[0] == float("inf")
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(top_k=2 ** 32 + 5), "top_k: whole numbers of 32 bits"),
+    (dict(top_k=[2 ** 32 + 5]), "top_k: whole numbers of 32 bits"),
+    (dict(top_k=0.5), "top_k: whole numbers of 32 bits"),
+    (dict(top_k=[1.5]), "top_k: whole numbers of 32 bits"),
+    (dict(top_k=float("nan")), "top_k: whole numbers of 32 bits"),
+    (dict(top_p="a"), "top_p: numbers expected"),
+    (dict(temperature=[None]), "temperature: numbers expected"),
+    (dict(min_p=[0.1, 0.2]), "min_p: .2. values for 1 rows"),
+])
+def test_refused(call, kw, text):
+    with pytest.raises(OmgError, match=text):
+        call(ONE, [0.5], **kw)
+
+
+@pytest.mark.parametrize("u", [None, 0.5, ["a"], [None], [], [0.1, 0.2], [[0.1]]])
+def test_uniforms_refused(call, u):
+    with pytest.raises(OmgError, match="uniforms"):
+        call(ONE, u)
