@@ -51,7 +51,7 @@ def _fail(msg: str):
 def _pack(op: str, s: struct.Struct, *values) -> bytes:
     try:
         return s.pack(*values)
-    except struct.error as e:
+    except (struct.error, OverflowError) as e:
         raise OmgError(f"{op}: an argument is not a number that fits ({e})") from None
 
 
