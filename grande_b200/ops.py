@@ -110,7 +110,8 @@ class PagedBatch:
         """Read the tables back (this waits for the device) and raise on the
         first thing a call over ``cache`` with ``tokens`` query rows could not
         honour: rows out of order, lengths below the query rows' or beyond the
-        tables, pages outside the pool, a page appended to twice."""
+        tables, pages outside the pool, a page appended to twice, or where a
+        prefix or another sequence has tokens."""
         n_pages, page = cache.shape[0], cache.shape[1]
         q, lens, pages = (t.cpu().numpy().astype(np.int64)
                           for t in (self.q_start, self.lens, self.pages))
@@ -120,16 +121,31 @@ class PagedBatch:
         self._lengths("sequence", lens, pages, page, n_pages)
         for s in np.flatnonzero(lens < new):
             _fail(f"PagedBatch: sequence {s} has {lens[s]} tokens, {new[s]} of them new")
-        writes = [pages[s, i] for s in np.flatnonzero(new > 0)
+        # Pages that rows go to, and the first row of each.
+        writes = [(int(pages[s, i]), max(lens[s] - new[s] - i * page, 0))
+                  for s in np.flatnonzero(new > 0)
                   for i in range((lens[s] - new[s]) // page, -(-lens[s] // page))]
-        if len(set(writes)) != len(writes):
+        first = dict(writes)
+        if len(first) != len(writes):
             _fail("PagedBatch: two sequences append to one page")
+        tables = [(lens, pages)]
         if self.group_start is not None:
             gs, plens, ppages = (t.cpu().numpy().astype(np.int64) for t in
                                  (self.group_start, self.prefix_lens, self.prefix_pages))
             if gs[0] != 0 or (np.diff(gs) < 0).any() or gs[-1] != lens.size:
                 _fail(f"PagedBatch: group_start must ascend from 0 to {lens.size}")
             self._lengths("prefix", plens, ppages, page, n_pages)
+            tables.append((plens, ppages))
+        # They have to lie behind all other tokens of their page. (A page may be
+        # shared by several readers.)
+        users = dict.fromkeys(first, 0)
+        for n, ids in tables:
+            held = np.clip(n[:, None] - np.arange(ids.shape[1]) * page, 0, page)
+            for p, rows in zip(ids[held > 0].tolist(), held[held > 0].tolist()):
+                if p in first and rows > first[p]:
+                    users[p] += 1
+                    if users[p] > 1:
+                        _fail(f"PagedBatch: page {p} is appended to and holds other tokens there")
 
     @staticmethod
     def _lengths(what, lens, pages, page, n_pages):
