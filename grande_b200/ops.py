@@ -246,6 +246,8 @@ def paged_append(qkv: torch.Tensor, cache: torch.Tensor, batch: PagedBatch, *, h
     if qkv.get_device() != index or (qkv.dtype is not torch.float32 and
                                      qkv.dtype is not cache.dtype):
         _fail(f"{op}: qkv must be float32 or {cache.dtype} on cuda:{index}")
+    if heads < 1:
+        _fail(f"{op}: heads {heads}")
     width = heads * hd
     if qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.size(1) not in (width, width + 2 * kvh * hd):
         _fail(f"{op}: qkv is {list(qkv.shape)}, expected [tokens, {width + 2 * kvh * hd}] (q, k, v "
