@@ -24,3 +24,112 @@ def test_head_counts_refused(device, torch, ops):  # noqa: F811
         with pytest.raises(ops.OmgError, match=f"paged_append: heads {heads}"):
             ops.paged_append(torch.zeros((1, (heads + 4) * 64), device=dev), cache,
                              b.device(ops, torch, dev), heads=heads)
+
+
+# Up to 148 tokens a block takes one, up to 740 two, beyond that four.
+@pytest.mark.parametrize("tokens", [147, 149, 301, 740, 803, 2501])
+@pytest.mark.parametrize("hd,heads,kvh,src,dtype,rot", [
+    (64, 3, 1, "f32", "f16", 64), (512, 2, 1, "bf16", "bf16", 128), (128, 16, 4, "f16", "f16", 128),
+    (256, 4, 1, "f32", "bf16", 0)])
+def test_appends_of_many_tokens(device, torch, ops, tokens, hd, heads, kvh, src, dtype, rot):  # noqa: F811
+    dev = device_of(torch, device)
+    rng = np.random.default_rng(tokens + hd)
+    g = torch.Generator(device=dev).manual_seed(tokens + hd)
+    # Ragged sequences, empty ones among them, 3 rows of padding.
+    new = []
+    while sum(new) < tokens - 3:
+        new += [0] * int(rng.integers(0, 3)) + [min(int(rng.integers(1, 90)), tokens - 3 - sum(new))]
+    seqs = [(int(rng.integers(0, 300)), n) for n in new]
+    b = Batch([(5000, seqs[::2]), (0, []), (77, seqs[1::2])], 256, rng)
+    cache = torch.randn((b.n_pages, 256, 2, kvh, hd), generator=g, device=dev).to(
+        dtype_of(torch, dtype))
+    before = cache.clone()
+    qkv = torch.randn((tokens, (heads + 2 * kvh) * hd), generator=g, device=dev).to(
+        dtype_of(torch, src))
+    qn, kn = (torch.randn(hd, generator=g, device=dev) * 0.2 for _ in range(2))
+    freq = ops.rope_frequencies(1e4, hd, rot, device=dev)
+    out = torch.full((tokens, heads, hd), 7.0, device=dev, dtype=cache.dtype)
+    ops.paged_append(qkv, cache, b.device(ops, torch, dev), heads=heads, q_norm=qn, k_norm=kn,
+                     norm_offset=1.0, v_norm=True, inv_freq=freq if rot else None, q_scale=0.25,
+                     out=out)
+    exp_q, exp_c = append(host(qkv), host(before), b, heads, host(qn), host(kn), 1.0, 1e-6, True,
+                          freq.cpu().numpy(), 0.25)
+    assert b.tokens == tokens - 3 and (out[b.tokens:] == 7).all()
+    touched = np.zeros(b.n_pages * 256, bool)
+    for s, _, _, rows, i0 in b.sequences():
+        touched[b.rows(b.pages[s], b.lens[s])[i0:]] = True
+    same = (cache.view(torch.int16) == before.view(torch.int16)).flatten(2).all(-1).flatten()
+    assert same.cpu().numpy()[~touched].all()
+
+    def check(got, exp):
+        half = np.roll(exp, hd // 2, -1)  # the other value of each rotated pair
+        tol = U[dtype] * np.abs(exp) + 2.0 ** -20 * (np.abs(exp) + np.abs(half)) + 2.0 ** -25
+        err = np.abs(got - exp)
+        assert (err <= tol).all(), (np.argwhere(err > tol)[:4], err[err > tol][:4])
+
+    check(host(out)[:b.tokens], exp_q)
+    check(host(cache).reshape(-1, 2, kvh, hd)[touched], exp_c.reshape(-1, 2, kvh, hd)[touched])
+
+
+def run_attention(torch, ops, dev, groups, page, hd, heads, kvh, dtype, window, seed, scale=None):  # noqa: F811
+    g = torch.Generator(device=dev).manual_seed(seed)
+    b = Batch(groups, page, np.random.default_rng(seed))
+    cache = make_cache(torch, dev, b, kvh, hd, dtype_of(torch, dtype), g)
+    q = torch.randn((b.tokens, heads, hd), generator=g, device=dev).to(cache.dtype)
+    scale = scale or 1.5 / np.sqrt(hd)
+    got = ops.paged_attention(q, cache, b.device(ops, torch, dev), scale=scale, window=window)
+    check_attention(got, q, cache, b, np.float32(scale), window, dtype)
+
+
+# A row tile holds 128 query heads of a KV head: these hold 33 to 129 runs.
+@pytest.mark.parametrize("hd,heads,kvh", [(64, 2, 2), (128, 3, 1), (256, 2, 1), (512, 1, 1)])
+@pytest.mark.parametrize("prefix", [0, 150])
+@pytest.mark.parametrize("window", [0, 9, 170])
+def test_many_sequences_in_a_row_tile(device, torch, ops, hd, heads, kvh, prefix, window):  # noqa: F811
+    dev = device_of(torch, device)
+    rng = np.random.default_rng(hd + prefix)
+    one = [(int(rng.integers(0, 60)), 1) for _ in range(70)]
+    gaps = [x for s in one for x in [s] + [(4, 0)] * int(rng.integers(0, 4))]
+    some = [(int(rng.integers(0, 60)), int(rng.integers(0, 4))) for _ in range(160)]
+    for i, groups in enumerate([[(prefix, one)], [(prefix, gaps), (20, one[:33])], [(prefix, some)],
+                                [(prefix, one * 2)]]):
+        run_attention(torch, ops, dev, groups, 16, hd, heads, kvh, "f16", window, hd + i)
+
+
+@pytest.mark.parametrize("heads,kvh", [(64, 1), (128, 1), (256, 2), (43, 1), (65, 1), (127, 1)])
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+@pytest.mark.parametrize("groups", [[(70, [(5, 1)])], [(70, [(5, 1), (0, 3), (40, 2)]), (0, [(9, 4)])]],
+                         ids=["one", "some"])
+def test_many_query_heads_of_a_kv_head(device, torch, ops, heads, kvh, hd, groups):  # noqa: F811
+    run_attention(torch, ops, device_of(torch, device), groups, 64, hd, heads, kvh, "bf16", 0, heads + hd)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+@pytest.mark.parametrize("window", [0, 100])
+def test_pages_of_256_rows(device, torch, ops, hd, window):  # noqa: F811
+    run_attention(torch, ops, device_of(torch, device),
+                  [(600, [(255, 1), (256, 1), (30, 260), (0, 1)]), (256, [(511, 2)])], 256, hd, 4, 2,
+                  "f16", window, hd)
+
+
+def test_elements_past_32_bits_of_the_pool(device, torch, ops):  # noqa: F811
+    """A pool of 9.2 GB: its last rows lie past 2^32 elements."""
+    dev = device_of(torch, device)
+    g = torch.Generator(device=dev).manual_seed(8)
+    b = Batch([(30, [(50, 1), (3, 2)])], 16, np.random.default_rng(8))
+    n_pages = 140000  # x 16 rows x 2,048 values
+    cache = torch.empty((n_pages, 16, 2, 4, 256), dtype=torch.float16, device=dev)
+    up = n_pages - b.n_pages
+    assert up * 16 * 2048 > 2 ** 32
+    cache[up:] = make_cache(torch, dev, b, 4, 256, torch.float16, g)
+    dev_b = b.device(ops, torch, dev, pages=b.pages + up, prefix_pages=b.prefix_pages + up)
+    qkv = torch.randn((b.tokens, 16 * 256), generator=g, device=dev)
+    before = cache[up:].clone()
+    q = ops.paged_append(qkv, cache, dev_b, heads=8)
+    _, exp = append(host(qkv), host(before), b, 8, None, None, 0.0, 0.0, False, np.zeros(0), 1.0)
+    used = b.used_rows()
+    got, exp = (x.reshape(-1, 2048)[used] for x in (host(cache[up:]), exp))
+    # Rounded once.
+    assert (np.abs(got - exp) <= U["f16"] * np.abs(exp) + 2.0 ** -25).all()
+    out = ops.paged_attention(q, cache, dev_b, scale=0.05)
+    check_attention(out, q, cache[up:], b, np.float32(0.05), 0, "f16")
