@@ -191,10 +191,13 @@ __device__ int plan_tile(const PagedAttnArgs& a, const int* q, const int* lens, 
       const int y = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += y;
     }
-    const unsigned have = __ballot_sync(0xffffffffu, n > 0);
+    // A sequence without a slot (a length below its query rows, a table of no
+    // pages, a window past it) keeps its run: its rows' own indices are there.
+    const bool here = ta < tb;
+    const unsigned have = __ballot_sync(0xffffffffu, here);
     const int at = n_runs + __popc(have & ((1u << lane) - 1));
     // (No more runs than tokens in a tile, but for tables out of order.)
-    if (n > 0 && at < a.tpt)
+    if (here && at < a.tpt)
       runs[1 + at] = PagedRun{rt, held + slots + upto - n,
                               n,  k0,
                               ke, ((ta - t0) * a.hpg) | (((tb - t0) * a.hpg) << 16),
@@ -869,8 +872,7 @@ __global__ void __launch_bounds__(kThreads, Shape<HD>::kCtasPerSm)
             }
           }
         }
-        // (A row without own keys, whose length is short of its query rows,
-        // sees nothing.)
+        // (A row without a run, by tables out of order, sees nothing.)
         mine = mine && own > INT_MIN / 2;
         if (!warp_wait(&bars[B_S0 + b], (g >> 1) & 1, abort_flag)) {
           ok = false;

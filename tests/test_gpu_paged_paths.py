@@ -133,3 +133,41 @@ def test_elements_past_32_bits_of_the_pool(device, torch, ops):  # noqa: F811
     assert (np.abs(got - exp) <= U["f16"] * np.abs(exp) + 2.0 ** -25).all()
     out = ops.paged_attention(q, cache, dev_b, scale=0.05)
     check_attention(out, q, cache[up:], b, np.float32(0.05), 0, "f16")
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256, 512])
+@pytest.mark.parametrize("window", [0, 7])
+@pytest.mark.parametrize("what", ["no pages", "no tokens", "some without tokens"])
+@pytest.mark.parametrize("seqs", [3, 200])
+def test_rows_without_own_keys_see_the_prefix(device, torch, ops, hd, window, what, seqs):  # noqa: F811
+    """A row sees its group's prefix up to its own position also where its own
+    keys are cut: by a table without pages, or by a length below its query rows
+    (own index -1: the prefix's last token is at its position)."""
+    dev = device_of(torch, device)
+    g = torch.Generator(device=dev).manual_seed(hd)
+    b = Batch([(40, [(0, 1)] * seqs), (0, [(0, 1)]), (21, [(0, 1)] * 2)], 16, np.random.default_rng(hd))
+    cache = make_cache(torch, dev, b, 2, hd, torch.float16, g)
+    q = torch.randn((b.tokens, 4, hd), generator=g, device=dev).half()
+    pages, lens = b.pages, np.array(b.lens)
+    if what == "no pages":
+        pages = b.pages[:, :0]
+    else:
+        lens[::1 if what == "no tokens" else 3] = 0
+    got = host(ops.paged_attention(q, cache, b.device(ops, torch, dev, pages=pages, lens=lens),
+                                   scale=0.1, window=window))
+    # As queries of the prefix alone, or of prefix and own key.
+    flat = host(cache).reshape(-1, 2, 2, hd).astype(np.float64)
+    exp, mag = np.zeros(q.shape), np.zeros(q.shape)
+    for s, plen, grp, rows, _ in b.sequences():
+        pos = plen + lens[s] - 1
+        kv = flat[np.concatenate([b.rows(b.prefix_pages[grp], plen),
+                                  b.rows(b.pages[s], lens[s] if what != "no pages" else 0)])]
+        kv = kv[max(0, pos - window + 1) if window else 0:]
+        for h in range(4 if len(kv) else 0):
+            z = kv[:, 0, h // 2] @ host(q)[rows[0], h].astype(np.float64) * np.float32(0.1)
+            p = np.exp(z - z.max())
+            p /= p.sum()
+            exp[rows[0], h], mag[rows[0], h] = p @ kv[:, 1, h // 2], p @ np.abs(kv[:, 1, h // 2])
+    tol = U["f16"] * np.abs(exp) + (U["f16"] + 2.0 ** -14) * mag + 42 * 2.0 ** -25 * 8
+    err = np.abs(got - exp)
+    assert (err <= tol).all(), (np.argwhere(err > tol)[:5], err[err > tol][:5])
