@@ -2,9 +2,11 @@
 // in the stream may be scheduled while this one drains, runs its prologue
 // (barrier init, TMEM allocation, tensor-map prefetch), and then waits in
 // griddep_wait() until this grid has completed and its writes are visible.
-// Every kernel launched this way calls griddep_wait() before its first read
-// of memory an earlier kernel wrote (and before any global write), and
-// griddep_launch() after its last global write.
+// Every thread of such a kernel that reads memory which an earlier kernel of the
+// stream wrote, or writes global memory, calls griddep_wait() first: what an
+// earlier grid wrote is visible behind that wait and nowhere else, also where
+// that grid is known to have ended. griddep_launch() may come before the last
+// write: the kernel that it lets start waits for the whole of this one.
 #pragma once
 #include <cuda_runtime.h>
 

@@ -1202,25 +1202,17 @@ __global__ void __launch_bounds__(32 * kMergeWarps) paged_merge_kernel(PagedAttn
   constexpr int kMany = 4;                        // ranges summed at a time
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int i = blockIdx.x + 1;
-  PagedPlan plan;
-  PagedStart st;
-  PagedTile t;
-  auto read = [&]() {
-    plan = *a.plan;
-    if (a.one_tile) {
-      const int w = i * plan.per, kv = plan.line ? w / plan.line : 0;
-      st = place(kv, 0, 0, w - kv * plan.line);
-    } else {
-      st = a.starts[i];
-    }
-    t = a.tiles[st.rt];
-  };
-  // A plan of the plan kernel is there before the attention kernel lets this
-  // one start; one that the attention kernel made comes with its end.
-  if (!a.one_tile) read();
   griddep_wait();
   griddep_launch();
-  if (a.one_tile) read();
+  const PagedPlan plan = *a.plan;
+  PagedStart st;
+  if (a.one_tile) {
+    const int w = i * plan.per, kv = plan.line ? w / plan.line : 0;
+    st = place(kv, 0, 0, w - kv * plan.line);
+  } else {
+    st = a.starts[i];
+  }
+  const PagedTile t = a.tiles[st.rt];
   const int per = plan.per, w = i * per;
   if (w >= plan.line * a.c.kv_heads) return;
   const int kv = st.kv, e0 = w - st.pos;  // the row tile's first key tile
