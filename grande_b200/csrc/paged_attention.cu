@@ -35,8 +35,8 @@
 //
 // Numerics: scores, max, exponentials and sums f32, O accumulated in f32; P
 // enters the second product in the cache's 16-bit type (its rounding is of
-// the size of the output's own and averages over keys). A row keeps a
-// reference max and moves it only when exceeded by 2^11.5 (kTau), so P stays
+// the size of the output's own and averages over keys). A row's
+// reference moves only when a score passes it by far (kReach), so that P stays
 // in range and O is rarely rescaled.
 #include <algorithm>
 #include <climits>
@@ -58,8 +58,14 @@ constexpr int kRows = kPagedTileRows;
 constexpr int kQChunk = kRows * 128;   // [128 rows][64 dims]
 constexpr int kKvChunk = kKeys * 128;  // [64 keys][64 dims]
 constexpr int kPBytes = kRows * kKeys * 2;
-constexpr float kTau = 8.0f;           // slack of the reference max, in log2 units x ln 2
-constexpr float kLog2e = 1.4426950408889634f;
+// A row's probabilities are 2^(score - m_ref) before their common division. At
+// a new maximum m_ref is set kLift below it, and again once a score passes
+// m_ref + kReach, so P stays below 2^kReach (f16 holds 2^16). f16's least is
+// 2^-24: without the lift a key below 2^-25 of the largest had no part in O,
+// but in the sum, and 40,000 of them beside a dominant key lost it 1e-3 of
+// their V. With it that is below 2^-33; bf16 has f32's range.
+template <class T> constexpr float kLift = std::is_same<T, __half>::value ? 8.0f : 0.0f;
+template <class T> constexpr float kReach = std::is_same<T, __half>::value ? 15.0f : 11.5f;
 constexpr int kPlanThreads = 1024;  // 32 warps (block_scan)
 constexpr int kThreads = 192;
 // What a row tile costs on the line beside its key tiles, in key tiles: its Q,
@@ -963,10 +969,11 @@ __global__ void __launch_bounds__(kThreads, Shape<HD>::kCtasPerSm)
                            a.scale_log2;
           float alpha = 1.f;
           bool rescale = false;
-          if (mine && mt > m_ref + kTau * kLog2e) {
+          if (mine && mt > m_ref + kReach<T>) {
             rescale = m_ref != -INFINITY;
-            alpha = rescale ? exp2_fast(m_ref - mt) : 0.f;
-            m_ref = mt;
+            const float to = mt - kLift<T>;
+            alpha = rescale ? exp2_fast(m_ref - to) : 0.f;
+            m_ref = to;
           }
           // A row that has seen nothing yet has no reference: its scores are
           // all -infinity, or NaN, which counts (fmaxf drops it).

@@ -171,3 +171,28 @@ def test_rows_without_own_keys_see_the_prefix(device, torch, ops, hd, window, wh
     tol = U["f16"] * np.abs(exp) + (U["f16"] + 2.0 ** -14) * mag + 42 * 2.0 ** -25 * 8
     err = np.abs(got - exp)
     assert (err <= tol).all(), (np.argwhere(err > tol)[:5], err[err > tol][:5])
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("hd,heads", [(64, 128), (128, 128), (256, 64), (512, 64)])
+@pytest.mark.parametrize("at", [0, 20000, 39999])
+def test_many_small_weights_beside_a_large_one(device, torch, ops, dtype, hd, heads, at):  # noqa: F811
+    """40,000 keys of e^-17.5 (2^-25.2) of one key's weight each hold 1e-3 of the
+    sum together. Every row tile's keys are in one or two CTAs' ranges. P of the
+    type: the large one's V is zero, so u per small one, f16 below 2^-14 half of
+    2^-24, of a weight of 2^8 for the largest."""
+    dev = device_of(torch, device)
+    keys, tokens = 40000, 400
+    b = Batch([(keys, [(0, 1)] * tokens)], 256, np.random.default_rng(1))
+    cache = torch.zeros((b.n_pages, 256, 2, 1, hd), device=dev).to(dtype_of(torch, dtype))
+    cache[:, :, 1] = 1.0
+    flat = cache.view(-1, 2, 1, hd)
+    large = int(b.rows(b.prefix_pages[0], keys)[at])
+    flat[large, 0, 0, 0], flat[large, 1] = 5.0, 0.0
+    q = torch.zeros((tokens, heads, hd), device=dev).to(cache.dtype)
+    q[..., 0] = 3.5
+    got = host(ops.paged_attention(q, cache, b.device(ops, torch, dev), scale=1.0))
+    exp = keys * np.exp(-17.5) / (1 + keys * np.exp(-17.5))  # with its own key, without the large one
+    u = U[dtype]
+    tol = 2 * u * exp + 2.0 ** -14 * exp + (keys * 2.0 ** -33 if dtype == "f16" else 0)
+    assert np.abs(got - exp).max() <= tol, (np.abs(got - exp).max(), tol)
