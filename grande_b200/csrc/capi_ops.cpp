@@ -246,8 +246,8 @@ int omg_sample(int device, const omg_sample_args* p, void* stream) {
     SampleArgs a{};
     a.dtype = p->dtype == OMG_TYPE_F32 ? kOpF32 : p->dtype == OMG_TYPE_F16 ? kOpF16 : kOpBf16;
     if (p->rows < 0 || p->rows > (1 << 24)) fail("%s: %d rows", op, p->rows);
-    if (p->vocab < 1 || p->vocab > sample_max_vocab(a.dtype))
-      fail("%s: vocabulary of %d (1 to %d)", op, p->vocab, sample_max_vocab(a.dtype));
+    if (p->vocab < 1 || p->vocab > sample_max_vocab())
+      fail("%s: vocabulary of %d (1 to %d)", op, p->vocab, sample_max_vocab());
     if (p->stride < p->vocab)
       fail("%s: stride %lld < vocabulary %d", op, static_cast<long long>(p->stride), p->vocab);
     if (p->rows == 0) return 0;

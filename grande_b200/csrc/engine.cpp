@@ -1369,8 +1369,8 @@ void Engine::evaluate_groups(const GroupIn* groups, size_t n, Want want, float* 
 
 void Engine::sample_groups(const GroupIn* groups, size_t n, const RowSampling& s,
                            int32_t* sources) {
-  if (config.vocab > sample_max_vocab(kOpF32))
-    fail("sampling from a vocabulary of %d (at most %d)", config.vocab, sample_max_vocab(kOpF32));
+  if (config.vocab > sample_max_vocab())
+    fail("sampling from a vocabulary of %d (at most %d)", config.vocab, sample_max_vocab());
   evaluate(groups, n, Want::Logits, nullptr, 0, sources, &s);
 }
 

@@ -221,11 +221,13 @@ __global__ void __launch_bounds__(kThreads, 4) paged_append_kernel(PagedAppendAr
 template <int HD, class TI, class TO>
 void launch(const PagedAppendArgs& a, int num_sms, cudaStream_t s) {
   // Tokens per block: the lookups and barriers are paid once for all of them,
-  // but few blocks leave SMs idle. us with 1, 2, 4, 8 tokens before the
-  // rotations' layout cost them no bank conflicts (5 to 15%), 8 + 2 x 2 heads
-  // of 512 from f32: 60 tokens 4.4, 5.2, 7.4, 11.9; 720 tokens 10.5, 9.3, 9.8,
-  // 12.3; 12,000 tokens 92, 80, 75, 76. 16 + 2 x 4 bf16 heads of 128: 1,024
-  // tokens 7.8, 6.6, 6.4, 7.6; 16,384 tokens 76, 62, 50, 47.
+  // but few blocks leave SMs idle. us with 1, 2, 4, 8 tokens, 8 + 2 x 2 heads
+  // of 512 from f32: 60 tokens 4.4, 5.1, 7.2, 11.7; 288 tokens 5.0, 5.3, 7.3,
+  // 11.9; 720 tokens 10.0, 8.7, 9.1, 12.0; 3,000 tokens 25.8, 22.3, 24.1, 27.2;
+  // 12,000 tokens 88.7, 74.0, 71.0, 73.2. 16 + 2 x 4 bf16 heads of 128: 512
+  // tokens 4.6, 4.7, 4.9, 6.9; 1,024 tokens 7.1, 5.9, 5.7, 7.0; 6,503 tokens
+  // 30.5, 24.1, 19.1, 19.0; 16,384 tokens 72.5, 57.6, 45.2, 42.5. (8 gains at
+  // the last alone and needs twice the shared memory.)
   const int tb = a.b.tokens <= num_sms ? 1 : a.b.tokens <= 5 * num_sms ? 2 : kMaxTokens;
   launch_pdl(paged_append_kernel<HD, TI, TO>, dim3((a.b.tokens + tb - 1) / tb), dim3(kThreads), 0, s,
              a, tb);

@@ -4,10 +4,11 @@
 //
 // Three launches, two for a single row tile, which the attention kernel plans
 // itself. The plan kernel (one CTA) cuts the query tokens into row tiles and
-// lays their key tiles on one line (paged.cuh). The attention kernel gives every CTA an equal range of the line, whatever it crosses; a
-// row tile inside one CTA's range is finished there, one that several CTAs
-// cross leaves per CTA an unnormalised O and each row's (max, sum), which the
-// merge kernel joins.
+// lays their key tiles on one line (paged.cuh). The attention kernel gives
+// every CTA an equal range of the line, whatever it crosses; a row tile inside
+// one CTA's range is finished there, one that several CTAs cross leaves per
+// CTA an unnormalised O and each row's (reference, sum), which the merge kernel
+// joins.
 //
 // Why all rows of a group in one tile: a prefix key is read from HBM once for
 // all of them, and an M = 128 tensor-core tile costs 16 clocks per key at
@@ -26,11 +27,11 @@
 // (64 KB) takes an SM 3,100 clocks, 90% of the copy rate, but slots hold more
 // keys than a short branch has, and two partial O per CTA go out and back: 64
 // states of up to 2,000 + 20 branches x 31 keys take 90 us, 2.8 TB/s. Long
-// sequences of a few rows each: 123 us for 64 of up to 8,192 keys, 4.4 TB/s.
+// sequences of a few rows each: 122 us for 64 of up to 8,192 keys, 5.0 TB/s.
 // Prompts: a tile's chain of scores, softmax and product, of which the two CTAs
 // of an SM overlap two (head_dim 128: 1,570 clocks a tile, 512 of them the
-// tensor pipe's): 780 TFLOP/s over 8,000 keys and more, 610 for a prompt of
-// 8,192 tokens alone. One state's next token: latency; 13 to 20 us are two
+// tensor pipe's): 770 TFLOP/s over 8,000 keys and more, 610 for a prompt of
+// 8,192 tokens alone. One state's next token: latency; 13 to 19 us are two
 // launches, the tables' chain of loads, a key tile per CTA and the merge.
 //
 // Numerics: scores, max, exponentials and sums f32, O accumulated in f32; P

@@ -1201,7 +1201,7 @@ void set_attributes() {
 
 }  // namespace
 
-int sample_max_vocab(int) { return 1 << 19; }  // (sums by thread stay below 2^53)
+int sample_max_vocab() { return 1 << 19; }  // (sums by thread stay below 2^53)
 
 void sample_setup_device() {
   set_attributes<float, true>();

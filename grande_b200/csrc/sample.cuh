@@ -27,8 +27,8 @@ struct SampleArgs {
   float* probs;        // [rows] or null
 };
 
-// The largest vocabulary of a dtype a call takes.
-int sample_max_vocab(int dtype);
+// The largest vocabulary that a call takes.
+int sample_max_vocab();
 void launch_sample(const SampleArgs& a, int num_sms, cudaStream_t s);
 void sample_setup_device();
 

@@ -72,7 +72,8 @@ class PagedBatch:
     ``pages[s]`` (own token i on page ``i // page``, row ``i % page``). Group g
     is the sequences ``group_start[g]:group_start[g + 1]`` and the
     ``prefix_lens[g]`` tokens before them in ``prefix_pages[g]``; without the
-    three group tensors there are no prefixes. Query rows past the last
+    three group tensors there are no prefixes, with them every sequence is in a
+    group. Query rows past the last
     sequence are padding and stay as they were. The tables are read when the
     kernels run: write a step's lengths into the tensors in place."""
     q_start: torch.Tensor
@@ -240,7 +241,7 @@ def paged_append(qkv: torch.Tensor, cache: torch.Tensor, batch: PagedBatch, *, h
     weights when ``v_norm``; the pairs (d, d + head_dim / 2) of q and k are
     rotated by position * inv_freq[d] (f64, :func:`rope_frequencies`). k and v
     go to their cache rows, q times ``q_scale`` is returned
-    [tokens, heads, head_dim]."""
+    [tokens, heads, head_dim] (``out``, which must not overlap ``qkv``)."""
     op = "paged_append"
     c, index, kvh, hd = _cache(op, cache, batch)
     if qkv.get_device() != index or (qkv.dtype is not torch.float32 and
@@ -274,7 +275,7 @@ def paged_attention(q: torch.Tensor, cache: torch.Tensor, batch: PagedBatch, *,
     cache: each row sees its group's prefix and its own sequence's keys up to
     its own position, the last ``window`` of them if that is not 0. A prefix
     is read once for all the sequences of its group. Rows that see nothing
-    are zero. ``workspace`` (uint8, :func:`paged_attention_workspace` bytes)
+    are zero. ``out`` must not overlap ``q``. ``workspace`` (uint8, :func:`paged_attention_workspace` bytes)
     is allocated from torch's pool when not given."""
     op = "paged_attention"
     c, index, kvh, hd = _cache(op, cache, batch)

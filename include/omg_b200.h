@@ -514,10 +514,12 @@ int omg_gemm_splitk_noalloc(int device, const void* x_f16, int m, int k, int lda
  * pages[s * max_pages + i / page_rows]. Group g is the sequences
  * group_start[g] .. group_start[g + 1] and the prefix_lens[g] tokens before
  * them, in pages prefix_pages[g * max_prefix_pages + ..]: own token i of a
- * sequence is at position prefix_lens[g] + i. n_groups 0 (group arrays NULL):
- * no prefixes. Query rows from q_start[n_seqs] on are padding and their
- * outputs are left as they were. Lengths beyond a table's columns are cut
- * there; page ids outside the pool are never read or written. */
+ * sequence is at position prefix_lens[g] + i, which stays below 2^31 - 1.
+ * n_groups 0 (group arrays NULL): no prefixes; otherwise every sequence is in
+ * one. Query rows from q_start[n_seqs] on are padding and their outputs are
+ * left as they were. Lengths beyond a table's columns are cut there; a length
+ * below a sequence's query rows leaves the first of those at positions before
+ * its own tokens; page ids outside the pool are never read or written. */
 enum { OMG_TYPE_F16 = 0, OMG_TYPE_BF16 = 1, OMG_TYPE_F32 = 2 };
 
 typedef struct {
@@ -550,7 +552,8 @@ typedef struct {
 /* The per-head norms, rotation and scaling of a fused projection row
  * (qk_prep.wgsl), q to q_out, k and v to the token's cache row. A token
  * whose row is outside its table or the pool gets its q row and no cache
- * row. Two tokens of one batch given the same cache row race. */
+ * row. Two tokens of one batch given the same cache row race. q_out must not
+ * overlap qkv. */
 int omg_paged_append(int device, const omg_paged_cache* cache, const omg_paged_batch* batch,
                      const omg_append_args* args, void* stream);
 
@@ -575,8 +578,9 @@ size_t omg_paged_attention_workspace(int device, const omg_paged_cache* cache,
  * pages): a prefix is read once for all the sequences of its group. A row
  * that sees no key gets zeros. Keys and values a row does not see never
  * reach it, whatever they hold; a page id outside the pool reads as zeros.
- * A row whose kernel gave up waiting (a bounded device wait) is NaN. `out`
- * must not overlap q. */
+ * A row whose kernel gave up waiting (a bounded device wait) is NaN. Sums of
+ * V are f32 before they are divided: bf16 values beyond about 2^100 may
+ * overflow them. `out` must not overlap q. */
 int omg_paged_attention(int device, const omg_paged_cache* cache, const omg_paged_batch* batch,
                         const omg_attention_args* args, void* workspace, size_t workspace_bytes,
                         void* stream);
@@ -606,7 +610,8 @@ typedef struct {
  * index order whose running sum of kept w exceeds u times their sum, its
  * probability that of the kept distribution. A temperature of 0 or less, or
  * NaN: the largest logit, lowest index first, with probability 1. NaN logits
- * count as -infinity; a row of nothing else gets token -1, probability 0.
+ * count as -infinity, which has no weight at any temperature, infinity
+ * included; a row of nothing else gets token -1, probability 0.
  * Weights are counted in units of 2^-43 of the largest. */
 int omg_sample(int device, const omg_sample_args* args, void* stream);
 
