@@ -1171,6 +1171,12 @@ __global__ void __launch_bounds__(kThreads, Shape<HD>::kCtasPerSm)
                                          c * 32)[lane & 7] = v[e];
             }
           }
+          // Two CTAs share a row at head_dim 512 and one of them writes its sum:
+          // each that gave up marks its own dims.
+          if (Sh::kHalves > 1 && !ok) {
+            __syncwarp();
+            for (int d = 0; d < VD && valid; ++d) po[static_cast<size_t>(r) * HD + d] = NAN;
+          }
         }
         __syncwarp();
       }
