@@ -275,8 +275,9 @@ def paged_attention(q: torch.Tensor, cache: torch.Tensor, batch: PagedBatch, *,
     cache: each row sees its group's prefix and its own sequence's keys up to
     its own position, the last ``window`` of them if that is not 0. A prefix
     is read once for all the sequences of its group. Rows that see nothing
-    are zero. ``out`` must not overlap ``q``. ``workspace`` (uint8, :func:`paged_attention_workspace` bytes)
-    is allocated from torch's pool when not given."""
+    are zero. ``out`` must not overlap ``q``. ``workspace`` (uint8,
+    :func:`paged_attention_workspace` bytes) is allocated from torch's pool
+    when not given."""
     op = "paged_attention"
     c, index, kvh, hd = _cache(op, cache, batch)
     if q.get_device() != index or q.dtype is not cache.dtype or q.dim() != 3 or q.size(2) != hd:
